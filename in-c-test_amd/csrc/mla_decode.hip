@@ -680,11 +680,11 @@ __device__ __forceinline__ void *lane_pick(void *p, int b) {
 }
 struct DescLane {  // this lane's entry of the table
     void *a, *b, *c;
-    int len, pos, split0, nsplit, rps;
+    int len, pos, split0, nsplit, rps, roff;
 };
 __device__ __forceinline__ DescLane desc_lane(const SeqTable &t) {
     const SeqDesc &m = t.s[threadIdx.x & 63];
-    return DescLane{m.a, m.b, m.c, m.len, m.pos, m.split0, m.nsplit, m.rps};
+    return DescLane{m.a, m.b, m.c, m.len, m.pos, m.split0, m.nsplit, m.rps, m.roff};
 }
 __device__ __forceinline__ SeqDesc desc_pick(const DescLane &m, int i) {
     SeqDesc s;
@@ -696,7 +696,7 @@ __device__ __forceinline__ SeqDesc desc_pick(const DescLane &m, int i) {
     s.split0 = lane_pick(m.split0, i);
     s.nsplit = lane_pick(m.nsplit, i);
     s.rps = lane_pick(m.rps, i);
-    s.pad1 = 0;
+    s.roff = lane_pick(m.roff, i);
     return s;
 }
 
@@ -729,6 +729,7 @@ __device__ __forceinline__ void append_body(const SeqTable &t, const Dims &d, co
     const int tid = threadIdx.x;
     const SeqDesc s = desc_pick(desc_lane(t), a.rows_mode ? 0 : b);
     const int R = d.R, DR = d.DR, half = DR / 2, pos = s.pos + (a.rows_mode ? b : 0);
+    const int hrow = pos + s.roff;  // the history row written
     const int nk = R + DR;
     const float *ky = a.y + (size_t)b * a.ldy + a.koff;
     // All global reads first, so that one memory round trip covers them: the projection row
@@ -770,7 +771,7 @@ __device__ __forceinline__ void append_body(const SeqTable &t, const Dims &d, co
         // reference's sequential `a > amax` scan followed by isfinite() does for Inf; NaN
         // never compares greater there, so it is simply skipped -- identical to fmaxf.
         const float amax = block256_max(m, redf);
-        int8_t *codes = (int8_t *)s.a + (size_t)pos * R;
+        int8_t *codes = (int8_t *)s.a + (size_t)hrow * R;
         const bool zero = !(amax > 0.0f) || !isfinite(amax);
         const float scale = zero ? 1.0f : amax / 127.0f;
         const float inv = zero ? 0.0f : 1.0f / scale;
@@ -786,17 +787,17 @@ __device__ __forceinline__ void append_body(const SeqTable &t, const Dims &d, co
             row_out[r] = (uint8_t)q;
         }
         if (tid == 0) {
-            ((float *)s.b)[pos] = scale;
+            ((float *)s.b)[hrow] = scale;
             *(float *)(row_out + R) = scale;
         }
     } else if (a.fmt == kFmtF32) {
-        float *dst = (float *)s.a + (size_t)pos * R;
+        float *dst = (float *)s.a + (size_t)hrow * R;
         for (int r = tid; r < R; r += 256) {
             dst[r] = lat[r];
             ((float *)row_out)[r] = lat[r];
         }
     } else if (a.fmt == kFmtBF16) {
-        uint16_t *dst = (uint16_t *)s.a + (size_t)pos * R;
+        uint16_t *dst = (uint16_t *)s.a + (size_t)hrow * R;
         for (int r = tid; r < R; r += 256) {
             const uint16_t h = f32_to_bf16_rne(lat[r]);
             dst[r] = h;
@@ -813,7 +814,7 @@ __device__ __forceinline__ void append_body(const SeqTable &t, const Dims &d, co
         const float ec = ev * cs.x, os = od * cs.y, oc = od * cs.x, es = ev * cs.y;
         const float d0 = ec - os, d1 = oc + es;
         if (a.fmt == kFmtQ8) {
-            uint16_t *rp = (uint16_t *)s.c + (size_t)pos * DR;
+            uint16_t *rp = (uint16_t *)s.c + (size_t)hrow * DR;
             const uint16_t h0 = f32_to_bf16_rne(d0), h1 = f32_to_bf16_rne(d1);
             rp[i] = h0;
             rp[half + i] = h1;
@@ -821,14 +822,14 @@ __device__ __forceinline__ void append_body(const SeqTable &t, const Dims &d, co
             ro[i] = h0;
             ro[half + i] = h1;
         } else if (a.fmt == kFmtF32) {
-            float *rp = (float *)s.b + (size_t)pos * DR;
+            float *rp = (float *)s.b + (size_t)hrow * DR;
             rp[i] = d0;
             rp[half + i] = d1;
             float *ro = (float *)row_out + R;
             ro[i] = d0;
             ro[half + i] = d1;
         } else if (a.fmt == kFmtBF16) {
-            uint16_t *rp = (uint16_t *)s.b + (size_t)pos * DR;
+            uint16_t *rp = (uint16_t *)s.b + (size_t)hrow * DR;
             const uint16_t h0 = f32_to_bf16_rne(d0), h1 = f32_to_bf16_rne(d1);
             rp[i] = h0;
             rp[half + i] = h1;

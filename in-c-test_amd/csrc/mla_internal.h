@@ -1,5 +1,5 @@
 // Internal interface between the host runtime (mla_runtime.cpp) and the HIP kernels
-// (mla_decode.hip, mla_prefill.hip) of libkvl_mla. Not installed; the public C ABI is
+// (mla_decode.hip, mla_prefill.hip, mla_tree.hip) of libkvl_mla. Not installed; the public C ABI is
 // include/kvl/*.h.
 #pragma once
 
@@ -41,7 +41,7 @@ struct SeqDesc {
     int split0;
     int nsplit;
     int rps;
-    int pad1;
+    int roff;  // the appended row is row pos + roff (0 but for the nodes of a tree: pos is their RoPE position)
 };
 
 struct SeqTable {
@@ -238,6 +238,54 @@ hipError_t launch_copy(hipStream_t st, void *dst, const void *src, size_t bytes)
 constexpr int kReadBlocks = 8192;
 hipError_t launch_read(hipStream_t st, const void *src, size_t bytes, void *sink);
 hipError_t launch_empty(hipStream_t st);
+
+// ---- trees and rows (mla_tree.hip) ----
+// A tree decode: the nodes of one or more sequences' drafts, each node attending its sequence's
+// history, its ancestors and itself.
+constexpr int kTreeNodes = 64;  // nodes of one tree, and of one launch group
+struct TreeSeq {
+    void *a, *b, *c;  // the history's device arrays (see Fmt); node i's row is row ctx + i
+    int ctx;          // rows of the history
+    int count;        // nodes
+    int node0;        // the tree's first node among the group's
+    int pad;
+};
+struct TreeTable {
+    TreeSeq s[kTreeNodes];
+    int8_t parent[kTreeNodes];  // per node of the group: its parent within its own tree, or -1
+    uint8_t seq[kTreeNodes];    // per node of the group: its sequence
+    int n, nodes;
+};
+// Attention of the group's nodes (queries w.qf) into w.part: node k's partial is split k.
+hipError_t launch_tree_attention(hipStream_t st, int fmt, const TreeTable &t, const Dims &d, const DecodeWork &w);
+
+// Copies of rows [r0, r1) between the device arrays of two states of one format (arrays with
+// e[0..2] bytes a row; 0: none).
+struct ForkDesc {
+    const void *src[3];
+    void *dst[3];
+    int r0, r1;
+};
+constexpr int kForkBatch = 48;
+struct ForkTable {
+    ForkDesc d[kForkBatch];
+    int n;
+    int e[3];
+};
+hipError_t launch_fork(hipStream_t st, const ForkTable &t);
+// Rows start + path[i] to start + i, i < n, path strictly increasing.
+struct AcceptDesc {
+    void *p[3];
+    int start, n;
+    uint8_t path[kTreeNodes];
+};
+constexpr int kAcceptBatch = 32;
+struct AcceptTable {
+    AcceptDesc d[kAcceptBatch];
+    int n;
+    int e[3];
+};
+hipError_t launch_accept(hipStream_t st, const AcceptTable &t);
 
 // ---- prefill (mla_prefill.hip) ----
 // Device workspace bytes of a causal prefill of S tokens (generic: on the generic route).

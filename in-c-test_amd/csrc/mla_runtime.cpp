@@ -16,6 +16,7 @@
 //   * one HIP stream; kernels are enqueued in order, results copied back, then synchronised.
 #include <hip/hip_runtime.h>
 
+#include <limits.h>
 #include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
@@ -23,6 +24,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <exception>
 #include <mutex>
 #include <string>
 #include <unordered_map>
@@ -1872,6 +1874,530 @@ int prefill_state(float *out, const float *x, int seq_len, const KvlMlaConfig *c
     return 0;
 }
 
+// ---------------------------------------------------------------- trees -----------------
+
+// One sequence of a tree decode: its mirror, the rows of its history, its nodes' parents.
+struct TreeIn {
+    Mirror *m;
+    int ctx, count;
+    const int *parents;
+};
+
+// What is wrong with a tree, or null: parents come before their children, -1 is the context.
+const char *tree_fault(const int *parents, int count) {
+    if (count < 1 || count > kTreeNodes) return "a tree has 1 to 64 nodes";
+    for (int i = 0; i < count; ++i)
+        if (parents[i] < -1 || parents[i] >= i) return "a node's parent is -1 or an earlier node";
+    return nullptr;
+}
+
+int tree_depth(const int *parents, int count) {  // of the deepest node, a child of the context: 0
+    int dep[kTreeNodes], most = 0;
+    for (int i = 0; i < count; ++i) {
+        dep[i] = parents[i] < 0 ? 0 : dep[parents[i]] + 1;
+        most = std::max(most, dep[i]);
+    }
+    return most;
+}
+
+// Sequences from g0 on that one launch group takes: at most kTreeNodes nodes.
+int tree_group_end(const int *counts, int batch, int g0) {
+    int n = 0, g = g0;
+    while (g < batch && n + counts[g] <= kTreeNodes) n += counts[g++];
+    return g;
+}
+
+size_t tree_part_bytes(const Dims &d, int nodes) { return (size_t)nodes * d.NH * (d.R + 2) * sizeof(float); }
+
+// One tree decode of a launch group: the steps of decode_group with the group's nodes as its
+// members, each member's row at history row ctx + i and its rotation at position ctx + depth.
+// Everything it needs has been acquired (tree_prepare).
+int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights &dw, const TreeIn *seqs, int n,
+               const float *d_x, float *d_out, bool residual, DecodeWork &w, const InNorm *in_norm = nullptr) {
+    Ctx &c = ctx();
+    hipStream_t st = c.stream;
+    TreeTable tt;
+    SeqTable t;
+    memset(&tt, 0, sizeof tt);
+    memset(&t, 0, sizeof t);
+    int k = 0, maxpos = 0;
+    for (int b = 0; b < n; ++b) {
+        const TreeIn &q = seqs[b];
+        tt.s[b] = {q.m->a, q.m->b, q.m->c, q.ctx, q.count, k, 0};
+        int dep[kTreeNodes];
+        for (int i = 0; i < q.count; ++i, ++k) {
+            dep[i] = q.parents[i] < 0 ? 0 : dep[q.parents[i]] + 1;
+            tt.parent[k] = (int8_t)q.parents[i];
+            tt.seq[k] = (uint8_t)b;
+            SeqDesc &s = t.s[k];
+            s.a = q.m->a;
+            s.b = q.m->b;
+            s.c = q.m->c;
+            s.pos = q.ctx + dep[i];
+            s.roff = i - dep[i];
+            s.split0 = k;
+            s.nsplit = 1;
+            maxpos = std::max(maxpos, s.pos);
+        }
+    }
+    tt.n = n;
+    tt.nodes = t.n = k;
+    const int N = k, ldy = d.QO + d.KVO;
+    const float2 *cs = nullptr;
+    if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
+    if (reserve_part(tree_part_bytes(d, N), &w.part) != 0) return -1;
+    if (in_norm) {
+        HIP_TRY(launch_rmsnorm(st, in_norm->buf, d_x, in_norm->w, d.H, N, eps));
+        d_x = in_norm->buf;
+    }
+    if (gemv_ksplit_ok(d.H, d.H)) {
+        if (((uintptr_t)d_x % 16) != 0) {  // the kernel reads 16-byte vectors
+            HIP_TRY(hipMemcpyAsync(w.x, d_x, (size_t)N * d.H * sizeof(float), hipMemcpyDeviceToDevice, st));
+            d_x = w.x;
+        }
+        w.ynp = kGemvKs;
+        w.ypstride = (size_t)N * ldy;
+        HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
+    } else {
+        w.ynp = 1;
+        w.ypstride = 0;
+        HIP_TRY(launch_gemv(st, w.y, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H, false));
+    }
+    HIP_TRY(launch_append_qprep(st, fmt, t, d, w.y, ldy, d.QO, w.ynp, w.ypstride, dw.norm, eps, cs, dw.kvb, dw.ukt, w,
+                                false));
+    HIP_TRY(launch_tree_attention(st, fmt, tt, d, w));
+    HIP_TRY(launch_combine(st, fmt, t, d, dw.kvb, w));
+    if (combine_writes_hos(fmt, d) && gemv_xs_ok(d.HO))
+        HIP_TRY(launch_gemv_xs(st, d_out, d.H, w.hos, N, dw.o, d.H, d.HO, residual));
+    else
+        HIP_TRY(launch_gemv(st, d_out, d.H, w.ho, d.HO, N, dw.o, d.H, nullptr, 0, d.HO, residual));
+    return 0;
+}
+
+// The library works on the device it was initialised on; its kernels are launched there.
+int on_device() {
+    int dev = -1;
+    HIP_TRY(hipGetDevice(&dev));
+    if (dev != ctx().device) {
+        set_err("current device %d is not the library's device %d", dev, ctx().device);
+        return -1;
+    }
+    return 0;
+}
+
+template <class S>
+bool twice(S *const *states, int n) {
+    std::vector<S *> v(states, states + n);
+    std::sort(v.begin(), v.end());
+    return std::adjacent_find(v.begin(), v.end()) != v.end();
+}
+
+// Checks of a tree decode, for every sequence before anything runs.
+template <class S>
+int tree_check(const int *counts, const int *parents, int batch, const KvlMlaConfig *cfg, S *const *states) {
+    size_t at = 0;
+    for (int i = 0; i < batch; ++i) {
+        const S *s = states[i];
+        if (!s || !state_dims_ok(s, cfg)) {
+            set_err("sequence %d: dims check failed", i);
+            return -1;
+        }
+        const char *f = tree_fault(counts[i] > 0 && counts[i] <= kTreeNodes ? parents + at : nullptr, counts[i]);
+        if (f) {
+            set_err("sequence %d: %s", i, f);
+            return -1;
+        }
+        if (s->len < 0 || s->len > s->capacity || counts[i] > s->capacity - s->len) {
+            set_err("sequence %d: %d nodes behind %d rows exceed the capacity of %d", i, counts[i], s->len, s->capacity);
+            return -1;
+        }
+        at += (size_t)counts[i];
+    }
+    if (at > (size_t)INT_MAX / 2) {
+        set_err("too many nodes");
+        return -1;
+    }
+    if (twice(states, batch)) {
+        set_err("a state stands twice in the batch");
+        return -1;
+    }
+    return 0;
+}
+
+// Acquires what the groups of a tree decode need, so that a failure leaves every state unchanged:
+// the device copies of the states, the RoPE table, the workspace and the partials of the largest group.
+template <class S>
+int tree_prepare(int fmt, const Dims &d, float theta, const int *counts, const int *parents, int batch, S *const *states,
+                 size_t rb, std::vector<TreeIn> &in, int *most) {
+    in.resize(batch);
+    int maxpos = 0;
+    for (int i = 0; i < batch; ++i) {
+        Mirror *m = nullptr;
+        if (mirror_get(states[i], view_of(states[i]), &m) != 0) return -1;
+        in[i] = {m, states[i]->len, counts[i], parents};
+        maxpos = std::max(maxpos, states[i]->len + tree_depth(parents, counts[i]));
+        parents += counts[i];
+    }
+    const float2 *cs = nullptr;
+    if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
+    *most = 0;
+    for (int g = 0; g < batch;) {
+        const int e = tree_group_end(counts, batch, g);
+        int n = 0;
+        for (; g < e; ++g) n += counts[g];
+        *most = std::max(*most, n);
+    }
+    DecodeWork wk;
+    float *pp = nullptr;
+    if (decode_work(d, *most, (int)rb, wk) != 0 || reserve_part(tree_part_bytes(d, *most), &pp) != 0) return -1;
+    return 0;
+}
+
+// A tree decode over host buffers (one sequence), synchronous: outputs, host rows and len written.
+template <class S>
+int tree_host(float *out, const float *x, const int *parents, int count, int start, const KvlMlaConfig *cfg,
+              const KvlMlaBF16 *w, S *state) {
+    Dims d;
+    if (!out || !x || !parents || !state || !weights_ok(w) || !dims_of(cfg, d) || start != state->len) {
+        set_err("invalid arguments");
+        return -1;
+    }
+    S *const st[1] = {state};
+    if (tree_check(&count, parents, 1, cfg, st) != 0) return -1;
+    if (!dims_supported(d)) return -1;
+    if (ensure_ready() != 0 || on_device() != 0) return -1;
+    Ctx &c = ctx();
+    if (c.capturing) {
+        set_err("host-buffer tree decode during graph capture");
+        return -1;
+    }
+    const int fmt = fmt_of<S>();
+    DevWeights dw;
+    if (dev_weights(w, d, dw) != 0) return -1;
+    const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0);
+    std::vector<TreeIn> in;
+    int most = 0;
+    if (tree_prepare(fmt, d, cfg->rope_theta, &count, parents, 1, st, rb, in, &most) != 0) return -1;
+    DecodeWork wk;
+    if (decode_work(d, count, (int)rb, wk) != 0) return -1;
+    const size_t xin = (size_t)count * d.H * sizeof(float);
+    if (pin_reserve(c.pin_in, xin) != 0 || pin_reserve(c.pin_out, xin + count * rb) != 0) return -1;
+    memcpy(c.pin_in.p, x, xin);
+    wk.rows = (uint8_t *)c.pin_out.p + xin;  // as in decode_block: x, outputs and rows in the pinned buffers
+    if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data(), 1, (const float *)c.pin_in.p, (float *)c.pin_out.p,
+                   false, wk) != 0)
+        return -1;
+    HIP_TRY(hipStreamSynchronize(c.stream));
+    memcpy(out, c.pin_out.p, xin);
+    const HostView v = view_of(state);
+    for (int i = 0; i < count; ++i) write_back_rows(fmt, v, start + i, (const uint8_t *)c.pin_out.p + xin + (size_t)i * rb);
+    state->len = start + count;
+    in[0].m->synced = state->len;
+    return 0;
+}
+
+// Stream-ordered tree decode of a batch over device buffers.
+template <class S>
+int tree_device(float *d_out, const float *d_x, const int *counts, const int *parents, int batch, const KvlMlaConfig *cfg,
+                const KvlMlaBF16 *w, S *const *states, unsigned flags, const InNorm *in_norm = nullptr) {
+    Dims d;
+    if (!d_out || !d_x || !counts || !parents || batch <= 0 || !states || !weights_ok(w) || !dims_of(cfg, d)) {
+        set_err("invalid arguments");
+        return -1;
+    }
+    if (flags & ~(unsigned)(KVL_MLA_RESIDUAL | KVL_MLA_NO_ADVANCE)) {
+        set_err("unsupported flags");
+        return -1;
+    }
+    if (tree_check(counts, parents, batch, cfg, states) != 0) return -1;
+    if (!dims_supported(d)) return -1;
+    if (ensure_ready() != 0 || on_device() != 0) return -1;
+    const int fmt = fmt_of<S>();
+    DevWeights dw;
+    if (dev_weights(w, d, dw) != 0) return -1;
+    const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0);
+    std::vector<TreeIn> in;
+    int most = 0;
+    if (tree_prepare(fmt, d, cfg->rope_theta, counts, parents, batch, states, rb, in, &most) != 0) return -1;
+    size_t at = 0;
+    for (int g = 0; g < batch;) {
+        const int e = tree_group_end(counts, batch, g);
+        int n = 0;
+        for (int i = g; i < e; ++i) n += counts[i];
+        DecodeWork wk;
+        if (decode_work(d, n, (int)rb, wk) != 0) return -1;
+        if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data() + g, e - g, d_x + at * d.H, d_out + at * d.H,
+                       (flags & KVL_MLA_RESIDUAL) != 0, wk, in_norm) != 0)
+            return -1;
+        if (!(flags & KVL_MLA_NO_ADVANCE))
+            for (int i = g; i < e; ++i) {
+                states[i]->len += counts[i];
+                in[i].m->synced = states[i]->len;  // host rows are not written
+            }
+        at += (size_t)n;
+        g = e;
+    }
+    return 0;
+}
+
+// The attention half of a decoder layer (attention_layer_device) for the nodes of trees.
+template <class S>
+int attention_layer_tree(float *d_h, float *d_n2, const int *counts, const int *parents, int batch, const KvlMlaConfig *cfg,
+                         const KvlMlaBF16 *w, const uint16_t *input_norm, const uint16_t *post_norm, S *const *states,
+                         unsigned flags) {
+    Dims d;
+    if (!d_h || !d_n2 || d_n2 == d_h || !counts || !parents || batch <= 0 || !states || !input_norm || !post_norm ||
+        !weights_ok(w) || !dims_of(cfg, d)) {
+        set_err("invalid arguments");
+        return -1;
+    }
+    if (flags & ~(unsigned)KVL_MLA_NO_ADVANCE) {
+        set_err("unsupported flags (the residual add is implied)");
+        return -1;
+    }
+    if (tree_check(counts, parents, batch, cfg, states) != 0) return -1;
+    if (!dims_supported(d)) return -1;
+    if (ensure_ready() != 0 || on_device() != 0) return -1;
+    Ctx &c = ctx();
+    const uint16_t *din = nullptr, *dpost = nullptr;
+    if (dev_weight(input_norm, (size_t)d.H, &din) != 0 || dev_weight(post_norm, (size_t)d.H, &dpost) != 0) return -1;
+    int rows = 0;
+    for (int i = 0; i < batch; ++i) rows += counts[i];
+    const size_t need = (size_t)std::min(rows, kTreeNodes) * d.H * sizeof(float);
+    if (c.layer.bytes < need) {
+        if (c.capturing) {
+            set_err("layer workspace growth during graph capture");
+            return -1;
+        }
+        if (dev_reserve(c.layer, need) != 0) return -1;
+    }
+    const InNorm in{din, (float *)c.layer.p};
+    if (tree_device(d_h, d_h, counts, parents, batch, cfg, w, states, flags | KVL_MLA_RESIDUAL, &in) != 0) return -1;
+    HIP_TRY(launch_rmsnorm(c.stream, d_n2, d_h, dpost, d.H, rows, cfg->rms_eps));
+    return 0;
+}
+
+// ---------------------------------------------------------------- rows ------------------
+
+void comps_of(const Mirror &m, int *e, void **p) {
+    size_t ea, eb, ec;
+    comp_bytes(m.fmt, m.d0, m.d1, m.d2, ea, eb, ec);
+    e[0] = (int)ea;
+    e[1] = (int)eb;
+    e[2] = (int)ec;
+    p[0] = m.a;
+    p[1] = m.b;
+    p[2] = m.c;
+}
+
+void *host_comp(const HostView &v, int k) { return (void *)(k == 0 ? v.ha : k == 1 ? v.hb : v.hc); }
+
+// Copies of rows [row0, row1) of srcs[i] to dsts[i], whose len becomes row1. host: the host rows too,
+// synchronous.
+template <class S>
+int fork_rows(S *const *dsts, S *const *srcs, const int *row0, const int *row1, int n, bool host) {
+    if (!dsts || !srcs || !row0 || !row1 || n <= 0) {
+        set_err("invalid arguments");
+        return -1;
+    }
+    for (int i = 0; i < n; ++i) {
+        const S *d = dsts[i], *s = srcs[i];
+        if (!d || !s || d->kv_lora_rank != s->kv_lora_rank || d->qk_rope_dim != s->qk_rope_dim ||
+            s->kv_lora_rank != srcs[0]->kv_lora_rank || s->qk_rope_dim != srcs[0]->qk_rope_dim || s->capacity <= 0 ||
+            d->capacity <= 0) {
+            set_err("pair %d: two initialised states of the same dims (one set of dims per call)", i);
+            return -1;
+        }
+        if (row0[i] < 0 || row1[i] < row0[i] || row1[i] > s->len || row0[i] > d->len || row1[i] > d->capacity ||
+            s->len > s->capacity || d->len > d->capacity) {
+            set_err("pair %d: rows %d .. %d of a source of %d rows, into a state of %d rows and capacity %d", i, row0[i],
+                    row1[i], s->len, d->len, d->capacity);
+            return -1;
+        }
+    }
+    {
+        std::vector<const void *> ds(dsts, dsts + n);
+        std::sort(ds.begin(), ds.end());
+        if (std::adjacent_find(ds.begin(), ds.end()) != ds.end()) {
+            set_err("a state stands twice among the destinations");
+            return -1;
+        }
+        for (int i = 0; i < n; ++i)
+            if (std::binary_search(ds.begin(), ds.end(), (const void *)srcs[i])) {
+                set_err("pair %d: its source is also a destination", i);
+                return -1;
+            }
+    }
+    if (ensure_ready() != 0 || on_device() != 0) return -1;
+    Ctx &c = ctx();
+    if (c.capturing) {
+        set_err("copy of state rows during graph capture");
+        return -1;
+    }
+    std::vector<Mirror *> md(n), ms(n);
+    for (int i = 0; i < n; ++i) {
+        if (mirror_get(srcs[i], view_of(srcs[i]), &ms[i]) != 0) return -1;
+        // of the destination only the rows that stay, [0, row0), have to be on the device
+        const HostView v = view_of(dsts[i]);
+        if (mirror_get(dsts[i], v, &md[i], true) != 0) return -1;
+        if (md[i]->synced < row0[i]) {
+            if (upload_rows(*md[i], v, md[i]->synced, row0[i], c.stream) != 0) return -1;
+            md[i]->synced = row0[i];
+        }
+    }
+    ForkTable t;
+    memset(&t, 0, sizeof t);
+    for (int i = 0; i < n; ++i) {
+        if (row1[i] > row0[i]) {
+            ForkDesc &f = t.d[t.n++];
+            void *p[3];
+            comps_of(*ms[i], t.e, p);
+            for (int k = 0; k < 3; ++k) f.src[k] = p[k];
+            comps_of(*md[i], t.e, p);
+            for (int k = 0; k < 3; ++k) f.dst[k] = p[k];
+            f.r0 = row0[i];
+            f.r1 = row1[i];
+        }
+        if (t.n == kForkBatch || (i == n - 1 && t.n > 0)) {
+            HIP_TRY(launch_fork(c.stream, t));
+            t.n = 0;
+        }
+    }
+    if (host) HIP_TRY(hipStreamSynchronize(c.stream));  // also: the uploads above have read the host rows
+    for (int i = 0; i < n; ++i) {
+        if (host) {
+            const HostView vs = view_of(srcs[i]), vd = view_of(dsts[i]);
+            int e[3];
+            void *p[3];
+            comps_of(*ms[i], e, p);
+            for (int k = 0; k < 3; ++k)
+                if (e[k])
+                    memcpy((char *)host_comp(vd, k) + (size_t)row0[i] * e[k], (const char *)host_comp(vs, k) + (size_t)row0[i] * e[k],
+                           (size_t)(row1[i] - row0[i]) * e[k]);
+        }
+        dsts[i]->len = row1[i];
+        md[i]->synced = row1[i];
+    }
+    return 0;
+}
+
+// Rows starts[i] + path (counts[i] of them, strictly increasing) become rows starts[i] .. of
+// states[i], whose len becomes starts[i] + counts[i]. host: the host rows too, synchronous.
+template <class S>
+int accept_rows(S *const *states, const int *starts, const int *counts, const int *paths, int batch, bool host) {
+    if (!states || !starts || !counts || batch <= 0) {
+        set_err("invalid arguments");
+        return -1;
+    }
+    size_t at = 0;
+    for (int i = 0; i < batch; ++i) {
+        const S *s = states[i];
+        if (!s || s->capacity <= 0 || s->kv_lora_rank != states[0]->kv_lora_rank || s->qk_rope_dim != states[0]->qk_rope_dim) {
+            set_err("state %d: an initialised state (one set of dims per call)", i);
+            return -1;
+        }
+        if (starts[i] < 0 || starts[i] > s->len || s->len > s->capacity || counts[i] < 0 || counts[i] > kTreeNodes ||
+            (counts[i] > 0 && !paths)) {
+            set_err("state %d: %d accepted nodes from row %d of %d", i, counts[i], starts[i], s->len);
+            return -1;
+        }
+        for (int j = 0; j < counts[i]; ++j) {
+            const int r = paths[at + j];
+            if (r < 0 || r >= kTreeNodes || r >= s->len - starts[i] || (j > 0 && r <= paths[at + j - 1])) {
+                set_err("state %d: accepted node %d at row %d + %d (the path is strictly increasing and within the tree)", i, j,
+                        starts[i], r);
+                return -1;
+            }
+        }
+        at += (size_t)counts[i];
+    }
+    if (twice(states, batch)) {
+        set_err("a state stands twice in the batch");
+        return -1;
+    }
+    if (ensure_ready() != 0 || on_device() != 0) return -1;
+    Ctx &c = ctx();
+    if (c.capturing) {
+        set_err("compaction of state rows during graph capture");
+        return -1;
+    }
+    std::vector<Mirror *> ms(batch);
+    for (int i = 0; i < batch; ++i)
+        if (mirror_get(states[i], view_of(states[i]), &ms[i]) != 0) return -1;
+    AcceptTable t;
+    memset(&t, 0, sizeof t);
+    at = 0;
+    for (int i = 0; i < batch; ++i) {
+        const int *path = paths + at;
+        int same = 0;  // the first nodes of the path that lie where they belong
+        while (same < counts[i] && path[same] == same) ++same;
+        if (same < counts[i]) {
+            AcceptDesc &a = t.d[t.n++];
+            comps_of(*ms[i], t.e, a.p);
+            a.start = starts[i] + same;
+            a.n = counts[i] - same;
+            for (int j = same; j < counts[i]; ++j) a.path[j - same] = (uint8_t)(path[j] - same);
+        }
+        if (t.n == kAcceptBatch || (i == batch - 1 && t.n > 0)) {
+            HIP_TRY(launch_accept(c.stream, t));
+            t.n = 0;
+        }
+        at += (size_t)counts[i];
+    }
+    if (host) HIP_TRY(hipStreamSynchronize(c.stream));
+    at = 0;
+    for (int i = 0; i < batch; ++i) {
+        if (host) {
+            const HostView v = view_of(states[i]);
+            int e[3];
+            void *p[3];
+            comps_of(*ms[i], e, p);
+            for (int j = 0; j < counts[i]; ++j)
+                for (int k = 0; k < 3; ++k)
+                    if (e[k] && paths[at + j] != j)
+                        memcpy((char *)host_comp(v, k) + (size_t)(starts[i] + j) * e[k],
+                               (const char *)host_comp(v, k) + (size_t)(starts[i] + paths[at + j]) * e[k], (size_t)e[k]);
+        }
+        states[i]->len = starts[i] + counts[i];
+        ms[i]->synced = states[i]->len;
+        at += (size_t)counts[i];
+    }
+    return 0;
+}
+
+// The device arrays of a state, its rows [0, len) uploaded where they were not yet.
+template <class S>
+int device_rows(S *state, void **a, void **b, void **c) {
+    const bool q8 = fmt_of<S>() == kFmtQ8;
+    if (!state || !a || !b || (q8 && !c) || state->capacity <= 0 || state->len < 0 || state->len > state->capacity) {
+        set_err("invalid arguments");
+        return -1;
+    }
+    if (ensure_ready() != 0 || on_device() != 0) return -1;
+    Mirror *m = nullptr;
+    if (mirror_get(state, view_of(state), &m) != 0) return -1;
+    *a = m->a;
+    *b = m->b;
+    if (c) *c = m->c;
+    return 0;
+}
+
+// A C entry point's body: one caller at a time, no exception past it.
+template <class F>
+int entry(F f) {
+    std::lock_guard<std::recursive_mutex> g(ctx().mu);
+    try {
+        g_err.clear();
+        return f();
+    } catch (const std::exception &e) {
+        try {
+            set_err("%s", e.what());
+        } catch (...) {
+        }
+        return -1;
+    }
+}
+
 // A captured graph and the free generation at its capture.
 struct GraphHandle {
     hipGraphExec_t exec;
@@ -2460,6 +2986,140 @@ int kvl_mla_attention_layer_bf16_device(float *d_h, float *d_n2, int batch, cons
                                         KvlMlaCompressedBF16State *const *states, unsigned flags) {
     Guard guard;
     return attention_layer_device(d_h, d_n2, batch, cfg, w, input_norm, post_attn_norm, states, flags);
+}
+
+// ---- trees, copies and accepted paths (include/kvl/mla_hip.h) ----------------------------
+
+int kvl_mla_decode_compressed_tree_bf16(float *out, const float *x, const int *parents, int count,
+                                           int start_position, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           KvlMlaCompressedState *state) {
+    return entry([&] { return tree_host(out, x, parents, count, start_position, cfg, w, state); });
+}
+
+int kvl_mla_decode_compressed_tree_batch_device(float *d_out, const float *d_x, const int *counts,
+                                                   const int *parents, int batch, const KvlMlaConfig *cfg,
+                                                   const KvlMlaBF16 *w, KvlMlaCompressedState *const *states,
+                                                   unsigned flags) {
+    return entry([&] { return tree_device(d_out, d_x, counts, parents, batch, cfg, w, states, flags); });
+}
+
+int kvl_mla_attention_layer_tree_device(float *d_h, float *d_n2, const int *counts, const int *parents,
+                                           int batch, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           const uint16_t *input_norm, const uint16_t *post_attn_norm,
+                                           KvlMlaCompressedState *const *states, unsigned flags) {
+    return entry([&] {
+        return attention_layer_tree(d_h, d_n2, counts, parents, batch, cfg, w, input_norm, post_attn_norm, states, flags);
+    });
+}
+
+int kvl_mla_compressed_state_fork(KvlMlaCompressedState *dst, KvlMlaCompressedState *src, int row0, int row1) {
+    return entry([&] { return fork_rows(&dst, &src, &row0, &row1, 1, true); });
+}
+
+int kvl_mla_compressed_state_fork_batch_device(KvlMlaCompressedState *const *dsts, KvlMlaCompressedState *const *srcs,
+                                                  const int *row0, const int *row1, int n) {
+    return entry([&] { return fork_rows(dsts, srcs, row0, row1, n, false); });
+}
+
+int kvl_mla_compressed_state_accept(KvlMlaCompressedState *state, int start, const int *path, int n) {
+    return entry([&] { return accept_rows(&state, &start, &n, path, 1, true); });
+}
+
+int kvl_mla_compressed_state_accept_batch_device(KvlMlaCompressedState *const *states, const int *starts,
+                                                    const int *counts, const int *paths, int batch) {
+    return entry([&] { return accept_rows(states, starts, counts, paths, batch, false); });
+}
+
+int kvl_mla_compressed_state_device_rows(KvlMlaCompressedState *state, void **latent, void **rope) {
+    return entry([&] { return device_rows(state, latent, rope, nullptr); });
+}
+
+int kvl_mla_decode_compressed_bf16_tree_bf16(float *out, const float *x, const int *parents, int count,
+                                           int start_position, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           KvlMlaCompressedBF16State *state) {
+    return entry([&] { return tree_host(out, x, parents, count, start_position, cfg, w, state); });
+}
+
+int kvl_mla_decode_compressed_bf16_tree_batch_device(float *d_out, const float *d_x, const int *counts,
+                                                   const int *parents, int batch, const KvlMlaConfig *cfg,
+                                                   const KvlMlaBF16 *w, KvlMlaCompressedBF16State *const *states,
+                                                   unsigned flags) {
+    return entry([&] { return tree_device(d_out, d_x, counts, parents, batch, cfg, w, states, flags); });
+}
+
+int kvl_mla_attention_layer_bf16_tree_device(float *d_h, float *d_n2, const int *counts, const int *parents,
+                                           int batch, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           const uint16_t *input_norm, const uint16_t *post_attn_norm,
+                                           KvlMlaCompressedBF16State *const *states, unsigned flags) {
+    return entry([&] {
+        return attention_layer_tree(d_h, d_n2, counts, parents, batch, cfg, w, input_norm, post_attn_norm, states, flags);
+    });
+}
+
+int kvl_mla_compressed_bf16_state_fork(KvlMlaCompressedBF16State *dst, KvlMlaCompressedBF16State *src, int row0, int row1) {
+    return entry([&] { return fork_rows(&dst, &src, &row0, &row1, 1, true); });
+}
+
+int kvl_mla_compressed_bf16_state_fork_batch_device(KvlMlaCompressedBF16State *const *dsts, KvlMlaCompressedBF16State *const *srcs,
+                                                  const int *row0, const int *row1, int n) {
+    return entry([&] { return fork_rows(dsts, srcs, row0, row1, n, false); });
+}
+
+int kvl_mla_compressed_bf16_state_accept(KvlMlaCompressedBF16State *state, int start, const int *path, int n) {
+    return entry([&] { return accept_rows(&state, &start, &n, path, 1, true); });
+}
+
+int kvl_mla_compressed_bf16_state_accept_batch_device(KvlMlaCompressedBF16State *const *states, const int *starts,
+                                                    const int *counts, const int *paths, int batch) {
+    return entry([&] { return accept_rows(states, starts, counts, paths, batch, false); });
+}
+
+int kvl_mla_compressed_bf16_state_device_rows(KvlMlaCompressedBF16State *state, void **latent, void **rope) {
+    return entry([&] { return device_rows(state, latent, rope, nullptr); });
+}
+
+int kvl_mla_decode_compressed_q8_tree_bf16(float *out, const float *x, const int *parents, int count,
+                                           int start_position, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           KvlMlaCompressedQ8State *state) {
+    return entry([&] { return tree_host(out, x, parents, count, start_position, cfg, w, state); });
+}
+
+int kvl_mla_decode_compressed_q8_tree_batch_device(float *d_out, const float *d_x, const int *counts,
+                                                   const int *parents, int batch, const KvlMlaConfig *cfg,
+                                                   const KvlMlaBF16 *w, KvlMlaCompressedQ8State *const *states,
+                                                   unsigned flags) {
+    return entry([&] { return tree_device(d_out, d_x, counts, parents, batch, cfg, w, states, flags); });
+}
+
+int kvl_mla_attention_layer_q8_tree_device(float *d_h, float *d_n2, const int *counts, const int *parents,
+                                           int batch, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           const uint16_t *input_norm, const uint16_t *post_attn_norm,
+                                           KvlMlaCompressedQ8State *const *states, unsigned flags) {
+    return entry([&] {
+        return attention_layer_tree(d_h, d_n2, counts, parents, batch, cfg, w, input_norm, post_attn_norm, states, flags);
+    });
+}
+
+int kvl_mla_compressed_q8_state_fork(KvlMlaCompressedQ8State *dst, KvlMlaCompressedQ8State *src, int row0, int row1) {
+    return entry([&] { return fork_rows(&dst, &src, &row0, &row1, 1, true); });
+}
+
+int kvl_mla_compressed_q8_state_fork_batch_device(KvlMlaCompressedQ8State *const *dsts, KvlMlaCompressedQ8State *const *srcs,
+                                                  const int *row0, const int *row1, int n) {
+    return entry([&] { return fork_rows(dsts, srcs, row0, row1, n, false); });
+}
+
+int kvl_mla_compressed_q8_state_accept(KvlMlaCompressedQ8State *state, int start, const int *path, int n) {
+    return entry([&] { return accept_rows(&state, &start, &n, path, 1, true); });
+}
+
+int kvl_mla_compressed_q8_state_accept_batch_device(KvlMlaCompressedQ8State *const *states, const int *starts,
+                                                    const int *counts, const int *paths, int batch) {
+    return entry([&] { return accept_rows(states, starts, counts, paths, batch, false); });
+}
+
+int kvl_mla_compressed_q8_state_device_rows(KvlMlaCompressedQ8State *state, void **codes, void **scales, void **rope) {
+    return entry([&] { return device_rows(state, codes, scales, rope); });
 }
 
 void *kvl_mla_stream(void) {

@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(HERE, "libkvl_mla.so")
 QSP = C.POINTER(abi.QS)
 CSP = C.POINTER(abi.CS)
 BSP = C.POINTER(abi.BS)
+INTP = C.POINTER(C.c_int)
 
 # include/kvl/mla_hip.h
 EXT_API = {
@@ -99,6 +100,21 @@ EXT_API = {
                                                            abi.BS]),
     "mla_attention_layer_bf16_device": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, abi.CFG, abi.W, abi.u16p,
                                                    abi.u16p, BSP, C.c_uint]),
+    # branching histories: trees of draft tokens, copies of rows, accepted paths
+    **{name: entry for f, S, SP, n in (("", abi.CS, CSP, 2), ("bf16_", abi.BS, BSP, 2), ("q8_", abi.QS, QSP, 3))
+       for name, entry in {
+           f"mla_decode_compressed_{f}tree_bf16": (C.c_int, [abi.f32p, abi.f32p, INTP, C.c_int, C.c_int, abi.CFG,
+                                                             abi.W, S]),
+           f"mla_decode_compressed_{f}tree_batch_device": (C.c_int, [C.c_void_p, C.c_void_p, INTP, INTP, C.c_int,
+                                                                     abi.CFG, abi.W, SP, C.c_uint]),
+           f"mla_attention_layer_{f}tree_device": (C.c_int, [C.c_void_p, C.c_void_p, INTP, INTP, C.c_int, abi.CFG,
+                                                             abi.W, abi.u16p, abi.u16p, SP, C.c_uint]),
+           f"mla_compressed_{f}state_fork": (C.c_int, [S, S, C.c_int, C.c_int]),
+           f"mla_compressed_{f}state_fork_batch_device": (C.c_int, [SP, SP, INTP, INTP, C.c_int]),
+           f"mla_compressed_{f}state_accept": (C.c_int, [S, C.c_int, INTP, C.c_int]),
+           f"mla_compressed_{f}state_accept_batch_device": (C.c_int, [SP, INTP, INTP, INTP, C.c_int]),
+           f"mla_compressed_{f}state_device_rows": (C.c_int, [S] + [C.POINTER(C.c_void_p)] * n),
+       }.items()},
 }
 
 # stage 1 is the fused append + query preparation of the compressed formats (the expanded

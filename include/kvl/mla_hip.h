@@ -12,6 +12,8 @@
  *   - explicit re-synchronisation of a state whose rows were edited in place on the host;
  *   - batched (ragged) decode over many sequences in one call;
  *   - stream-ordered device-pointer variants (no host sync), capturable in a HIP graph;
+ *   - branching histories: trees of draft tokens verified in one call, copies of a state's
+ *     rows, and the compaction of a state to the accepted path;
  *   - the quantiser boundary (fp32 latent -> Q8 row) as a standalone entry point;
  *   - device-side synthetic histories for benchmarks.
  * Every int-returning function returns 0 on success and -1 on failure; the reason is then
@@ -226,6 +228,101 @@ int kvl_mla_prefill_compressed_bf16_state_bf16(float *out, const float *x, int s
 int kvl_mla_prefill_compressed_bf16_state_device(float *d_out, const float *d_x, int seq_len,
                                                  const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
                                                  KvlMlaCompressedBF16State *state);
+
+/* ---- Branching histories (extensions, no counterpart in the reference) -----------------------
+ *
+ * A tree of draft tokens over one sequence's history of n = len rows: node i (0 <= i < count,
+ * count <= 64) hangs on parents[i], an earlier node of its tree (parents[i] < i), or on the
+ * history's last token (-1). Its position is n + its depth (0 for a child of the history), its row
+ * is row n + i, and it attends rows [0, n), the rows of its ancestors and its own; rows of other
+ * branches do not enter, whatever they hold. A tree of one node is a single-token decode, a chain a
+ * block decode: the appended rows equal theirs bit for bit, the outputs up to the order of
+ * summation.
+ * After a tree decode len = n + count: *_accept keeps one path's rows, *_truncate(state, n) drops
+ * the draft. Until then rows n .. n + count - 1 are the tree's, in node order, not a continuation.
+ *
+ * Host buffers, one sequence: out, x [count, hidden]; start_position must equal len. Synchronous;
+ * host rows written. */
+int kvl_mla_decode_compressed_tree_bf16(float *out, const float *x, const int *parents, int count,
+                                           int start_position, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           KvlMlaCompressedState *state);
+int kvl_mla_decode_compressed_bf16_tree_bf16(float *out, const float *x, const int *parents, int count,
+                                           int start_position, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           KvlMlaCompressedBF16State *state);
+int kvl_mla_decode_compressed_q8_tree_bf16(float *out, const float *x, const int *parents, int count,
+                                           int start_position, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           KvlMlaCompressedQ8State *state);
+/* Stream-ordered, a batch of sequences each with its own tree, over device buffers: tree b has
+ * counts[b] nodes (1 .. 64); the nodes of all trees stand one tree after another in parents (host,
+ * within-tree indices), d_x and d_out ([sum of counts, hidden] fp32). flags as the batch decodes:
+ * KVL_MLA_RESIDUAL, and KVL_MLA_NO_ADVANCE (rows written at len + i, len left). counts and parents
+ * are read during the call only; no state may stand twice. The appended rows stay on the device.
+ * Capturable once warm (trees, lengths and buffers are the captured ones). */
+int kvl_mla_decode_compressed_tree_batch_device(float *d_out, const float *d_x, const int *counts,
+                                                   const int *parents, int batch, const KvlMlaConfig *cfg,
+                                                   const KvlMlaBF16 *w, KvlMlaCompressedState *const *states,
+                                                   unsigned flags);
+int kvl_mla_decode_compressed_bf16_tree_batch_device(float *d_out, const float *d_x, const int *counts,
+                                                   const int *parents, int batch, const KvlMlaConfig *cfg,
+                                                   const KvlMlaBF16 *w, KvlMlaCompressedBF16State *const *states,
+                                                   unsigned flags);
+int kvl_mla_decode_compressed_q8_tree_batch_device(float *d_out, const float *d_x, const int *counts,
+                                                   const int *parents, int batch, const KvlMlaConfig *cfg,
+                                                   const KvlMlaBF16 *w, KvlMlaCompressedQ8State *const *states,
+                                                   unsigned flags);
+/* The attention half of a decoder layer (kvl_mla_attention_layer_device and its kin) for the nodes
+ * of trees: d_h, d_n2 [sum of counts, hidden]. flags: 0 or KVL_MLA_NO_ADVANCE. */
+int kvl_mla_attention_layer_tree_device(float *d_h, float *d_n2, const int *counts, const int *parents,
+                                           int batch, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           const uint16_t *input_norm, const uint16_t *post_attn_norm,
+                                           KvlMlaCompressedState *const *states, unsigned flags);
+int kvl_mla_attention_layer_bf16_tree_device(float *d_h, float *d_n2, const int *counts, const int *parents,
+                                           int batch, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           const uint16_t *input_norm, const uint16_t *post_attn_norm,
+                                           KvlMlaCompressedBF16State *const *states, unsigned flags);
+int kvl_mla_attention_layer_q8_tree_device(float *d_h, float *d_n2, const int *counts, const int *parents,
+                                           int batch, const KvlMlaConfig *cfg, const KvlMlaBF16 *w,
+                                           const uint16_t *input_norm, const uint16_t *post_attn_norm,
+                                           KvlMlaCompressedQ8State *const *states, unsigned flags);
+/* dst takes over rows [row0, row1) of src, on the device and in the host arrays, and has len =
+ * row1; its own rows [0, row0) stay. Both states initialised with the same dims, 0 <= row0 <= row1,
+ * row0 <= dst->len, row1 <= src->len, row1 <= dst's capacity. Synchronous. (Host rows of src that
+ * were never written, as after stream-ordered calls, are copied as they are.) */
+int kvl_mla_compressed_state_fork(KvlMlaCompressedState *dst, KvlMlaCompressedState *src, int row0, int row1);
+int kvl_mla_compressed_bf16_state_fork(KvlMlaCompressedBF16State *dst, KvlMlaCompressedBF16State *src, int row0, int row1);
+int kvl_mla_compressed_q8_state_fork(KvlMlaCompressedQ8State *dst, KvlMlaCompressedQ8State *src, int row0, int row1);
+/* The same for n pairs, stream-ordered, on the device only (host rows are not written). A source may
+ * serve several pairs; no destination may stand twice or be a source of the same call; all states of
+ * a call have the same dims. Not capturable. */
+int kvl_mla_compressed_state_fork_batch_device(KvlMlaCompressedState *const *dsts, KvlMlaCompressedState *const *srcs,
+                                                  const int *row0, const int *row1, int n);
+int kvl_mla_compressed_bf16_state_fork_batch_device(KvlMlaCompressedBF16State *const *dsts, KvlMlaCompressedBF16State *const *srcs,
+                                                  const int *row0, const int *row1, int n);
+int kvl_mla_compressed_q8_state_fork_batch_device(KvlMlaCompressedQ8State *const *dsts, KvlMlaCompressedQ8State *const *srcs,
+                                                  const int *row0, const int *row1, int n);
+/* Keeps the accepted path of a tree whose first node is row start: rows start + path[i], i < n,
+ * become rows start + i and len becomes start + n (n = 0 drops the whole tree). path: strictly
+ * increasing node indices, below 64 and below len - start; the nodes of a path from a child of the
+ * history down, so that a row's rotation is that of its new place. On the device and in the host
+ * arrays. Synchronous. */
+int kvl_mla_compressed_state_accept(KvlMlaCompressedState *state, int start, const int *path, int n);
+int kvl_mla_compressed_bf16_state_accept(KvlMlaCompressedBF16State *state, int start, const int *path, int n);
+int kvl_mla_compressed_q8_state_accept(KvlMlaCompressedQ8State *state, int start, const int *path, int n);
+/* The same for a batch of states (the layers of sequences), stream-ordered, on the device only:
+ * state b keeps counts[b] nodes from row starts[b] on, the paths standing one after another in paths.
+ * No state may stand twice; all have the same dims. Not capturable. */
+int kvl_mla_compressed_state_accept_batch_device(KvlMlaCompressedState *const *states, const int *starts,
+                                                    const int *counts, const int *paths, int batch);
+int kvl_mla_compressed_bf16_state_accept_batch_device(KvlMlaCompressedBF16State *const *states, const int *starts,
+                                                    const int *counts, const int *paths, int batch);
+int kvl_mla_compressed_q8_state_accept_batch_device(KvlMlaCompressedQ8State *const *states, const int *starts,
+                                                    const int *counts, const int *paths, int batch);
+/* The device addresses of a state's row arrays (the layout of its host arrays; [0, len) is
+ * uploaded first where it was not yet), for programs that read rows on the device in the order of
+ * kvl_mla_stream(). Valid until the state is freed or initialised again; read only. */
+int kvl_mla_compressed_state_device_rows(KvlMlaCompressedState *state, void **latent, void **rope);
+int kvl_mla_compressed_bf16_state_device_rows(KvlMlaCompressedBF16State *state, void **latent, void **rope);
+int kvl_mla_compressed_q8_state_device_rows(KvlMlaCompressedQ8State *state, void **codes, void **scales, void **rope);
 
 /* The library's HIP stream (hipStream_t) and helpers for callers without a HIP binding.
  * kvl_mla_synchronize waits for the stream; it returns -1 when a stream-ordered fused decode
