@@ -1673,10 +1673,6 @@ constexpr int kB16SpOff = kB16Ring * kB16Slot;     // score halves [2][16 heads]
 constexpr int kB16SmemB = kB16SpOff + 2 * 16 * kB16SpHs * 4;
 static_assert(kB16SmemB <= 160 * 1024, "LDS of one CU");
 
-// bits (r3, r2, r1, r0) of a chunk row -> slot XOR (r3, r1, r0, r2): a bijection on 16 rows, and
-// (r3, r1, r0) -> distinct slot pairs for the 8 rows of a transposed half-wave read
-__device__ __forceinline__ int b16_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8); }
-
 // Max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48 with the gfx950 lane-swap instructions (VALU,
 // no LDS round trip): v_permlane16_swap with both operands v gives every lane the values of its
 // lane pair (l & ~16, l | 16), v_permlane32_swap those of (l & ~32, l | 32); the lower lane's value
@@ -1695,13 +1691,6 @@ __device__ __forceinline__ float xgroup_sum(float v) {
 }
 
 constexpr float kB16LnPmax = 1.3862944f;  // ln 4: the weights p_j = exp(s_j - m) stay <= 4
-
-typedef short v4s __attribute__((ext_vector_type(4)));
-// ds_read_b64_tr_b16: within each 16-lane group, destination lane i element e is element i & 3
-// of the four addressed by source lane 4e + (i >> 2).
-__device__ __forceinline__ v4s lds_read_tr16(const uint8_t *p) {
-    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(p));
-}
 
 template <bool ONCE>  // ONCE: each history row is read by one workgroup (non-temporal loads)
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_attn_bf16_mfma(KVL_ATTN_HOT_PARAMS, AttnArgs a) {

@@ -308,6 +308,19 @@ __device__ __forceinline__ void wait_vmcnt() {
 // Workgroup barrier after this wave's LDS writes have completed.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
+// 16-byte slots of a 1 KB latent row in LDS, XOR-swizzled so that the score reads (16 rows, one slot)
+// and the transposed reads (4 rows x 32 bytes per 16 lanes) spread over the banks:
+// bits (r3, r2, r1, r0) of a chunk row -> slot XOR (r3, r1, r0, r2): a bijection on 16 rows, and
+// (r3, r1, r0) -> distinct slot pairs for the 8 rows of a transposed half-wave read
+__device__ __forceinline__ int b16_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8); }
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+// ds_read_b64_tr_b16: within each 16-lane group, destination lane i element e is element i & 3
+// of the four addressed by source lane 4e + (i >> 2).
+__device__ __forceinline__ v4s lds_read_tr16(const uint8_t *p) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)(p));
+}
+
 // SplitMix64 output k (k >= 1) of the stream seeded by `seed`.
 __device__ __forceinline__ uint64_t splitmix64_at(uint64_t seed, uint64_t k) {
     uint64_t z = seed + k * 0x9E3779B97F4A7C15ull;

@@ -248,15 +248,21 @@ struct TreeSeq {
     int ctx;          // rows of the history
     int count;        // nodes
     int node0;        // the tree's first node among the group's
-    int pad;
+    int part0;        // its first partial: node i's are part0 + i * (ns + 1) .., ns of the history and one
+    int ns, rps;      //   of the tree's rows; the history in ns splits of rps rows (the last: the rest)
+    int tiles, unit0; // ceil(count / nm); the splits of the sequences before it
 };
 struct TreeTable {
     TreeSeq s[kTreeNodes];
     int8_t parent[kTreeNodes];  // per node of the group: its parent within its own tree, or -1
     uint8_t seq[kTreeNodes];    // per node of the group: its sequence
     int n, nodes;
+    int nm;  // nodes per history workgroup (2 or 4); 0: the route for any dims (every row in one partial)
 };
-// Attention of the group's nodes (queries w.qf) into w.part: node k's partial is split k.
+// The plan of a group (t.n, t.nodes, t.s[].ctx, count, node0 given): nm, the splits and the partials;
+// returns the number of partials.
+int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu);
+// Attention of the group's nodes (queries w.qf) into w.part.
 hipError_t launch_tree_attention(hipStream_t st, int fmt, const TreeTable &t, const Dims &d, const DecodeWork &w);
 
 // Copies of rows [r0, r1) between the device arrays of two states of one format (arrays with

@@ -1907,7 +1907,22 @@ int tree_group_end(const int *counts, int batch, int g0) {
     return g;
 }
 
-size_t tree_part_bytes(const Dims &d, int nodes) { return (size_t)nodes * d.NH * (d.R + 2) * sizeof(float); }
+// A group's table (without the parents) and plan; bytes of its partials.
+size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &tt) {
+    memset(&tt, 0, sizeof tt);
+    tt.n = n;
+    for (int b = 0; b < n; ++b) {
+        TreeSeq &s = tt.s[b];
+        s.a = seqs[b].m->a;
+        s.b = seqs[b].m->b;
+        s.c = seqs[b].m->c;
+        s.ctx = seqs[b].ctx;
+        s.count = seqs[b].count;
+        s.node0 = tt.nodes;
+        tt.nodes += s.count;
+    }
+    return (size_t)plan_tree(fmt, d, tt, ctx().ncu) * d.NH * (d.R + 2) * sizeof(float);
+}
 
 // One tree decode of a launch group: the steps of decode_group with the group's nodes as its
 // members, each member's row at history row ctx + i and its rotation at position ctx + depth.
@@ -1918,12 +1933,11 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
     hipStream_t st = c.stream;
     TreeTable tt;
     SeqTable t;
-    memset(&tt, 0, sizeof tt);
+    const size_t part_bytes = tree_plan(fmt, d, seqs, n, tt);
     memset(&t, 0, sizeof t);
     int k = 0, maxpos = 0;
     for (int b = 0; b < n; ++b) {
         const TreeIn &q = seqs[b];
-        tt.s[b] = {q.m->a, q.m->b, q.m->c, q.ctx, q.count, k, 0};
         int dep[kTreeNodes];
         for (int i = 0; i < q.count; ++i, ++k) {
             dep[i] = q.parents[i] < 0 ? 0 : dep[q.parents[i]] + 1;
@@ -1935,17 +1949,16 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
             s.c = q.m->c;
             s.pos = q.ctx + dep[i];
             s.roff = i - dep[i];
-            s.split0 = k;
-            s.nsplit = 1;
+            s.nsplit = tt.s[b].ns + 1;
+            s.split0 = tt.s[b].part0 + i * s.nsplit;
             maxpos = std::max(maxpos, s.pos);
         }
     }
-    tt.n = n;
-    tt.nodes = t.n = k;
+    t.n = k;
     const int N = k, ldy = d.QO + d.KVO;
     const float2 *cs = nullptr;
     if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
-    if (reserve_part(tree_part_bytes(d, N), &w.part) != 0) return -1;
+    if (reserve_part(part_bytes, &w.part) != 0) return -1;
     if (in_norm) {
         HIP_TRY(launch_rmsnorm(st, in_norm->buf, d_x, in_norm->w, d.H, N, eps));
         d_x = in_norm->buf;
@@ -2028,7 +2041,7 @@ int tree_check(const int *counts, const int *parents, int batch, const KvlMlaCon
 // the device copies of the states, the RoPE table, the workspace and the partials of the largest group.
 template <class S>
 int tree_prepare(int fmt, const Dims &d, float theta, const int *counts, const int *parents, int batch, S *const *states,
-                 size_t rb, std::vector<TreeIn> &in, int *most) {
+                 size_t rb, std::vector<TreeIn> &in) {
     in.resize(batch);
     int maxpos = 0;
     for (int i = 0; i < batch; ++i) {
@@ -2040,16 +2053,18 @@ int tree_prepare(int fmt, const Dims &d, float theta, const int *counts, const i
     }
     const float2 *cs = nullptr;
     if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
-    *most = 0;
+    int most = 0;
+    size_t part = 0;
     for (int g = 0; g < batch;) {
         const int e = tree_group_end(counts, batch, g);
-        int n = 0;
-        for (; g < e; ++g) n += counts[g];
-        *most = std::max(*most, n);
+        TreeTable tt;
+        part = std::max(part, tree_plan(fmt, d, in.data() + g, e - g, tt));
+        most = std::max(most, tt.nodes);
+        g = e;
     }
     DecodeWork wk;
     float *pp = nullptr;
-    if (decode_work(d, *most, (int)rb, wk) != 0 || reserve_part(tree_part_bytes(d, *most), &pp) != 0) return -1;
+    if (decode_work(d, most, (int)rb, wk) != 0 || reserve_part(part, &pp) != 0) return -1;
     return 0;
 }
 
@@ -2076,8 +2091,7 @@ int tree_host(float *out, const float *x, const int *parents, int count, int sta
     if (dev_weights(w, d, dw) != 0) return -1;
     const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0);
     std::vector<TreeIn> in;
-    int most = 0;
-    if (tree_prepare(fmt, d, cfg->rope_theta, &count, parents, 1, st, rb, in, &most) != 0) return -1;
+    if (tree_prepare(fmt, d, cfg->rope_theta, &count, parents, 1, st, rb, in) != 0) return -1;
     DecodeWork wk;
     if (decode_work(d, count, (int)rb, wk) != 0) return -1;
     const size_t xin = (size_t)count * d.H * sizeof(float);
@@ -2117,8 +2131,7 @@ int tree_device(float *d_out, const float *d_x, const int *counts, const int *pa
     if (dev_weights(w, d, dw) != 0) return -1;
     const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0);
     std::vector<TreeIn> in;
-    int most = 0;
-    if (tree_prepare(fmt, d, cfg->rope_theta, counts, parents, batch, states, rb, in, &most) != 0) return -1;
+    if (tree_prepare(fmt, d, cfg->rope_theta, counts, parents, batch, states, rb, in) != 0) return -1;
     size_t at = 0;
     for (int g = 0; g < batch;) {
         const int e = tree_group_end(counts, batch, g);
