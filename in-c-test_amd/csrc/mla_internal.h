@@ -241,29 +241,41 @@ hipError_t launch_empty(hipStream_t st);
 
 // ---- trees and rows (mla_tree.hip) ----
 // A tree decode: the nodes of one or more sequences' drafts, each node attending its sequence's
-// history, its ancestors and itself.
-constexpr int kTreeNodes = 64;  // nodes of one tree, and of one launch group
+// history, its ancestors and itself. A launch group: up to kMaxBatch sequences and kTreeGroup nodes; what
+// is told per node travels in kernel arguments for kTreeNodes nodes at a time.
+constexpr int kTreeNodes = 64;   // nodes of one tree
+constexpr int kTreeGroup = 256;
 struct TreeSeq {
     void *a, *b, *c;  // the history's device arrays (see Fmt); node i's row is row ctx + i
     int ctx;          // rows of the history
     int count;        // nodes
     int node0;        // the tree's first node among the group's
-    int part0;        // its first partial: node i's are part0 + i * (ns + 1) .., ns of the history and one
-    int ns, rps;      //   of the tree's rows; the history in ns splits of rps rows (the last: the rest)
+    int part0;        // its first partial: node i's are part0 + i * ns .. (ns = 0: part0 + i, of all its rows)
+    int ns, rps;      // the history in ns splits of rps rows (the last: the rest)
     int tiles, unit0; // ceil(count / nm); the splits of the sequences before it
 };
 struct TreeTable {
-    TreeSeq s[kTreeNodes];
-    int8_t parent[kTreeNodes];  // per node of the group: its parent within its own tree, or -1
-    uint8_t seq[kTreeNodes];    // per node of the group: its sequence
+    TreeSeq s[kMaxBatch];
     int n, nodes;
     int nm;  // nodes per history workgroup (2 or 4); 0: the route for any dims (every row in one partial)
+};
+struct TreeNodes {  // nodes first .. first + n - 1 of the group
+    uint64_t path[kTreeNodes];  // the node and its ancestors: bit i = node i of its tree
+    uint8_t seq[kTreeNodes];    // its sequence
+    int first, n;
 };
 // The plan of a group (t.n, t.nodes, t.s[].ctx, count, node0 given): nm, the splits and the partials;
 // returns the number of partials.
 int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu);
-// Attention of the group's nodes (queries w.qf) into w.part.
-hipError_t launch_tree_attention(hipStream_t st, int fmt, const TreeTable &t, const Dims &d, const DecodeWork &w);
+// History attention of the group's nodes (queries w.qf) into w.part (nm != 0).
+hipError_t launch_tree_history(hipStream_t st, int fmt, const TreeTable &t, const Dims &d, const DecodeWork &w);
+// The nodes' own paths, the merge with the history's partials and W_UV: w.hos, plane stride
+// t.nodes * HO (nm != 0).
+hipError_t launch_tree_combine(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
+                               const uint16_t *kv_b, const DecodeWork &w);
+// Attention of the nodes over all their rows into w.part (nm == 0).
+hipError_t launch_tree_generic(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
+                               const DecodeWork &w);
 
 // Copies of rows [r0, r1) between the device arrays of two states of one format (arrays with
 // e[0..2] bytes a row; 0: none).

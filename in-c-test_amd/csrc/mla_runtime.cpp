@@ -1900,10 +1900,20 @@ int tree_depth(const int *parents, int count) {  // of the deepest node, a child
     return most;
 }
 
-// Sequences from g0 on that one launch group takes: at most kTreeNodes nodes.
+// Whether a group's trees of one node each go through the single-token decode of the batch: its kernels
+// are made for that; not over Q8 rows, where it takes the query in 15 bits and a tree's outputs are to be
+// good to 1e-5.
+bool tree_as_tokens(int fmt, const Dims &d, const int *counts, int batch) {
+    if (fmt == kFmtQ8 || !kimi_attn(d)) return false;
+    for (int i = 0; i < batch; ++i)
+        if (counts[i] != 1) return false;
+    return true;
+}
+
+// Sequences from g0 on that one launch group takes: at most kMaxBatch, and at most kTreeGroup nodes.
 int tree_group_end(const int *counts, int batch, int g0) {
     int n = 0, g = g0;
-    while (g < batch && n + counts[g] <= kTreeNodes) n += counts[g++];
+    while (g < batch && g - g0 < kMaxBatch && n + counts[g] <= kTreeGroup) n += counts[g++];
     return g;
 }
 
@@ -1927,37 +1937,18 @@ size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &t
 // One tree decode of a launch group: the steps of decode_group with the group's nodes as its
 // members, each member's row at history row ctx + i and its rotation at position ctx + depth.
 // Everything it needs has been acquired (tree_prepare).
-int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights &dw, const TreeIn *seqs, int n,
+int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights &dw, const TreeIn *seqs, int n, bool tokens,
                const float *d_x, float *d_out, bool residual, DecodeWork &w, const InNorm *in_norm = nullptr) {
     Ctx &c = ctx();
     hipStream_t st = c.stream;
-    TreeTable tt;
-    SeqTable t;
-    const size_t part_bytes = tree_plan(fmt, d, seqs, n, tt);
-    memset(&t, 0, sizeof t);
-    int k = 0, maxpos = 0;
-    for (int b = 0; b < n; ++b) {
-        const TreeIn &q = seqs[b];
-        int dep[kTreeNodes];
-        for (int i = 0; i < q.count; ++i, ++k) {
-            dep[i] = q.parents[i] < 0 ? 0 : dep[q.parents[i]] + 1;
-            tt.parent[k] = (int8_t)q.parents[i];
-            tt.seq[k] = (uint8_t)b;
-            SeqDesc &s = t.s[k];
-            s.a = q.m->a;
-            s.b = q.m->b;
-            s.c = q.m->c;
-            s.pos = q.ctx + dep[i];
-            s.roff = i - dep[i];
-            s.nsplit = tt.s[b].ns + 1;
-            s.split0 = tt.s[b].part0 + i * s.nsplit;
-            maxpos = std::max(maxpos, s.pos);
-        }
+    if (tokens) {
+        SeqIn one[kMaxBatch];
+        for (int b = 0; b < n; ++b) one[b] = {seqs[b].m, seqs[b].ctx};
+        return decode_group(fmt, d, eps, theta, dw, one, n, d_x, d_out, residual, w, false, 0, in_norm);
     }
-    t.n = k;
-    const int N = k, ldy = d.QO + d.KVO;
-    const float2 *cs = nullptr;
-    if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
+    TreeTable tt;
+    const size_t part_bytes = tree_plan(fmt, d, seqs, n, tt);
+    const int N = tt.nodes, ldy = d.QO + d.KVO;
     if (reserve_part(part_bytes, &w.part) != 0) return -1;
     if (in_norm) {
         HIP_TRY(launch_rmsnorm(st, in_norm->buf, d_x, in_norm->w, d.H, N, eps));
@@ -1976,14 +1967,72 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         w.ypstride = 0;
         HIP_TRY(launch_gemv(st, w.y, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H, false));
     }
-    HIP_TRY(launch_append_qprep(st, fmt, t, d, w.y, ldy, d.QO, w.ynp, w.ypstride, dw.norm, eps, cs, dw.kvb, dw.ukt, w,
-                                false));
-    HIP_TRY(launch_tree_attention(st, fmt, tt, d, w));
-    HIP_TRY(launch_combine(st, fmt, t, d, dw.kvb, w));
-    if (combine_writes_hos(fmt, d) && gemv_xs_ok(d.HO))
+    // What is told per node goes kTreeNodes nodes at a time.
+    const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0), qs = (size_t)std::max(d.R + d.DR, d.QD);
+    const float2 *cs = nullptr;
+    TreeNodes nds[(kTreeGroup + kTreeNodes - 1) / kTreeNodes];
+    int b = 0, i = 0, dep[kTreeNodes];
+    uint64_t path[kTreeNodes];
+    for (int k0 = 0, z = 0; k0 < N; k0 += kTreeNodes, ++z) {
+        TreeNodes &nd = nds[z];
+        SeqTable t;
+        memset(&t, 0, sizeof t);
+        memset(&nd, 0, sizeof nd);
+        nd.first = k0;
+        nd.n = t.n = std::min(kTreeNodes, N - k0);
+        int maxpos = 0;
+        for (int k = 0; k < t.n; ++k, ++i) {
+            while (i == seqs[b].count) {
+                i = 0;
+                ++b;
+            }
+            const TreeIn &q = seqs[b];
+            const int p = q.parents[i];
+            dep[i] = p < 0 ? 0 : dep[p] + 1;
+            path[i] = (p < 0 ? 0 : path[p]) | (uint64_t)1 << i;
+            nd.path[k] = path[i];
+            nd.seq[k] = (uint8_t)b;
+            SeqDesc &s = t.s[k];
+            s.a = q.m->a;
+            s.b = q.m->b;
+            s.c = q.m->c;
+            s.pos = q.ctx + dep[i];
+            s.roff = i - dep[i];
+            maxpos = std::max(maxpos, s.pos);
+        }
+        if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
+        DecodeWork wk = w;
+        wk.y += (size_t)k0 * ldy;
+        wk.qf += (size_t)k0 * d.NH * qs;
+        wk.rows += (size_t)k0 * rb;
+        HIP_TRY(launch_append_qprep(st, fmt, t, d, wk.y, ldy, d.QO, w.ynp, w.ypstride, dw.norm, eps, cs, dw.kvb,
+                                    dw.ukt, wk, false));
+    }
+    if (tt.nm) {
+        HIP_TRY(launch_tree_history(st, fmt, tt, d, w));
+        for (int k0 = 0, z = 0; k0 < N; k0 += kTreeNodes, ++z) HIP_TRY(launch_tree_combine(st, fmt, tt, nds[z], d, dw.kvb, w));
         HIP_TRY(launch_gemv_xs(st, d_out, d.H, w.hos, N, dw.o, d.H, d.HO, residual));
-    else
-        HIP_TRY(launch_gemv(st, d_out, d.H, w.ho, d.HO, N, dw.o, d.H, nullptr, 0, d.HO, residual));
+        return 0;
+    }
+    for (int k0 = 0, z = 0; k0 < N; k0 += kTreeNodes, ++z) {
+        HIP_TRY(launch_tree_generic(st, fmt, tt, nds[z], d, w));
+        SeqTable t;
+        memset(&t, 0, sizeof t);
+        t.n = nds[z].n;
+        for (int k = 0; k < t.n; ++k) {
+            t.s[k].split0 = k0 + k;
+            t.s[k].nsplit = 1;
+        }
+        DecodeWork wk = w;
+        wk.mix += (size_t)k0 * d.NH * std::max(d.R, d.DV);
+        wk.ho += (size_t)k0 * d.HO;
+        HIP_TRY(launch_combine(st, fmt, t, d, dw.kvb, wk));
+        // the planes of a combine's head outputs lie t.n rows apart: o_proj follows slice by slice
+        if (combine_writes_hos(fmt, d) && gemv_xs_ok(d.HO))
+            HIP_TRY(launch_gemv_xs(st, d_out + (size_t)k0 * d.H, d.H, wk.hos, t.n, dw.o, d.H, d.HO, residual));
+        else
+            HIP_TRY(launch_gemv(st, d_out + (size_t)k0 * d.H, d.H, wk.ho, d.HO, t.n, dw.o, d.H, nullptr, 0, d.HO, residual));
+    }
     return 0;
 }
 
@@ -2041,7 +2090,14 @@ int tree_check(const int *counts, const int *parents, int batch, const KvlMlaCon
 // the device copies of the states, the RoPE table, the workspace and the partials of the largest group.
 template <class S>
 int tree_prepare(int fmt, const Dims &d, float theta, const int *counts, const int *parents, int batch, S *const *states,
-                 size_t rb, std::vector<TreeIn> &in) {
+                 size_t rb, bool tokens, std::vector<TreeIn> &in) {
+    if (tokens) {
+        std::vector<Mirror *> ms;
+        if (prepare_groups(fmt, d, theta, states, batch, rb, ms) != 0) return -1;
+        in.resize(batch);
+        for (int i = 0; i < batch; ++i) in[i] = {ms[i], states[i]->len, 1, parents + i};
+        return 0;
+    }
     in.resize(batch);
     int maxpos = 0;
     for (int i = 0; i < batch; ++i) {
@@ -2091,15 +2147,16 @@ int tree_host(float *out, const float *x, const int *parents, int count, int sta
     if (dev_weights(w, d, dw) != 0) return -1;
     const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0);
     std::vector<TreeIn> in;
-    if (tree_prepare(fmt, d, cfg->rope_theta, &count, parents, 1, st, rb, in) != 0) return -1;
+    const bool tokens = tree_as_tokens(fmt, d, &count, 1);
+    if (tree_prepare(fmt, d, cfg->rope_theta, &count, parents, 1, st, rb, tokens, in) != 0) return -1;
     DecodeWork wk;
     if (decode_work(d, count, (int)rb, wk) != 0) return -1;
     const size_t xin = (size_t)count * d.H * sizeof(float);
     if (pin_reserve(c.pin_in, xin) != 0 || pin_reserve(c.pin_out, xin + count * rb) != 0) return -1;
     memcpy(c.pin_in.p, x, xin);
     wk.rows = (uint8_t *)c.pin_out.p + xin;  // as in decode_block: x, outputs and rows in the pinned buffers
-    if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data(), 1, (const float *)c.pin_in.p, (float *)c.pin_out.p,
-                   false, wk) != 0)
+    if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data(), 1, tokens, (const float *)c.pin_in.p,
+                   (float *)c.pin_out.p, false, wk) != 0)
         return -1;
     HIP_TRY(hipStreamSynchronize(c.stream));
     memcpy(out, c.pin_out.p, xin);
@@ -2131,7 +2188,8 @@ int tree_device(float *d_out, const float *d_x, const int *counts, const int *pa
     if (dev_weights(w, d, dw) != 0) return -1;
     const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0);
     std::vector<TreeIn> in;
-    if (tree_prepare(fmt, d, cfg->rope_theta, counts, parents, batch, states, rb, in) != 0) return -1;
+    const bool tokens = tree_as_tokens(fmt, d, counts, batch);
+    if (tree_prepare(fmt, d, cfg->rope_theta, counts, parents, batch, states, rb, tokens, in) != 0) return -1;
     size_t at = 0;
     for (int g = 0; g < batch;) {
         const int e = tree_group_end(counts, batch, g);
@@ -2139,8 +2197,8 @@ int tree_device(float *d_out, const float *d_x, const int *counts, const int *pa
         for (int i = g; i < e; ++i) n += counts[i];
         DecodeWork wk;
         if (decode_work(d, n, (int)rb, wk) != 0) return -1;
-        if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data() + g, e - g, d_x + at * d.H, d_out + at * d.H,
-                       (flags & KVL_MLA_RESIDUAL) != 0, wk, in_norm) != 0)
+        if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data() + g, e - g, tokens, d_x + at * d.H,
+                       d_out + at * d.H, (flags & KVL_MLA_RESIDUAL) != 0, wk, in_norm) != 0)
             return -1;
         if (!(flags & KVL_MLA_NO_ADVANCE))
             for (int i = g; i < e; ++i) {
@@ -2176,7 +2234,7 @@ int attention_layer_tree(float *d_h, float *d_n2, const int *counts, const int *
     if (dev_weight(input_norm, (size_t)d.H, &din) != 0 || dev_weight(post_norm, (size_t)d.H, &dpost) != 0) return -1;
     int rows = 0;
     for (int i = 0; i < batch; ++i) rows += counts[i];
-    const size_t need = (size_t)std::min(rows, kTreeNodes) * d.H * sizeof(float);
+    const size_t need = (size_t)std::min(rows, kTreeGroup) * d.H * sizeof(float);
     if (c.layer.bytes < need) {
         if (c.capturing) {
             set_err("layer workspace growth during graph capture");

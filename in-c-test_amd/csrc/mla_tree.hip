@@ -3,6 +3,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mla_device.h"
 #include "mla_internal.h"
@@ -16,14 +17,23 @@ namespace kvl {
 //   s_j = (q_lat . lat_j + q_rope . key_j) / sqrt(QD),  mix = sum_j softmax(s)_j lat_j.
 // Rows of other branches are never read for it, so nothing they hold (NaN, infinities) reaches it.
 
+// What the kernels that go by node need of a sequence (kernel arguments stay below 4 KB).
+struct TreeRows {
+    void *a, *b, *c;
+    int ctx, node0, part0, ns;
+};
+struct TreeRowsTable {
+    TreeRows s[kMaxBatch];
+};
+
 template <int FMT>
-__device__ __forceinline__ float tree_lat(const TreeSeq &s, size_t row, int R, int k) {
+__device__ __forceinline__ float tree_lat(const TreeRows &s, size_t row, int R, int k) {
     if (FMT == kFmtQ8) return (float)((const int8_t *)s.a)[row * R + k] * ((const float *)s.b)[row];
     if (FMT == kFmtF32) return ((const float *)s.a)[row * R + k];
     return bf16_to_f32(((const uint16_t *)s.a)[row * R + k]);
 }
 template <int FMT>
-__device__ __forceinline__ float tree_key(const TreeSeq &s, size_t row, int DR, int k) {
+__device__ __forceinline__ float tree_key(const TreeRows &s, size_t row, int DR, int k) {
     if (FMT == kFmtQ8) return bf16_to_f32(((const uint16_t *)s.c)[row * DR + k]);
     if (FMT == kFmtF32) return ((const float *)s.b)[row * DR + k];
     return bf16_to_f32(((const uint16_t *)s.b)[row * DR + k]);
@@ -31,11 +41,23 @@ __device__ __forceinline__ float tree_key(const TreeSeq &s, size_t row, int DR, 
 
 struct TreeArgs {
     TreeTable t;
-    Dims d;
     const float *qf;
     float *part;
     float smscale;
 };
+struct TreeNodeArgs {
+    TreeRowsTable t;
+    TreeNodes nd;
+    const float *qf;
+    float *part;
+    float smscale;
+    int NH, R, DR;
+};
+static TreeRowsTable tree_rows(const TreeTable &t) {
+    TreeRowsTable r{};
+    for (int b = 0; b < t.n; ++b) r.s[b] = {t.s[b].a, t.s[b].b, t.s[b].c, t.s[b].ctx, t.s[b].node0, t.s[b].part0, t.s[b].ns};
+    return r;
+}
 
 constexpr int kTgRows = 256;  // rows taken at a time: a thread per row
 constexpr int kTgCols = 4;    // latent columns per thread: R <= 1024
@@ -44,21 +66,20 @@ constexpr int kTgCols = 4;    // latent columns per thread: R <= 1024
 // running maximum and sum of the softmax; a thread per row forms the scores, a thread per latent
 // column the mix.
 template <int FMT>
-__global__ __launch_bounds__(256) void k_tree_generic(TreeArgs a) {
+__global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
     __shared__ float q[1024 + 256];
     __shared__ float p[kTgRows];
     __shared__ float redm[4], reds[4];
     __shared__ int path[kTreeNodes];
     __shared__ int npath;
-    const int tid = threadIdx.x, NH = a.d.NH, R = a.d.R, DR = a.d.DR;
-    const int k = blockIdx.x / NH, h = blockIdx.x % NH;
-    const TreeSeq s = a.t.s[a.t.seq[k]];
+    const int tid = threadIdx.x, NH = a.NH, R = a.R, DR = a.DR;
+    const int k = a.nd.first + blockIdx.x / NH, h = blockIdx.x % NH;
+    const TreeRows s = a.t.s[a.nd.seq[k - a.nd.first]];
     for (int i = tid; i < R + DR; i += 256) q[i] = a.qf[((size_t)k * NH + h) * (R + DR) + i];
     if (tid == 0) {  // the node and its ancestors, in the order of their rows
         int n = 0;
-        for (int i = k - s.node0; i >= 0; i = a.t.parent[s.node0 + i]) ++n;
+        for (uint64_t m = a.nd.path[k - a.nd.first]; m; m &= m - 1) path[n++] = __builtin_ctzll(m);
         npath = n;
-        for (int i = k - s.node0; i >= 0; i = a.t.parent[s.node0 + i]) path[--n] = i;
     }
     __syncthreads();
     const int rows = s.ctx + npath;
@@ -98,87 +119,13 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeArgs a) {
         }
         __syncthreads();  // p and the reductions are rewritten
     }
-    float *P = a.part + (size_t)k * NH * (R + 2);
+    float *P = a.part + (size_t)(s.part0 + k - s.node0) * NH * (R + 2);
 #pragma unroll
     for (int c = 0; c < kTgCols; ++c)
         if (tid + 256 * c < R) P[(size_t)h * R + tid + 256 * c] = acc[c];
     if (tid == 0) {
         P[(size_t)NH * R + h] = m;
         P[(size_t)NH * R + NH + h] = l;
-    }
-}
-
-// ---- the tree's own rows (Kimi shapes: NH = 16, R = 512, DR = 64) ----------------------------------
-
-// One workgroup of eight waves per node, wave w its heads 2w, 2w + 1, lane l columns l + 64 q and key
-// column l: the scores of the node's path (at most 64 rows: row j's in lane j), their maximum and
-// weights, then the mix. fp32 throughout. The partial after the node's history partials.
-template <int FMT>
-__global__ __launch_bounds__(512) void k_tree_path(TreeArgs a) {
-    constexpr int R = 512, DR = 64, NH = 16;
-    __shared__ int path[kTreeNodes];
-    __shared__ int npath;
-    const int tid = threadIdx.x, l = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), k = blockIdx.x;
-    const TreeSeq s = a.t.s[a.t.seq[k]];
-    if (tid == 0) {
-        int n = 0;
-        for (int i = k - s.node0; i >= 0; i = a.t.parent[s.node0 + i]) ++n;
-        npath = n;
-        for (int i = k - s.node0; i >= 0; i = a.t.parent[s.node0 + i]) path[--n] = i;
-    }
-    float q[2][9];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < 9; ++c) q[h][c] = a.qf[((size_t)k * NH + 2 * w + h) * (R + DR) + 64 * c + l] * a.smscale;
-    __syncthreads();
-    const int n = npath;
-    float sc[2] = {-INFINITY, -INFINITY};
-    for (int j = 0; j < n; ++j) {
-        const size_t row = (size_t)s.ctx + path[j];
-        float v0 = 0.f, v1 = 0.f;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const float x = tree_lat<FMT>(s, row, R, 64 * c + l);
-            v0 = fmaf(q[0][c], x, v0);
-            v1 = fmaf(q[1][c], x, v1);
-        }
-        const float x = tree_key<FMT>(s, row, DR, l);
-        v0 = wave_sum(fmaf(q[0][8], x, v0));
-        v1 = wave_sum(fmaf(q[1][8], x, v1));
-        if (l == j) {
-            sc[0] = v0;
-            sc[1] = v1;
-        }
-    }
-    float m[2], p[2], sum[2], acc[2][8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        m[h] = wave_max(sc[h]);
-        p[h] = l < n ? __expf(sc[h] - m[h]) : 0.f;
-        sum[h] = wave_sum(p[h]);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) acc[h][c] = 0.f;
-    }
-    for (int j = 0; j < n; ++j) {
-        const size_t row = (size_t)s.ctx + path[j];
-        const float p0 = lane_f32(p[0], j), p1 = lane_f32(p[1], j);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            const float x = tree_lat<FMT>(s, row, R, 64 * c + l);
-            acc[0][c] = fmaf(p0, x, acc[0][c]);
-            acc[1][c] = fmaf(p1, x, acc[1][c]);
-        }
-    }
-    float *P = a.part + (size_t)(s.part0 + (k - s.node0) * (s.ns + 1) + s.ns) * NH * (R + 2);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-        for (int c = 0; c < 8; ++c) P[(2 * w + h) * R + 64 * c + l] = acc[h][c];
-        if (l == 0) {
-            P[NH * R + 2 * w + h] = m[h];
-            P[NH * R + NH + 2 * w + h] = sum[h];
-        }
     }
 }
 
@@ -199,8 +146,7 @@ __global__ __launch_bounds__(512) void k_tree_path(TreeArgs a) {
 // whatever the scales, the running maximum is that of score + ln(scale), so that weight times scale stays
 // <= 4.
 constexpr int kThCh = 32;       // rows of a chunk
-constexpr int kThSp = 36;       // floats per query in a score half
-constexpr int kThPw = 80;       // bytes per query in a weight plane (32 bf16, padded)
+constexpr int kThFree = 0x16;   // sched_barrier: vector, scalar and global memory instructions may cross
 template <int FMT, int NM>
 struct ThShape {
     static constexpr int NW = 2 * NM, NT = 64 * NW, NQ = 16 * NM;
@@ -208,40 +154,78 @@ struct ThShape {
     static constexpr int LatB = kThCh * 1024, KeyB = kThCh * 128, PlaneB = LatB + KeyB;
     static constexpr int ScB = FMT == kFmtQ8 ? 2 * kThCh * 4 : 0;  // scales, their logarithms
     static constexpr int Slot = NP * PlaneB + ScB;
-    static constexpr int Ring = FMT == kFmtF32 || NM < 4 ? 1 : 2;
+    static constexpr int Ring = FMT == kFmtF32 || NM < 4 ? 1 : 3;
+    static constexpr bool Pipe = Ring == 3;
     static constexpr int SpOff = Ring * Slot;
-    static constexpr int PwOff = SpOff + 2 * NQ * kThSp * 4;
-    static constexpr int AlOff = PwOff + 2 * NQ * kThPw;
+    static constexpr int SpH = NQ * 36;  // floats of a half of the scores (th_sp)
+    static constexpr int SpB = 2 * SpH * 4;
+    static constexpr int PwOff = SpOff + (Pipe ? 2 : 1) * SpB;
+    static constexpr int PwB = NQ * 64;  // bytes of a plane of weights (th_pw)
+    static constexpr int AlOff = PwOff + 2 * PwB;
     static constexpr int FlOff = AlOff + NQ * 4;
     static constexpr int Smem = FlOff + 2 * 8 * 4;
     static_assert(Smem <= 160 * 1024, "LDS of one CU");
 };
+// Places in LDS, chosen so that the lanes served together hit distinct banks. A 16-byte read serves 16
+// lanes a cycle, and not neighbours: lanes 0-3, 12-15, 20-23, 24-27, then 4-7, 8-11, 16-19, 28-31 and so
+// on (found with patterns of conflicting addresses and the LDS counters). With rows n = lane % 16 and
+// words + lane / 16, as the products read, that is rows 0-3 and 12-15 of one word beside 4-11 of the next.
+//   word c of latent row r: c ^ th_swz(r), which also spreads the transposed reads (4 rows x 32 bytes);
+//   word of 8 weights of query q: th_pw;  score of query q, row 0 (floats): th_sp;
+// 18 + 8 such reads of a chunk and wave: 97 -> 0 cycles of conflicts.
+__device__ __forceinline__ int th_swz(int r) { return ((r & 3) << 1) | ((((r >> 2) ^ (r >> 3)) & 1) << 3) | ((r >> 3) & 1); }
+__device__ __forceinline__ int th_sp(int q) { return (q >> 2) * 144 + (q & 3) * 32; }
+__device__ __forceinline__ int th_pw(int q, int word) {
+    const int z = (q >> 2) & 3;
+    return q * 64 + 16 * (word ^ (((z ^ (z << 1)) & 2) | (z >> 1)));
+}
+// word c of key row r
+__device__ __forceinline__ int th_key(int r, int c) { return r * 128 + 16 * (c ^ ((r >> 1) & 7)); }
 
 // Workgroup -> (sequence, split, tile). Workgroup i runs on XCD i % 8; the units (a sequence's split) go
 // to the XCDs in turn, and the tiles of a unit follow one another on its XCD, so that its L2 serves the
-// rows they share. Lane b of every wave counts what sequence b has on this XCD.
-__device__ __forceinline__ bool tree_unit(const TreeTable &t, int &b, int &split, int &tile) {
+// rows they share. Lane b of every wave reads sequence b's entry and counts what it has on this XCD; the
+// workgroup's entry then comes from its lane, in scalar registers.
+__device__ __forceinline__ int tree_lane(int v, int b) { return __builtin_amdgcn_readlane(v, b); }
+__device__ __forceinline__ uint8_t *tree_lane(void *p, int b) {
+    const uint64_t u = (uint64_t)p;
+    const uint32_t lo = (uint32_t)tree_lane((int)(uint32_t)u, b), hi = (uint32_t)tree_lane((int)(uint32_t)(u >> 32), b);
+    return (uint8_t *)(((uint64_t)hi << 32) | lo);
+}
+struct TreeUnit {
+    uint8_t *a, *b, *c;
+    int ctx, count, node0, part0, ns, rps, split, tile;
+};
+__device__ __forceinline__ bool tree_unit(const TreeTable &t, TreeUnit &u) {
     const int lane = threadIdx.x & 63, xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
-    const TreeSeq &q = t.s[lane];
-    const int live = lane < t.n ? 1 : 0, u0 = live ? q.unit0 : 0, ns = live ? q.ns : 0, tiles = live ? q.tiles : 0;
-    const int first = (xcd - u0) & 7;  // the first of its splits on this XCD
-    const int mine = (ns > first ? (ns - first + 7) / 8 : 0) * tiles;
+    const TreeSeq q = t.s[lane];
+    const int live = lane < t.n ? 1 : 0, ns = live ? q.ns : 0;
+    const int first = (xcd - q.unit0) & 7;  // the first of its splits on this XCD
+    const int mine = (ns > first ? (ns - first + 7) / 8 : 0) * q.tiles;
     int sum = mine;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
         const int v = __shfl_up(sum, o);
         if (lane >= o) sum += v;
     }
-    if (j >= __shfl(sum, 63)) return false;
-    b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(sum <= j));
-    const int r = j - __shfl(sum - mine, b), tl = __shfl(tiles, b);
-    split = __shfl(first, b) + 8 * (r / tl);
-    tile = r % tl;
-    b = __builtin_amdgcn_readfirstlane(b);
-    split = __builtin_amdgcn_readfirstlane(split);
-    tile = __builtin_amdgcn_readfirstlane(tile);
+    if (j >= tree_lane(sum, 63)) return false;
+    const int b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(sum <= j));
+    const int r = j - tree_lane(sum - mine, b), tiles = tree_lane(q.tiles, b);
+    u.split = tree_lane(first, b) + 8 * (r / tiles);
+    u.tile = r % tiles;
+    u.a = tree_lane(q.a, b);
+    u.b = tree_lane(q.b, b);
+    u.c = tree_lane(q.c, b);
+    u.ctx = tree_lane(q.ctx, b);
+    u.count = tree_lane(q.count, b);
+    u.node0 = tree_lane(q.node0, b);
+    u.part0 = tree_lane(q.part0, b);
+    u.ns = tree_lane(q.ns, b);
+    u.rps = tree_lane(q.rps, b);
     return true;
 }
+
+typedef int v2i __attribute__((ext_vector_type(2)));
 
 template <int FMT>
 __device__ __forceinline__ v4f th_mfma(const v4i &a, const v4i &b, const v4f &c) {
@@ -266,173 +250,168 @@ __device__ __forceinline__ void th_split(const v4f &x0, const v4f &x1, v4i &hi, 
     }
 }
 
-// Sixteen int8 codes -> sixteen fp16 values, exact: the code + 128 as the low mantissa bits of 1024,
-// minus 1152.
-__device__ __forceinline__ void codes_f16(const v4i &c, v4i &o0, v4i &o1) {
+// Eight int8 codes -> eight fp16 values, exact: the code + 128 as the low mantissa bits of 1024, minus
+// 1152.
+__device__ __forceinline__ v4i codes_f16(const v2i &c) {
     const v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
-    uint32_t o[8];
+    uint32_t o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
         const uint32_t u = (uint32_t)c[i] ^ 0x80808080u;
-        const uint32_t a = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
-        const uint32_t b = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
-        o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, a) - off);
-        o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, b) - off);
+        o[2 * i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off);
+        o[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(v2h, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off);
     }
-    o0 = v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
-    o1 = v4i{(int)o[4], (int)o[5], (int)o[6], (int)o[7]};
+    return v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
+}
+
+// Four weights as hi and lo halves. fp16: both cut toward zero (one instruction per pair), what is left
+// out is below 2^-20 of the weight.
+template <bool F16>
+__device__ __forceinline__ void th_split4(const v4f &x, int2 &hi, int2 &lo) {
+    if constexpr (F16) {
+        const v2h h0 = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
+        const v2h h1 = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[2], x[3]));
+        const v2h l0 = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[0] - (float)h0.x, x[1] - (float)h0.y));
+        const v2h l1 = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[2] - (float)h1.x, x[3] - (float)h1.y));
+        hi = int2{__builtin_bit_cast(int, h0), __builtin_bit_cast(int, h1)};
+        lo = int2{__builtin_bit_cast(int, l0), __builtin_bit_cast(int, l1)};
+    } else {
+        const v2bf h0 = __builtin_convertvector((v2f{x[0], x[1]}), v2bf), h1 = __builtin_convertvector((v2f{x[2], x[3]}), v2bf);
+        const v2bf l0 = __builtin_convertvector((v2f{x[0] - (float)h0.x, x[1] - (float)h0.y}), v2bf);
+        const v2bf l1 = __builtin_convertvector((v2f{x[2] - (float)h1.x, x[3] - (float)h1.y}), v2bf);
+        hi = int2{__builtin_bit_cast(int, h0), __builtin_bit_cast(int, h1)};
+        lo = int2{__builtin_bit_cast(int, l0), __builtin_bit_cast(int, l1)};
+    }
 }
 
 template <int FMT, int NM>
 __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_tree_hist(TreeArgs a) {
     using Sh = ThShape<FMT, NM>;
-    constexpr int NT = Sh::NT, NW = Sh::NW, NQ = Sh::NQ, NP = Sh::NP, Ring = Sh::Ring;
+    constexpr int NT = Sh::NT, NW = Sh::NW, NP = Sh::NP;
     constexpr int NC = 512 / NW / 16;  // 16-column blocks of a wave in the mix
     constexpr bool kQ8 = FMT == kFmtQ8;
     __shared__ __attribute__((aligned(16))) uint8_t smem[Sh::Smem];
     const int tid = threadIdx.x, l = tid & 63, n = l & 15, g = l >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int b, split, tile;
-    if (!tree_unit(a.t, b, split, tile)) return;
-    const TreeSeq &s = a.t.s[b];
+    TreeUnit s;
+    if (!tree_unit(a.t, s)) return;
+    const int split = s.split, tile = s.tile;
     const int r0 = split * s.rps, r1 = split == s.ns - 1 ? s.ctx : r0 + s.rps;
     const int nch = (r1 - r0 + kThCh - 1) / kThCh;
     const int first = tile * NM, live = min(NM, s.count - first);  // nodes of this tile
-    float *sp = (float *)(smem + Sh::SpOff);
 
-    // ---- staging: a chunk's rows from memory to registers, and from there to an LDS slot. Row j's
-    // 16-byte word c lies at word c ^ b16_swz(j) of its latents, c ^ (j & 7) of its key. Rows past the
-    // split's end repeat its last row (their scores are masked).
-    constexpr int NL = (kQ8 ? 1024 : 2048) / NT;  // latent items of a thread (16 codes, or 8 values)
-    constexpr int NK = (256 + NT - 1) / NT;       // key items (8 values)
-    v4i la[NL], lb[FMT == kFmtF32 ? NL : 1], ka[NK], kb[FMT == kFmtF32 ? NK : 1];
+    // ---- staging: a chunk's rows from memory to registers, and from there to an LDS slot. A thread
+    // takes eight values at a time: word tid % 64 of latent rows tid / 64 + NW i, word tid % 8 of key rows
+    // tid / 8 + NT / 8 i. Row j's word c lies at word c ^ th_swz(j). Rows past the split's end repeat its
+    // last row (their scores are masked).
+    constexpr int NL = kThCh / NW, NK = (256 + NT - 1) / NT;
+    constexpr int LE = kQ8 ? 1 : FMT == kFmtF32 ? 4 : 2, KE = FMT == kFmtF32 ? 4 : 2;  // bytes of an element
+    constexpr int LV = LE == 4 ? 2 : 1, KV = KE == 4 ? 2 : 1;
+    v4i la[kQ8 ? 1 : NL * LV], ka[NK * KV];
+    v2i lc[kQ8 ? NL : 1];
     float rsc = 0.f;
+    const int lrow = tid >> 6, krow = tid >> 3;
+    // the split's rows as buffers: a read past the last row gives zeros (its score is masked)
+    const int nrow = r1 - r0;
+    const auto ba = __builtin_amdgcn_make_buffer_rsrc(s.a + (size_t)r0 * (512 * LE), 0, nrow * (512 * LE), 0x00027000);
+    const auto bk = __builtin_amdgcn_make_buffer_rsrc((kQ8 ? s.c : s.b) + (size_t)r0 * (64 * KE), 0, nrow * (64 * KE), 0x00027000);
+    const auto bs = __builtin_amdgcn_make_buffer_rsrc(s.b + (size_t)r0 * 4, 0, kQ8 ? nrow * 4 : 0, 0x00027000);
+    const int va = tid * (8 * LE), vk = tid * (8 * KE);  // rows lie one after another, so do the threads' words
     auto fetch = [&](int c) __attribute__((always_inline)) {
-        const int base = r0 + c * kThCh;
+        const int oa = va + c * (kThCh * 512 * LE), ok = vk + c * (kThCh * 64 * KE);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int it = tid + NT * i;
-            if constexpr (kQ8) {
-                la[i] = *(const v4i *)((const int8_t *)s.a + (size_t)min(base + (it >> 5), r1 - 1) * 512 + 16 * (it & 31));
-            } else if constexpr (FMT == kFmtF32) {
-                const float *p = (const float *)s.a + (size_t)min(base + (it >> 6), r1 - 1) * 512 + 8 * (it & 63);
-                la[i] = *(const v4i *)p;
-                lb[i] = *(const v4i *)(p + 4);
-            } else {
-                la[i] = *(const v4i *)((const uint16_t *)s.a + (size_t)min(base + (it >> 6), r1 - 1) * 512 + 8 * (it & 63));
-            }
+            if constexpr (kQ8)
+                lc[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(ba, oa + i * (NT * 8 * LE), 0, 0));
+            else
+#pragma unroll
+                for (int v = 0; v < LV; ++v)
+                    la[LV * i + v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ba, oa + i * (NT * 8 * LE) + 16 * v, 0, 0));
         }
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const int it = tid + NT * i;
-            if (it < 256) {
-                const size_t row = (size_t)min(base + (it >> 3), r1 - 1);
-                if constexpr (FMT == kFmtF32) {
-                    const float *p = (const float *)s.b + row * 64 + 8 * (it & 7);
-                    ka[i] = *(const v4i *)p;
-                    kb[i] = *(const v4i *)(p + 4);
-                } else {
-                    ka[i] = *(const v4i *)((const uint16_t *)(kQ8 ? s.c : s.b) + row * 64 + 8 * (it & 7));
-                }
-            }
-        }
-        if constexpr (kQ8) rsc = ((const float *)s.b)[min(base + (tid & 31), r1 - 1)];
+        for (int i = 0; i < NK; ++i)
+            if (NT <= 256 || tid < 256)
+#pragma unroll
+                for (int v = 0; v < KV; ++v)
+                    ka[KV * i + v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(bk, ok + i * (NT * 8 * KE) + 16 * v, 0, 0));
+        if constexpr (kQ8)
+            rsc = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(bs, 4 * (c * kThCh + (tid & 31)), 0, 0));
     };
-    auto stage = [&](int c) __attribute__((always_inline)) {
-        uint8_t *buf = smem + (c % Ring) * Sh::Slot;
+    auto put = [&](uint8_t *at, const v4i *v) __attribute__((always_inline)) {
+        if constexpr (NP == 2) {
+            v4i hi, lo;
+            th_split<false>(__builtin_bit_cast(v4f, v[0]), __builtin_bit_cast(v4f, v[1]), hi, lo);
+            *(v4i *)at = hi;
+            *(v4i *)(at + Sh::PlaneB) = lo;
+        } else {
+            *(v4i *)at = v[0];
+        }
+    };
+    const int sa = lrow * 1024 + 16 * (l ^ th_swz(lrow)), sk = Sh::LatB + th_key(krow, tid & 7);
+    auto stage = [&](uint8_t *buf) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
-            const int it = tid + NT * i;
-            if constexpr (kQ8) {
-                const int row = it >> 5, word = 2 * (it & 31), z = b16_swz(row);
-                v4i o0, o1;
-                codes_f16(la[i], o0, o1);
-                *(v4i *)(buf + row * 1024 + 16 * (word ^ z)) = o0;
-                *(v4i *)(buf + row * 1024 + 16 * ((word + 1) ^ z)) = o1;
-            } else {
-                const int row = it >> 6, at = row * 1024 + 16 * ((it & 63) ^ b16_swz(row));
-                if constexpr (FMT == kFmtF32) {
-                    v4i hi, lo;
-                    th_split<false>(__builtin_bit_cast(v4f, la[i]), __builtin_bit_cast(v4f, lb[i]), hi, lo);
-                    *(v4i *)(buf + at) = hi;
-                    *(v4i *)(buf + Sh::PlaneB + at) = lo;
-                } else {
-                    *(v4i *)(buf + at) = la[i];
-                }
-            }
+            // row lrow + NW i: b16_swz changes by the bits of NW i below 16
+            uint8_t *at = buf + (sa ^ (16 * th_swz((NW * i) & 15))) + NW * i * 1024;
+            if constexpr (kQ8) *(v4i *)at = codes_f16(lc[i]);
+            else put(at, la + LV * i);
         }
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const int it = tid + NT * i;
-            if (it < 256) {
-                const int row = it >> 3, at = Sh::LatB + row * 128 + 16 * ((it & 7) ^ (row & 7));
-                if constexpr (FMT == kFmtF32) {
-                    v4i hi, lo;
-                    th_split<false>(__builtin_bit_cast(v4f, ka[i]), __builtin_bit_cast(v4f, kb[i]), hi, lo);
-                    *(v4i *)(buf + at) = hi;
-                    *(v4i *)(buf + Sh::PlaneB + at) = lo;
-                } else {
-                    *(v4i *)(buf + at) = ka[i];
-                }
-            }
-        }
+        for (int i = 0; i < NK; ++i)
+            if (NT <= 256 || tid < 256) put(buf + sk + i * (NT / 8) * 128, ka + KV * i);
         if constexpr (kQ8) {
             if (tid < kThCh) {
                 float *sc = (float *)(buf + NP * Sh::PlaneB);
                 sc[tid] = rsc;
-                sc[kThCh + tid] = __logf(fmaxf(fabsf(rsc), 1e-35f));
+                sc[kThCh + tid] = __log2f(fmaxf(fabsf(rsc), 1e-35f));
             }
         }
     };
 
     fetch(0);
-    // ---- queries: A operand of the scores, head n of node m, columns 32 kb + 8 g ..
+    // ---- queries: A operand of the scores, head n of node m: columns 32 kb + 8 g .. of the eight
+    // latent blocks kb = 8 kh + j and of the key block kh (j = 8). Scores are in units of log2.
     const int m = w % NM, kh = w / NM;
     v4i qh[9], ql[9];
-    float qi = 1.0f;  // Q8: undoes the query's power of two, per head 4 g + i below
-    float qd[4] = {1.f, 1.f, 1.f, 1.f};
+    float qd[4] = {1.f, 1.f, 1.f, 1.f};  // Q8: undoes the query's power of two, heads 4 g + i
     {
         const float *qrow = a.qf + ((size_t)(s.node0 + first + min(m, live - 1)) * 16 + n) * 576 + 8 * g;
+        const float unit = a.smscale * 1.44269504f;
         v4f qv[18];
 #pragma unroll
         for (int j = 0; j < 9; ++j) {
-            qv[2 * j] = *(const v4f *)(qrow + 32 * (9 * kh + j));
-            qv[2 * j + 1] = *(const v4f *)(qrow + 32 * (9 * kh + j) + 4);
+            const float *p = qrow + (j < 8 ? 32 * (8 * kh + j) : 512 + 32 * kh);
+            qv[2 * j] = *(const v4f *)p * unit;
+            qv[2 * j + 1] = *(const v4f *)(p + 4) * unit;
         }
-        float qs = a.smscale;
+        float qs = 1.0f;
         if constexpr (kQ8) {
             float mx = 0.f;
 #pragma unroll
-            for (int j = 0; j < 18; ++j)
-                if (kh == 0 || j < 14)
+            for (int j = 0; j < 16; ++j)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(qv[j][e]));
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(qv[j][e]));
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            mx *= a.smscale;
             // 2^(10 - e) with 2^(e - 1) <= mx < 2^e, kept within the normal exponents
             const int e = mx > 0.f && mx < INFINITY ? min(max(ilogbf(mx) + 1, -100), 100) : 10;
-            qs = ldexpf(a.smscale, 10 - e);
-            qi = ldexpf(1.0f, e - 10);
+            qs = ldexpf(1.0f, 10 - e);
+            const float qi = ldexpf(1.0f, e - 10);
 #pragma unroll
             for (int i = 0; i < 4; ++i) qd[i] = __shfl(qi, 4 * g + i);
         }
 #pragma unroll
-        for (int j = 0; j < 9; ++j) {
-            if (kQ8 && (kh == 0 || j < 7)) th_split<true>(qv[2 * j] * qs, qv[2 * j + 1] * qs, qh[j], ql[j]);
-            else th_split<false>(qv[2 * j] * a.smscale, qv[2 * j + 1] * a.smscale, qh[j], ql[j]);
-        }
+        for (int j = 0; j < 8; ++j) th_split<kQ8>(qv[2 * j] * qs, qv[2 * j + 1] * qs, qh[j], ql[j]);
+        th_split<false>(qv[16], qv[17], qh[8], ql[8]);
     }
-    stage(0);
+    stage(smem);
     if (nch > 1) fetch(1);
 
-    // score operands: row n of a 16-row half (16 KB / 2 KB apart), words 4 kb + g
-    int bofs[9];
+    // score operands: row n of a 16-row half (16 KB / 2 KB apart), block j at bofs[j % 4] + 256 (j / 4)
+    int bofs[4];
 #pragma unroll
-    for (int j = 0; j < 9; ++j) {
-        const int kb = 9 * kh + j;
-        bofs[j] = kb < 16 ? n * 1024 + 16 * ((4 * kb + g) ^ b16_swz(n)) : Sh::LatB + n * 128 + 16 * ((4 * (kb - 16) + g) ^ (n & 7));
-    }
+    for (int j = 0; j < 4; ++j) bofs[j] = n * 1024 + 16 * ((4 * (8 * kh + j) + g) ^ th_swz(n));
+    const int kofs = Sh::LatB + th_key(n, 4 * kh + g);
     // transposed reads of column block NC w + t: rows 8 g + 4 h + (n >> 2), see lds_read_tr16
     int tro[2][NC];
 #pragma unroll
@@ -440,7 +419,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         const int row = 8 * g + 4 * h + (n >> 2);
 #pragma unroll
         for (int t = 0; t < NC; ++t)
-            tro[h][t] = row * 1024 + 16 * ((2 * (NC * w + t) + ((n >> 1) & 1)) ^ b16_swz(row)) + 8 * (n & 1);
+            tro[h][t] = row * 1024 + 16 * ((2 * (NC * w + t) + ((n >> 1) & 1)) ^ th_swz(row)) + 8 * (n & 1);
     }
     const int sq = tid >> 3, sr = 4 * (tid & 7);  // softmax: this thread's query and rows
     float m_run = -INFINITY, l_run = 0.f;
@@ -451,125 +430,170 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         for (int t = 0; t < NC; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
     lds_barrier();
 
-    for (int c = 0; c < nch; ++c) {
-        const uint8_t *buf = smem + (c % Ring) * Sh::Slot;
-        const float *scl = (const float *)(buf + NP * Sh::PlaneB);
-        // ---- scores
+    // The operand reads of a product run W reads ahead of it: the order of reads and products below is
+    // kept as it is written (left to itself the compiler reads each operand right before its use and waits
+    // for LDS every time); vector instructions may move across.
+    const int spw = Sh::SpOff + 4 * (kh * Sh::SpH + th_sp(16 * m + 4 * g) + n), spr = Sh::SpOff + 4 * (th_sp(sq) + sr);
+    auto scores = [&](const uint8_t *buf, int c) __attribute__((always_inline)) {
+        float *sp = (float *)(smem + spw + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
+        constexpr int N = 18 * NP, W = 6;  // read i: plane i % NP of rows 16 (i / NP % 2) of block i / NP / 2
+        auto get = [&](int i) __attribute__((always_inline)) {
+            const int j = i / (2 * NP), rb = i / NP % 2;
+            return *(const v4i *)(buf + (i % NP) * Sh::PlaneB + (j < 8 ? bofs[j & 3] + 256 * (j >> 2) + 16384 * rb : kofs + 2048 * rb));
+        };
+        v4f d[2], dk[2];
+        v4i bv[W];
+        float x[2] = {1.f, 1.f};
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
-            v4f dl = {0.f, 0.f, 0.f, 0.f}, dk = {0.f, 0.f, 0.f, 0.f};  // over latents, over the key
-#pragma unroll
-            for (int j = 0; j < 9; ++j) {
-                const bool key = j >= 7 && kh == 1;
-                const uint8_t *p = buf + bofs[j] + (j >= 7 && kh == 1 ? rb * 2048 : rb * 16384);
-                const v4i bv = *(const v4i *)p;
-                if (kQ8 && key) {
-                    dk = th_mfma<kFmtBF16>(qh[j], bv, dk);
-                    dk = th_mfma<kFmtBF16>(ql[j], bv, dk);
-                } else {
-                    dl = th_mfma<FMT>(qh[j], bv, dl);
-                    dl = th_mfma<FMT>(ql[j], bv, dl);
-                }
-                if constexpr (NP == 2) dl = th_mfma<FMT>(qh[j], *(const v4i *)(p + Sh::PlaneB), dl);
-            }
-            if constexpr (kQ8) {
-                const float x = scl[16 * rb + n];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) dl[i] = fmaf(dl[i], qd[i] * x, dk[i]);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sp[(size_t)(kh * NQ + 16 * m + 4 * g + i) * kThSp + 16 * rb + n] = dl[i];
+            d[rb] = dk[rb] = v4f{0.f, 0.f, 0.f, 0.f};
+            if constexpr (kQ8) x[rb] = *(const float *)(buf + NP * Sh::PlaneB + 4 * (16 * rb + n));
         }
-        lds_barrier();  // both halves of every score are in LDS
-        // ---- softmax
-        {
-            const v4f s0 = *(const v4f *)(sp + sq * kThSp + sr), s1 = *(const v4f *)(sp + (NQ + sq) * kThSp + sr);
-            const int nv = r1 - (r0 + c * kThCh) - sr;  // of this thread's rows, the ones in the split
-            v4f x, t, rs;
-            if constexpr (kQ8) {
-                rs = *(const v4f *)(scl + sr);
-                t = *(const v4f *)(scl + kThCh + sr);
-            }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[e] = e < nv ? s0[e] + s1[e] : -INFINITY;
-                t[e] = kQ8 ? x[e] + t[e] : x[e];
-            }
-            float cm = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-            cm = fmaxf(cm, dpp_f32<0xB1>(cm));
-            cm = fmaxf(cm, dpp_f32<0x4E>(cm));
-            cm = fmaxf(cm, dpp_f32<0x141>(cm));  // row_half_mirror: the other four of the eight
-            const bool mv = cm > m_run + 1.3862944f;
-            float alpha = 1.0f;
-            if (mv) {
-                alpha = __expf(m_run - cm);
-                m_run = cm;
-                l_run *= alpha;
-            }
-            if ((tid & 7) == 0) *(float *)(smem + Sh::AlOff + 4 * sq) = alpha;
-            const bool any = __any(mv);
-            if (l == 0) *(int *)(smem + Sh::FlOff + 32 * (c & 1) + 4 * w) = any ? 1 : 0;
-            v4f p;
-            float ps = 0.f;
+        for (int i = 0; i < W; ++i) bv[i] = get(i);
+        __builtin_amdgcn_sched_barrier(kThFree);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                p[e] = __expf(x[e] - m_run);
-                ps += p[e];
-                if constexpr (kQ8) p[e] *= rs[e];
+        for (int i = 0; i < N; ++i) {
+            const int j = i / (2 * NP), rb = i / NP % 2;
+            const v4i v = bv[i % W];
+            if (kQ8 && j == 8) {
+                dk[rb] = th_mfma<kFmtBF16>(qh[j], v, dk[rb]);
+                dk[rb] = th_mfma<kFmtBF16>(ql[j], v, dk[rb]);
+            } else {
+                d[rb] = th_mfma<FMT>(qh[j], v, d[rb]);
+                if (i % NP == 0) d[rb] = th_mfma<FMT>(ql[j], v, d[rb]);  // not lo . lo
             }
-            l_run += ps;  // this thread's rows; the eight threads' sums are added at the end
-            v4i hi, lo;
-            th_split<kQ8>(p, v4f{0.f, 0.f, 0.f, 0.f}, hi, lo);
-            *(int2 *)(smem + Sh::PwOff + sq * kThPw + 2 * sr) = int2{hi[0], hi[1]};
-            *(int2 *)(smem + Sh::PwOff + (NQ + sq) * kThPw + 2 * sr) = int2{lo[0], lo[1]};
+            if (i + W < N) bv[i % W] = get(i + W);
+            __builtin_amdgcn_sched_barrier(kThFree);
         }
-        if constexpr (Ring == 2) {
-            if (c + 1 < nch) stage(c + 1);
-            if (c + 2 < nch) fetch(c + 2);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            if constexpr (kQ8)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[rb][i] = fmaf(d[rb][i], qd[i] * x[rb], dk[rb][i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sp[32 * i + 16 * rb] = d[rb][i];
         }
-        lds_barrier();  // the weights (and the next chunk) are in LDS
-        // ---- mix
-        {
-            int any = 0;
+    };
+    // softmax of a chunk: its reads, then (after other work) its arithmetic and writes
+    v4f sx, st, sr4;
+    auto softmax_read = [&](const uint8_t *buf, int c) __attribute__((always_inline)) {
+        const float *scl = (const float *)(buf + NP * Sh::PlaneB);
+        const float *sp = (const float *)(smem + spr + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
+        const v4f s0 = *(const v4f *)sp, s1 = *(const v4f *)(sp + Sh::SpH);
+        if constexpr (kQ8) {
+            sr4 = *(const v4f *)(scl + sr);
+            st = *(const v4f *)(scl + kThCh + sr);
+        }
+        sx = s0 + s1;
+    };
+    auto softmax = [&](int c) __attribute__((always_inline)) {
+        const int nv = r1 - (r0 + c * kThCh) - sr;  // of this thread's rows, the ones in the split
+        v4f x, t;
 #pragma unroll
-            for (int i = 0; i < NW / 4; ++i) {
-                const v4i f = *(const v4i *)(smem + Sh::FlOff + 32 * (c & 1) + 16 * i);
-                any |= f[0] | f[1] | f[2] | f[3];
-            }
-            if (__builtin_amdgcn_readfirstlane(any)) {
+        for (int e = 0; e < 4; ++e) x[e] = e < nv ? sx[e] : -INFINITY;
+        t = x;
+        if constexpr (kQ8) t += st;
+        float cm = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        cm = fmaxf(cm, dpp_f32<0xB1>(cm));
+        cm = fmaxf(cm, dpp_f32<0x4E>(cm));
+        cm = fmaxf(cm, dpp_f32<0x141>(cm));  // row_half_mirror: the other four of the eight
+        const bool mv = cm > m_run + 2.0f;
+        const bool any = __any(mv);
+        const float alpha = mv ? __builtin_amdgcn_exp2f(m_run - cm) : 1.0f;
+        m_run = mv ? cm : m_run;
+        l_run *= alpha;
+        v4f p;
 #pragma unroll
-                for (int i = 0; i < NM; ++i) {
-                    const v4f al = *(const v4f *)(smem + Sh::AlOff + 64 * i + 16 * g);
+        for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - m_run);
+        l_run += (p[0] + p[1]) + (p[2] + p[3]);  // this thread's rows; the eight threads' sums are added at the end
+        if constexpr (kQ8) p *= sr4;
+        int2 hi, lo;
+        th_split4<kQ8>(p, hi, lo);
+        uint8_t *pw = smem + Sh::PwOff + th_pw(sq, sr >> 3) + 2 * (sr & 4);
+        *(int2 *)pw = hi;
+        *(int2 *)(pw + Sh::PwB) = lo;
+        if ((tid & 7) == 0) *(float *)(smem + Sh::AlOff + 4 * sq) = alpha;
+        if (l == 0) *(int *)(smem + Sh::FlOff + 32 * (c & 1) + 4 * w) = any ? 1 : 0;
+    };
+    auto mix = [&](const uint8_t *buf, int c) __attribute__((always_inline)) {
+        v4i f[NW / 4], ph[NM], pl[NM], bt[2][NP];
 #pragma unroll
-                    for (int t = 0; t < NC; ++t) acc[i][t] *= al;
-                }
-            }
-            v4i ph[NM], pl[NM];
+        for (int i = 0; i < NW / 4; ++i) f[i] = *(const v4i *)(smem + Sh::FlOff + 32 * (c & 1) + 16 * i);
+        auto get = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+            for (int z = 0; z < NP; ++z)
+                bt[t & 1][z] = __builtin_bit_cast(v4i, __builtin_shufflevector(lds_read_tr16(buf + z * Sh::PlaneB + tro[0][t]),
+                                                                               lds_read_tr16(buf + z * Sh::PlaneB + tro[1][t]), 0,
+                                                                               1, 2, 3, 4, 5, 6, 7));
+        };
+#pragma unroll
+        for (int i = 0; i < NM; ++i) {
+            ph[i] = *(const v4i *)(smem + Sh::PwOff + th_pw(16 * i + n, g));
+            if (i == 0) get(0);
+            pl[i] = *(const v4i *)(smem + Sh::PwOff + Sh::PwB + th_pw(16 * i + n, g));
+        }
+        get(1);
+        int any = 0;
+#pragma unroll
+        for (int i = 0; i < NW / 4; ++i) any |= f[i][0] | f[i][1] | f[i][2] | f[i][3];
+        if (__builtin_amdgcn_readfirstlane(any)) {
 #pragma unroll
             for (int i = 0; i < NM; ++i) {
-                ph[i] = *(const v4i *)(smem + Sh::PwOff + (16 * i + n) * kThPw + 16 * g);
-                pl[i] = *(const v4i *)(smem + Sh::PwOff + (NQ + 16 * i + n) * kThPw + 16 * g);
-            }
+                const v4f al = *(const v4f *)(smem + Sh::AlOff + 64 * i + 16 * g);
 #pragma unroll
-            for (int t = 0; t < NC; ++t) {
-                v4i bt[NP];
-#pragma unroll
-                for (int z = 0; z < NP; ++z)
-                    bt[z] = __builtin_bit_cast(v4i, __builtin_shufflevector(lds_read_tr16(buf + z * Sh::PlaneB + tro[0][t]),
-                                                                            lds_read_tr16(buf + z * Sh::PlaneB + tro[1][t]), 0, 1,
-                                                                            2, 3, 4, 5, 6, 7));
-#pragma unroll
-                for (int i = 0; i < NM; ++i) {
-                    acc[i][t] = th_mfma<FMT>(ph[i], bt[0], acc[i][t]);
-                    acc[i][t] = th_mfma<FMT>(pl[i], bt[0], acc[i][t]);
-                    if constexpr (NP == 2) acc[i][t] = th_mfma<FMT>(ph[i], bt[1], acc[i][t]);
-                }
+                for (int t = 0; t < NC; ++t) acc[i][t] *= al;
             }
         }
-        if constexpr (Ring == 1) {
+        __builtin_amdgcn_sched_barrier(kThFree);
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+                acc[i][t] = th_mfma<FMT>(ph[i], bt[t & 1][0], acc[i][t]);
+                if constexpr (NP == 2) acc[i][t] = th_mfma<FMT>(ph[i], bt[t & 1][1], acc[i][t]);
+            }
+#pragma unroll
+            for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(pl[i], bt[t & 1][0], acc[i][t]);
+            if (t + 2 < NC) get(t + 2);
+            __builtin_amdgcn_sched_barrier(kThFree);
+        }
+    };
+
+    if constexpr (Sh::Pipe) {
+        // Two barriers a chunk. Between them the waves hold a product and vector work that do not depend
+        // on each other: scores of chunk c + 1 beside the softmax of chunk c, then the mix of chunk c
+        // beside the staging of chunk c + 2. (The scores of the chunk past the last are not used.)
+        uint8_t *cur = smem, *next = smem + Sh::Slot, *then = smem + 2 * Sh::Slot;
+        if (nch > 1) stage(next);
+        if (nch > 2) fetch(2);
+        scores(cur, 0);
+        lds_barrier();
+        for (int c = 0; c < nch; ++c) {
+            softmax_read(cur, c);
+            scores(next, c + 1);
+            softmax(c);
+            lds_barrier();
+            mix(cur, c);
+            if (c + 2 < nch) stage(then);
+            if (c + 3 < nch) fetch(c + 3);
+            lds_barrier();
+            uint8_t *t = cur;
+            cur = next;
+            next = then;
+            then = t;
+        }
+    } else {
+        for (int c = 0; c < nch; ++c) {
+            scores(smem, c);
+            lds_barrier();  // both halves of every score are in LDS
+            softmax_read(smem, c);
+            softmax(c);
+            lds_barrier();  // the weights are in LDS
+            mix(smem, c);
             if (c + 1 < nch) {
                 lds_barrier();  // every wave is done with the chunk
-                stage(c + 1);
+                stage(smem);
                 if (c + 2 < nch) fetch(c + 2);
                 lds_barrier();
             }
@@ -582,24 +606,254 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
     for (int i = 0; i < NM; ++i) {
         if (i >= live) break;
-        float *P = a.part + (size_t)(s.part0 + (first + i) * (s.ns + 1) + split) * 16 * 514;
+        float *P = a.part + (size_t)(s.part0 + (first + i) * s.ns + split) * 16 * 514;
 #pragma unroll
         for (int t = 0; t < NC; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) P[(4 * g + e) * 512 + 16 * (NC * w + t) + n] = acc[i][t][e];
     }
     if ((tid & 7) == 0 && sq / 16 < live) {
-        float *P = a.part + (size_t)(s.part0 + (first + sq / 16) * (s.ns + 1) + split) * 16 * 514 + 8192;
-        P[sq % 16] = m_run;
+        float *P = a.part + (size_t)(s.part0 + (first + sq / 16) * s.ns + split) * 16 * 514 + 8192;
+        P[sq % 16] = m_run * 0.693147181f;  // in units of the natural logarithm
         P[16 + sq % 16] = l_run;
     }
 }
 
-// Splits of the history: as many rows per split (a multiple of the chunk, at least kThMin) as it takes for
-// the launch's workgroups, ceil(count / nm) per split, to be one round on the CUs.
+// ---- the nodes' own rows, the merge and W_UV (Kimi shapes, DV = 128) --------------------------------
+
+constexpr int kTcNodes = 4;  // nodes of a combine workgroup (at most)
+struct TreeCombArgs {
+    TreeRowsTable t;
+    TreeNodes nd;
+    const float *qf, *part;
+    const uint16_t *kv_b;
+    uint16_t *hos;
+    size_t plane;  // words between the hi and lo planes of hos
+    float smscale;
+    int DN, tn;  // tn: nodes per workgroup (1, 2, 4)
+};
+
+// Workgroup = one head of tn nodes, eight waves, 8 / tn of them per node (in turn over the history's splits).
+//   merge: mix = (sum_s e^(m_s - M) acc_s + the path's) / (sum_s e^(m_s - M) l_s + the path's), lane l columns
+//     4 l .. and 256 + 4 l ..;
+//   path: the node's first wave takes the node's own row and its ancestors' (rows ctx + i, at most 64), four at
+//     a time: scores in fp32 (row j's in lane j), their weights, their mix. Rows of other branches are not read;
+//   W_UV: head output d = sum_r W[d, r] mix[r] on MFMA, wave w rows 16 w .., its W operands requested at the
+//     start; the mix enters as three bf16 planes (24 bits), plane p of node j as column 4 p + j.
+// The output is written as the bf16 hi | lo planes that o_proj's launch takes.
+template <int FMT>
+__global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
+    constexpr int R = 512, DR = 64, NH = 16;
+    __shared__ __attribute__((aligned(16))) uint8_t xs[16 * 1024];  // column c's words of 8: word ^ (c & 15)
+    __shared__ __attribute__((aligned(16))) float red[8][R];
+    const int tid = threadIdx.x, l = tid & 63, n = l & 15, g = l >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = blockIdx.x % NH, tn = a.tn, first = blockIdx.x / NH * tn;
+    // this lane's entries of the tables
+    const TreeRows q = a.t.s[l];
+    const uint64_t lane_path = a.nd.path[l];
+    const int lane_seq = a.nd.seq[l];
+    const uint16_t *wrow = a.kv_b + ((size_t)h * (a.DN + 128) + a.DN + 16 * w + n) * R + 8 * g;
+    v4i wa[16];
+#pragma unroll
+    for (int kb = 0; kb < 16; ++kb) wa[kb] = *(const v4i *)(wrow + 32 * kb);
+    const int wpn = 8 / tn, j = w / wpn, u = w % wpn;  // node of the workgroup, turn
+    const int k = min(first + j, a.nd.n - 1);
+    const int b = tree_lane(lane_seq, k);
+    const TreeRows s{tree_lane(q.a, b), tree_lane(q.b, b), tree_lane(q.c, b), tree_lane(q.ctx, b), tree_lane(q.node0, b),
+                     tree_lane(q.part0, b), tree_lane(q.ns, b)};
+    const int ns = s.ns, i0 = a.nd.first + k - s.node0;
+    const float *P = a.part + (size_t)(s.part0 + i0 * ns) * (NH * (R + 2));
+    constexpr size_t stride = NH * (R + 2);
+    const float *Pm = P + NH * R + h, *Pa = P + h * R + 4 * l;
+
+    // ---- the history's splits: maximum, denominator, this wave's share of the sum
+    float mh = -INFINITY, den = 0.f;
+    for (int s0 = 0; s0 < ns; s0 += 64) mh = fmaxf(mh, s0 + l < ns ? Pm[(size_t)(s0 + l) * stride] : -INFINITY);
+    mh = wave_max(mh);
+    v4f c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
+    for (int s0 = 0; s0 < ns; s0 += 64) {
+        float e = 0.f, ls = 0.f;
+        if (s0 + l < ns) {
+            e = __expf(Pm[(size_t)(s0 + l) * stride] - mh);
+            ls = Pm[(size_t)(s0 + l) * stride + NH];
+        }
+        den = fmaf(ls, e, den);
+        const int top = min(64, ns - s0);
+        for (int t = u; t < top; t += 4 * wpn) {
+            v4f x0[4], x1[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float *p = Pa + (size_t)(s0 + min(t + r * wpn, top - 1)) * stride;
+                x0[r] = *(const v4f *)p;
+                x1[r] = *(const v4f *)(p + 256);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (t + r * wpn >= top) break;
+                const float wt = lane_f32(e, t + r * wpn);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    c0[z] = fmaf(x0[r][z], wt, c0[z]);
+                    c1[z] = fmaf(x1[r][z], wt, c1[z]);
+                }
+            }
+        }
+    }
+    den = wave_sum(den);
+    // ---- the path (the node's first wave)
+    float mp = -INFINITY, lp = 0.f;
+    v4f p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0;
+    if (u == 0) {
+        const uint32_t mlo = (uint32_t)tree_lane((int)(uint32_t)lane_path, k), mhi = (uint32_t)tree_lane((int)(uint32_t)(lane_path >> 32), k);
+        const uint64_t mask = ((uint64_t)mhi << 32) | mlo;
+        const float *qr = a.qf + ((size_t)(a.nd.first + k) * NH + h) * (R + DR);
+        const v4f q0 = *(const v4f *)(qr + 4 * l) * a.smscale, q1 = *(const v4f *)(qr + 256 + 4 * l) * a.smscale;
+        const float qk = qr[R + l] * a.smscale;
+        auto lat = [&](size_t row, v4f &x0, v4f &x1) __attribute__((always_inline)) {
+            if constexpr (FMT == kFmtQ8) {
+                const int8_t *p = (const int8_t *)s.a + row * R + 4 * l;
+                const int a0 = *(const int *)p, a1 = *(const int *)(p + 256);
+                const float sc = ((const float *)s.b)[row];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    x0[z] = (float)(int8_t)(a0 >> (8 * z)) * sc;
+                    x1[z] = (float)(int8_t)(a1 >> (8 * z)) * sc;
+                }
+            } else if constexpr (FMT == kFmtF32) {
+                const float *p = (const float *)s.a + row * R + 4 * l;
+                x0 = *(const v4f *)p;
+                x1 = *(const v4f *)(p + 256);
+            } else {
+                const uint16_t *p = (const uint16_t *)s.a + row * R + 4 * l;
+                const uint2 a0 = *(const uint2 *)p, a1 = *(const uint2 *)(p + 256);
+                x0 = v4f{__uint_as_float(a0.x << 16), __uint_as_float(a0.x & 0xffff0000u), __uint_as_float(a0.y << 16), __uint_as_float(a0.y & 0xffff0000u)};
+                x1 = v4f{__uint_as_float(a1.x << 16), __uint_as_float(a1.x & 0xffff0000u), __uint_as_float(a1.y << 16), __uint_as_float(a1.y & 0xffff0000u)};
+            }
+        };
+        const int np = __builtin_popcountll(mask);
+        // four rows at a time; rows past the path's end repeat its last
+        auto four = [&](uint64_t &m, size_t *row) __attribute__((always_inline)) {
+            int last = 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (m) last = __builtin_ctzll(m);
+                m &= m - 1;
+                row[r] = (size_t)s.ctx + last;
+            }
+        };
+        float sc = -INFINITY;
+        uint64_t m = mask;
+        for (int t = 0; t < np; t += 4) {
+            size_t row[4];
+            four(m, row);
+            float v[4];
+            v4f x0[4], x1[4];
+            float xk[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                lat(row[r], x0[r], x1[r]);
+                xk[r] = tree_key<FMT>(s, row[r], DR, l);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                v[r] = qk * xk[r];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) v[r] = fmaf(q1[z], x1[r][z], fmaf(q0[z], x0[r][z], v[r]));
+                v[r] = wave_sum(v[r]);
+                if (l == t + r && t + r < np) sc = v[r];
+            }
+        }
+        mp = wave_max(sc);
+        const float e = l < np ? __expf(sc - mp) : 0.f;
+        lp = wave_sum(e);
+        m = mask;
+        for (int t = 0; t < np; t += 4) {
+            size_t row[4];
+            four(m, row);
+            v4f x0[4], x1[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) lat(row[r], x0[r], x1[r]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (t + r >= np) break;
+                const float wt = lane_f32(e, t + r);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    p0[z] = fmaf(x0[r][z], wt, p0[z]);
+                    p1[z] = fmaf(x1[r][z], wt, p1[z]);
+                }
+            }
+        }
+    }
+    if (wpn > 1) {  // the node's waves in turn order
+        *(v4f *)&red[w][4 * l] = c0;
+        *(v4f *)&red[w][256 + 4 * l] = c1;
+        __syncthreads();
+        if (u == 0)
+            for (int t = 1; t < wpn; ++t) {
+                c0 += *(const v4f *)&red[w + t][4 * l];
+                c1 += *(const v4f *)&red[w + t][256 + 4 * l];
+            }
+    }
+    if (u == 0) {
+        const float M = fmaxf(mh, mp);
+        const float eh = ns > 0 ? __expf(mh - M) : 0.f, ep = __expf(mp - M);
+        const float inv = 1.0f / fmaf(den, eh, lp * ep);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const v4f c = half ? c1 : c0, p = half ? p1 : p0;
+            v4f x;
+#pragma unroll
+            for (int z = 0; z < 4; ++z) x[z] = fmaf(c[z], eh, p[z] * ep) * inv;
+#pragma unroll
+            for (int pl = 0; pl < 3; ++pl) {
+                const v2bf b0 = __builtin_convertvector((v2f{x[0], x[1]}), v2bf), b1 = __builtin_convertvector((v2f{x[2], x[3]}), v2bf);
+                const int col = kTcNodes * pl + j;
+                *(int2 *)(xs + col * 1024 + 16 * ((32 * half + (l >> 1)) ^ col) + 8 * (l & 1)) =
+                    int2{__builtin_bit_cast(int, b0), __builtin_bit_cast(int, b1)};
+                x -= v4f{(float)b0.x, (float)b0.y, (float)b1.x, (float)b1.y};
+            }
+        }
+    }
+    __syncthreads();
+    v4f acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int kb = 0; kb < 16; ++kb)
+        acc = mfma_bf16(__builtin_bit_cast(v8bf, wa[kb]), *(const v8bf *)(xs + n * 1024 + 16 * ((4 * kb + g) ^ n)), acc);
+    // columns j, 4 + j, 8 + j are the planes of node j (columns without one are not used)
+    const int node = first + n;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float mid = dpp_f32<0x12C>(acc[i]), low = dpp_f32<0x128>(acc[i]);  // row_ror:12, row_ror:8: lanes n + 4, n + 8
+        const float v = acc[i] + (mid + low);
+        if (n < tn && node < a.nd.n) {
+            uint16_t hi, lo;
+            split_bf16(v, hi, lo);
+            const size_t o = (size_t)(a.nd.first + node) * (NH * 128) + h * 128 + 16 * w + 4 * g + i;
+            a.hos[o] = hi;
+            a.hos[a.plane + o] = lo;
+        }
+    }
+}
+
+// Splits of the history: the fewest rows per split (a multiple of the chunk, at least kThMin) whose
+// workgroups, ceil(count / nm) per split, are one round on the CUs of every XCD.
 constexpr int kThMin = 64;
+static int tree_fullest(const TreeTable &t) {  // workgroups of the fullest XCD (tree_unit)
+    int most = 0;
+    for (int x = 0; x < 8; ++x) {
+        int n = 0;
+        for (int b = 0; b < t.n; ++b) {
+            const int first = (x - t.s[b].unit0) & 7;
+            if (t.s[b].ns > first) n += (t.s[b].ns - first + 7) / 8 * t.s[b].tiles;
+        }
+        most = std::max(most, n);
+    }
+    return most;
+}
 int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
-    const bool kimi = d.NH == 16 && d.R == 512 && d.DR == 64;
+    const bool kimi = d.NH == 16 && d.R == 512 && d.DR == 64 && d.DV == 128;
     int most = 0, longest = 0;
     for (int b = 0; b < t.n; ++b) {
         most = std::max(most, t.s[b].count);
@@ -607,78 +861,99 @@ int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
     }
     t.nm = !kimi ? 0 : most > 2 || fmt == kFmtF32 ? 4 : 2;
     auto splits = [](long ctx, long r) { return (ctx + r - 1) / r; };
-    long r = kThMin;
-    if (t.nm) {
-        const long places = (long)ncu * (t.nm == 2 ? 2 : 1);
-        auto groups = [&](long rows) {
-            long n = 0;
-            for (int b = 0; b < t.n; ++b) n += (t.s[b].count + t.nm - 1) / t.nm * splits(t.s[b].ctx, rows);
-            return n;
-        };
-        long lo = kThMin / kThCh, hi = std::max(lo, splits(longest, kThCh));
-        while (lo < hi) {  // groups() does not increase with the rows
-            const long mid = (lo + hi) / 2;
-            if (groups(mid * kThCh) <= places) hi = mid;
-            else lo = mid + 1;
+    auto lay = [&](long r) {  // partials
+        int part = 0, unit = 0;
+        for (int b = 0; b < t.n; ++b) {
+            TreeSeq &s = t.s[b];
+            s.rps = (int)r;
+            s.ns = t.nm ? (int)splits(s.ctx, r) : 0;
+            s.tiles = t.nm ? (s.count + t.nm - 1) / t.nm : 0;
+            s.part0 = part;
+            s.unit0 = unit;
+            part += s.count * (t.nm ? s.ns : 1);
+            unit += s.ns;
         }
-        // the combine takes at most kMaxSplits partials of a node
-        r = std::max(lo * kThCh, (splits(longest, kMaxSplits - 1) + kThCh - 1) / kThCh * kThCh);
+        return part;
+    };
+    if (!t.nm) return lay(kThMin);
+    const long per = t.nm == 2 ? 2 : 1, places = ncu * per;
+    auto groups = [&](long rows) {
+        long n = 0;
+        for (int b = 0; b < t.n; ++b) n += (t.s[b].count + t.nm - 1) / t.nm * splits(t.s[b].ctx, rows);
+        return n;
+    };
+    long lo = kThMin / kThCh, hi = std::max(lo, splits(longest, kThCh));
+    while (lo < hi) {  // groups() does not increase with the rows
+        const long mid = (lo + hi) / 2;
+        if (groups(mid * kThCh) <= places) hi = mid;
+        else lo = mid + 1;
     }
-    int part = 0, unit = 0;
-    for (int b = 0; b < t.n; ++b) {
-        TreeSeq &s = t.s[b];
-        s.rps = (int)r;
-        s.ns = t.nm ? (int)splits(s.ctx, r) : 0;
-        s.tiles = t.nm ? (s.count + t.nm - 1) / t.nm : 0;
-        s.part0 = part;
-        s.unit0 = unit;
-        part += s.count * (s.ns + 1);
-        unit += s.ns;
+    // from there on, the first length whose fullest XCD has no second round; a quarter more rows at most
+    long best = lo;
+    for (long c = lo; c <= lo + lo / 4 && c - lo < 32; ++c) {
+        lay(c * kThCh);
+        if (tree_fullest(t) <= places / 8) {
+            best = c;
+            break;
+        }
     }
-    return part;
+    return lay(best * kThCh);
 }
 
 template <int FMT>
-static void tree_launch(hipStream_t st, const TreeArgs &a) {
-    if (a.t.nm == 0) {
-        hipLaunchKernelGGL(k_tree_generic<FMT>, dim3((unsigned)(a.t.nodes * a.d.NH)), dim3(256), 0, st, a);
-        return;
-    }
-    hipLaunchKernelGGL(k_tree_path<FMT>, dim3((unsigned)a.t.nodes), dim3(512), 0, st, a);
-    int most = 0;  // workgroups of the fullest XCD (tree_unit)
-    for (int x = 0; x < 8; ++x) {
-        int n = 0;
-        for (int b = 0; b < a.t.n; ++b) {
-            const int first = (x - a.t.s[b].unit0) & 7;
-            if (a.t.s[b].ns > first) n += (a.t.s[b].ns - first + 7) / 8 * a.t.s[b].tiles;
-        }
-        most = std::max(most, n);
-    }
-    if (most == 0) return;  // no history
-    const dim3 grid((unsigned)(8 * most));
+static void tree_launch(hipStream_t st, const TreeArgs &a, unsigned grid) {
     if constexpr (FMT != kFmtF32) {
         if (a.t.nm == 2) {
-            hipLaunchKernelGGL((k_tree_hist<FMT, 2>), grid, dim3(256), 0, st, a);
+            hipLaunchKernelGGL((k_tree_hist<FMT, 2>), dim3(grid), dim3(256), 0, st, a);
             return;
         }
     }
-    hipLaunchKernelGGL((k_tree_hist<FMT, 4>), grid, dim3(512), 0, st, a);
+    hipLaunchKernelGGL((k_tree_hist<FMT, 4>), dim3(grid), dim3(512), 0, st, a);
 }
 
-hipError_t launch_tree_attention(hipStream_t st, int fmt, const TreeTable &t, const Dims &d, const DecodeWork &w) {
-    if (d.R > 256 * kTgCols || d.DR > 256 || t.n < 1 || t.nodes < 1 || t.nodes > kTreeNodes) return hipErrorInvalidValue;
-    if (t.nm != 0 && (d.NH != 16 || d.R != 512 || d.DR != 64)) return hipErrorInvalidValue;
-    if (t.nm != 0 && t.nm != 4 && (t.nm != 2 || fmt == kFmtF32)) return hipErrorInvalidValue;
-    TreeArgs a;
-    a.t = t;
-    a.d = d;
-    a.qf = w.qf;
-    a.part = w.part;
-    a.smscale = 1.0f / sqrtf((float)d.QD);
-    if (fmt == kFmtQ8) tree_launch<kFmtQ8>(st, a);
-    else if (fmt == kFmtF32) tree_launch<kFmtF32>(st, a);
-    else if (fmt == kFmtBF16) tree_launch<kFmtBF16>(st, a);
-    else return hipErrorInvalidValue;
+static bool tree_table_ok(int fmt, const TreeTable &t, const Dims &d, bool kimi) {
+    if (t.n < 1 || t.n > kMaxBatch || t.nodes < 1 || t.nodes > kTreeGroup) return false;
+    if (fmt != kFmtQ8 && fmt != kFmtF32 && fmt != kFmtBF16) return false;
+    if (!kimi) return t.nm == 0 && d.R <= 256 * kTgCols && d.DR <= 256;
+    return (t.nm == 4 || (t.nm == 2 && fmt != kFmtF32)) && d.NH == 16 && d.R == 512 && d.DR == 64 && d.DV == 128;
+}
+
+hipError_t launch_tree_history(hipStream_t st, int fmt, const TreeTable &t, const Dims &d, const DecodeWork &w) {
+    if (!tree_table_ok(fmt, t, d, true)) return hipErrorInvalidValue;
+    const int most = tree_fullest(t);
+    if (most == 0) return hipSuccess;  // no history
+    const TreeArgs a{t, w.qf, w.part, 1.0f / sqrtf((float)d.QD)};
+    if (fmt == kFmtQ8) tree_launch<kFmtQ8>(st, a, 8u * most);
+    else if (fmt == kFmtF32) tree_launch<kFmtF32>(st, a, 8u * most);
+    else tree_launch<kFmtBF16>(st, a, 8u * most);
+    return hipGetLastError();
+}
+
+hipError_t launch_tree_combine(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
+                               const uint16_t *kv_b, const DecodeWork &w) {
+    if (!tree_table_ok(fmt, t, d, true) || nd.n < 1 || nd.n > kTreeNodes || nd.first < 0 || nd.first + nd.n > t.nodes)
+        return hipErrorInvalidValue;
+    TreeCombArgs a{tree_rows(t), nd, w.qf, w.part, kv_b, w.hos, (size_t)t.nodes * d.HO, 1.0f / sqrtf((float)d.QD), d.DN, 1};
+    // nodes per workgroup: enough workgroups for the CUs first, then W_UV (128 KB a workgroup) shared by more
+    a.tn = nd.n <= 16 ? 1 : nd.n <= 32 ? 2 : 4;
+    const dim3 grid((unsigned)((nd.n + a.tn - 1) / a.tn * 16));
+    if (fmt == kFmtQ8) hipLaunchKernelGGL(k_tree_combine<kFmtQ8>, grid, dim3(512), 0, st, a);
+    else if (fmt == kFmtF32) hipLaunchKernelGGL(k_tree_combine<kFmtF32>, grid, dim3(512), 0, st, a);
+    else hipLaunchKernelGGL(k_tree_combine<kFmtBF16>, grid, dim3(512), 0, st, a);
+    return hipGetLastError();
+}
+
+static_assert(sizeof(TreeCombArgs) <= 4096 && sizeof(TreeNodeArgs) <= 4096 && sizeof(TreeArgs) <= 4096, "kernel arguments");
+
+hipError_t launch_tree_generic(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
+                               const DecodeWork &w) {
+    if (!tree_table_ok(fmt, t, d, false) || nd.n < 1 || nd.n > kTreeNodes || nd.first < 0 || nd.first + nd.n > t.nodes)
+        return hipErrorInvalidValue;
+    const TreeNodeArgs a{tree_rows(t), nd, w.qf, w.part, 1.0f / sqrtf((float)d.QD), d.NH, d.R, d.DR};
+    const dim3 grid((unsigned)(nd.n * d.NH));
+    if (fmt == kFmtQ8) hipLaunchKernelGGL(k_tree_generic<kFmtQ8>, grid, dim3(256), 0, st, a);
+    else if (fmt == kFmtF32) hipLaunchKernelGGL(k_tree_generic<kFmtF32>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(k_tree_generic<kFmtBF16>, grid, dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
