@@ -252,11 +252,12 @@ struct TreeSeq {
     int node0;        // the tree's first node among the group's
     int part0;        // its first partial: node i's are part0 + i * ns .. (ns = 0: part0 + i, of all its rows)
     int ns, rps;      // the history in ns splits of rps rows (the last: the rest)
-    int tiles, unit0; // ceil(count / nm); the splits of the sequences before it
+    int tiles, unit0; // ceil(count / nm); the history workgroups of the sequences before it
 };
 struct TreeTable {
     TreeSeq s[kMaxBatch];
     int n, nodes;
+    int units;  // history workgroups
     int nm;  // nodes per history workgroup (2 or 4); 0: the route for any dims (every row in one partial)
 };
 struct TreeNodes {  // nodes first .. first + n - 1 of the group

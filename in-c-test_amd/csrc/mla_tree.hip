@@ -2,6 +2,8 @@
 // over a latent history, copies of a state's rows, and the compaction of an accepted path's rows.
 #include <hip/hip_runtime.h>
 
+#include <limits.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -182,10 +184,11 @@ __device__ __forceinline__ int th_pw(int q, int word) {
 // word c of key row r
 __device__ __forceinline__ int th_key(int r, int c) { return r * 128 + 16 * (c ^ ((r >> 1) & 7)); }
 
-// Workgroup -> (sequence, split, tile). Workgroup i runs on XCD i % 8; the units (a sequence's split) go
-// to the XCDs in turn, and the tiles of a unit follow one another on its XCD, so that its L2 serves the
-// rows they share. Lane b of every wave reads sequence b's entry and counts what it has on this XCD; the
-// workgroup's entry then comes from its lane, in scalar registers.
+// Workgroup -> (sequence, split, tile). The workgroups of a launch, sequence by sequence, split by split,
+// the tiles of a split one after another, are cut into eight equal runs, one per XCD (workgroup i runs on
+// XCD i % 8): an XCD's L2 serves the rows that the tiles of a split share, and no XCD has more workgroups
+// than another. Lane b of every wave reads sequence b's entry; the workgroup's entry then comes from its
+// lane, in scalar registers.
 __device__ __forceinline__ int tree_lane(int v, int b) { return __builtin_amdgcn_readlane(v, b); }
 __device__ __forceinline__ uint8_t *tree_lane(void *p, int b) {
     const uint64_t u = (uint64_t)p;
@@ -199,19 +202,12 @@ struct TreeUnit {
 __device__ __forceinline__ bool tree_unit(const TreeTable &t, TreeUnit &u) {
     const int lane = threadIdx.x & 63, xcd = blockIdx.x & 7, j = blockIdx.x >> 3;
     const TreeSeq q = t.s[lane];
-    const int live = lane < t.n ? 1 : 0, ns = live ? q.ns : 0;
-    const int first = (xcd - q.unit0) & 7;  // the first of its splits on this XCD
-    const int mine = (ns > first ? (ns - first + 7) / 8 : 0) * q.tiles;
-    int sum = mine;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int v = __shfl_up(sum, o);
-        if (lane >= o) sum += v;
-    }
-    if (j >= tree_lane(sum, 63)) return false;
-    const int b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(sum <= j));
-    const int r = j - tree_lane(sum - mine, b), tiles = tree_lane(q.tiles, b);
-    u.split = tree_lane(first, b) + 8 * (r / tiles);
+    const int each = t.units >> 3, more = t.units & 7;
+    if (j >= each + (xcd < more ? 1 : 0)) return false;
+    const int i = xcd * each + min(xcd, more) + j;
+    const int b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane > 0 && lane < t.n && i >= q.unit0));
+    const int r = i - tree_lane(q.unit0, b), tiles = tree_lane(q.tiles, b);
+    u.split = r / tiles;
     u.tile = r % tiles;
     u.a = tree_lane(q.a, b);
     u.b = tree_lane(q.b, b);
@@ -837,21 +833,11 @@ __global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
     }
 }
 
-// Splits of the history: the fewest rows per split (a multiple of the chunk, at least kThMin) whose
-// workgroups, ceil(count / nm) per split, are one round on the CUs of every XCD.
-constexpr int kThMin = 64;
-static int tree_fullest(const TreeTable &t) {  // workgroups of the fullest XCD (tree_unit)
-    int most = 0;
-    for (int x = 0; x < 8; ++x) {
-        int n = 0;
-        for (int b = 0; b < t.n; ++b) {
-            const int first = (x - t.s[b].unit0) & 7;
-            if (t.s[b].ns > first) n += (t.s[b].ns - first + 7) / 8 * t.s[b].tiles;
-        }
-        most = std::max(most, n);
-    }
-    return most;
-}
+// Splits of the history, r rows each (a multiple of the chunk, at least kThMin). A launch of k rounds of
+// workgroups (ceil(count / nm) per split) on the CUs takes about k (r / kThCh + kThStart) chunks' time, the
+// start of a workgroup (its queries, its first chunk) being worth kThStart chunks: for each k up to
+// kThRounds the fewest rows that make k rounds, and of these the shortest.
+constexpr int kThMin = 64, kThStart = 4, kThRounds = 4;
 int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
     const bool kimi = d.NH == 16 && d.R == 512 && d.DR == 64 && d.DV == 128;
     int most = 0, longest = 0;
@@ -861,43 +847,46 @@ int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
     }
     t.nm = !kimi ? 0 : most > 2 || fmt == kFmtF32 ? 4 : 2;
     auto splits = [](long ctx, long r) { return (ctx + r - 1) / r; };
-    auto lay = [&](long r) {  // partials
-        int part = 0, unit = 0;
-        for (int b = 0; b < t.n; ++b) {
-            TreeSeq &s = t.s[b];
-            s.rps = (int)r;
-            s.ns = t.nm ? (int)splits(s.ctx, r) : 0;
-            s.tiles = t.nm ? (s.count + t.nm - 1) / t.nm : 0;
-            s.part0 = part;
-            s.unit0 = unit;
-            part += s.count * (t.nm ? s.ns : 1);
-            unit += s.ns;
-        }
-        return part;
-    };
-    if (!t.nm) return lay(kThMin);
-    const long per = t.nm == 2 ? 2 : 1, places = ncu * per;
-    auto groups = [&](long rows) {
-        long n = 0;
-        for (int b = 0; b < t.n; ++b) n += (t.s[b].count + t.nm - 1) / t.nm * splits(t.s[b].ctx, rows);
-        return n;
-    };
-    long lo = kThMin / kThCh, hi = std::max(lo, splits(longest, kThCh));
-    while (lo < hi) {  // groups() does not increase with the rows
-        const long mid = (lo + hi) / 2;
-        if (groups(mid * kThCh) <= places) hi = mid;
-        else lo = mid + 1;
-    }
-    // from there on, the first length whose fullest XCD has no second round; a quarter more rows at most
-    long best = lo;
-    for (long c = lo; c <= lo + lo / 4 && c - lo < 32; ++c) {
-        lay(c * kThCh);
-        if (tree_fullest(t) <= places / 8) {
-            best = c;
-            break;
+    long best = kThMin / kThCh;  // in chunks
+    if (t.nm) {
+        const long places = (long)ncu * (t.nm == 2 ? 2 : 1);
+        auto groups = [&](long chunks) {
+            long n = 0;
+            for (int b = 0; b < t.n; ++b) n += (t.s[b].count + t.nm - 1) / t.nm * splits(t.s[b].ctx, chunks * kThCh);
+            return n;
+        };
+        // the combine's table of a node's splits; also keeps offsets within a split below 2^31 bytes
+        const long least = std::max<long>(kThMin / kThCh, splits(splits(longest, kMaxSplits), kThCh));
+        long cost = LONG_MAX, hi = std::max(least, splits(longest, kThCh));
+        for (int k = 1; k <= kThRounds; ++k) {
+            long lo = least, up = hi;
+            while (lo < up) {  // groups() does not increase with the chunks
+                const long mid = (lo + up) / 2;
+                if (groups(mid) <= k * places) up = mid;
+                else lo = mid + 1;
+            }
+            const long c = k * (lo + kThStart);
+            if (c < cost) {
+                cost = c;
+                best = lo;
+            }
+            hi = lo;  // more rounds need no more rows
+            if (lo == least) break;
         }
     }
-    return lay(best * kThCh);
+    int part = 0;
+    t.units = 0;
+    for (int b = 0; b < t.n; ++b) {
+        TreeSeq &s = t.s[b];
+        s.rps = (int)(best * kThCh);
+        s.ns = t.nm ? (int)splits(s.ctx, s.rps) : 0;
+        s.tiles = t.nm ? (s.count + t.nm - 1) / t.nm : 1;
+        s.part0 = part;
+        s.unit0 = t.units;
+        part += s.count * (t.nm ? s.ns : 1);
+        t.units += s.ns * s.tiles;
+    }
+    return part;
 }
 
 template <int FMT>
@@ -920,12 +909,12 @@ static bool tree_table_ok(int fmt, const TreeTable &t, const Dims &d, bool kimi)
 
 hipError_t launch_tree_history(hipStream_t st, int fmt, const TreeTable &t, const Dims &d, const DecodeWork &w) {
     if (!tree_table_ok(fmt, t, d, true)) return hipErrorInvalidValue;
-    const int most = tree_fullest(t);
-    if (most == 0) return hipSuccess;  // no history
+    if (t.units == 0) return hipSuccess;  // no history
+    const unsigned grid = 8u * (unsigned)((t.units + 7) / 8);
     const TreeArgs a{t, w.qf, w.part, 1.0f / sqrtf((float)d.QD)};
-    if (fmt == kFmtQ8) tree_launch<kFmtQ8>(st, a, 8u * most);
-    else if (fmt == kFmtF32) tree_launch<kFmtF32>(st, a, 8u * most);
-    else tree_launch<kFmtBF16>(st, a, 8u * most);
+    if (fmt == kFmtQ8) tree_launch<kFmtQ8>(st, a, grid);
+    else if (fmt == kFmtF32) tree_launch<kFmtF32>(st, a, grid);
+    else tree_launch<kFmtBF16>(st, a, grid);
     return hipGetLastError();
 }
 
