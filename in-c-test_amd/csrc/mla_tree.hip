@@ -148,7 +148,6 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 // whatever the scales, the running maximum is that of score + ln(scale), so that weight times scale stays
 // <= 4.
 constexpr int kThCh = 32;       // rows of a chunk
-constexpr int kThFree = 0x16;   // sched_barrier: vector, scalar and global memory instructions may cross
 template <int FMT, int NM>
 struct ThShape {
     static constexpr int NW = 2 * NM, NT = 64 * NW, NQ = 16 * NM;
@@ -297,41 +296,41 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int first = tile * NM, live = min(NM, s.count - first);  // nodes of this tile
 
     // ---- staging: a chunk's rows from memory to registers, and from there to an LDS slot. A thread
-    // takes eight values at a time: word tid % 64 of latent rows tid / 64 + NW i, word tid % 8 of key rows
-    // tid / 8 + NT / 8 i. Row j's word c lies at word c ^ th_swz(j). Rows past the split's end repeat its
-    // last row (their scores are masked).
-    constexpr int NL = kThCh / NW, NK = (256 + NT - 1) / NT;
+    // takes eight values of a latent row (word tid % 64 of rows tid / 64 + NW i) and four of a key row (half a
+    // word: tid % 16 of rows tid / 16 + NT / 16 i).
+    constexpr int NL = kThCh / NW, NK = 512 / NT;
     constexpr int LE = kQ8 ? 1 : FMT == kFmtF32 ? 4 : 2, KE = FMT == kFmtF32 ? 4 : 2;  // bytes of an element
-    constexpr int LV = LE == 4 ? 2 : 1, KV = KE == 4 ? 2 : 1;
-    v4i la[kQ8 ? 1 : NL * LV], ka[NK * KV];
-    v2i lc[kQ8 ? NL : 1];
-    float rsc = 0.f;
-    const int lrow = tid >> 6, krow = tid >> 3;
+    constexpr int LV = LE == 4 ? 2 : 1;
+    struct Held {
+        v4i la[kQ8 ? 1 : NL * LV], kf[KE == 4 ? NK : 1];
+        v2i lc[kQ8 ? NL : 1], kb[KE == 4 ? 1 : NK];
+        float rsc;
+    };
+    const int lrow = tid >> 6, krow = tid >> 4;
     // the split's rows as buffers: a read past the last row gives zeros (its score is masked)
     const int nrow = r1 - r0;
     const auto ba = __builtin_amdgcn_make_buffer_rsrc(s.a + (size_t)r0 * (512 * LE), 0, nrow * (512 * LE), 0x00027000);
     const auto bk = __builtin_amdgcn_make_buffer_rsrc((kQ8 ? s.c : s.b) + (size_t)r0 * (64 * KE), 0, nrow * (64 * KE), 0x00027000);
     const auto bs = __builtin_amdgcn_make_buffer_rsrc(s.b + (size_t)r0 * 4, 0, kQ8 ? nrow * 4 : 0, 0x00027000);
-    const int va = tid * (8 * LE), vk = tid * (8 * KE);  // rows lie one after another, so do the threads' words
-    auto fetch = [&](int c) __attribute__((always_inline)) {
+    const int va = tid * (8 * LE), vk = tid * (4 * KE);  // rows lie one after another, so do the threads' words
+    auto fetch = [&](int c, Held &f) __attribute__((always_inline)) {
         const int oa = va + c * (kThCh * 512 * LE), ok = vk + c * (kThCh * 64 * KE);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             if constexpr (kQ8)
-                lc[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(ba, oa + i * (NT * 8 * LE), 0, 0));
+                f.lc[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(ba, oa + i * (NT * 8 * LE), 0, 0));
             else
 #pragma unroll
                 for (int v = 0; v < LV; ++v)
-                    la[LV * i + v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ba, oa + i * (NT * 8 * LE) + 16 * v, 0, 0));
+                    f.la[LV * i + v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ba, oa + i * (NT * 8 * LE) + 16 * v, 0, 0));
         }
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
-            if (NT <= 256 || tid < 256)
-#pragma unroll
-                for (int v = 0; v < KV; ++v)
-                    ka[KV * i + v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(bk, ok + i * (NT * 8 * KE) + 16 * v, 0, 0));
+        for (int i = 0; i < NK; ++i) {
+            if constexpr (KE == 4) f.kf[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(bk, ok + i * (NT * 4 * KE), 0, 0));
+            else f.kb[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(bk, ok + i * (NT * 4 * KE), 0, 0));
+        }
         if constexpr (kQ8)
-            rsc = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(bs, 4 * (c * kThCh + (tid & 31)), 0, 0));
+            f.rsc = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(bs, 4 * (c * kThCh + (tid & 31)), 0, 0));
     };
     auto put = [&](uint8_t *at, const v4i *v) __attribute__((always_inline)) {
         if constexpr (NP == 2) {
@@ -343,28 +342,43 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             *(v4i *)at = v[0];
         }
     };
-    const int sa = lrow * 1024 + 16 * (l ^ th_swz(lrow)), sk = Sh::LatB + th_key(krow, tid & 7);
-    auto stage = [&](uint8_t *buf) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            // row lrow + NW i: b16_swz changes by the bits of NW i below 16
+    const int sa = lrow * 1024 + 16 * (l ^ th_swz(lrow)), sk = Sh::LatB + th_key(krow, (tid & 15) >> 1) + 8 * (tid & 1);
+    // piece i < NL: a latent item; the last piece: the key items and the scales
+    auto stage = [&](uint8_t *buf, const Held &f, int i) __attribute__((always_inline)) {
+        if (i < NL) {
+            // row lrow + NW i: th_swz changes by the bits of NW i below 16
             uint8_t *at = buf + (sa ^ (16 * th_swz((NW * i) & 15))) + NW * i * 1024;
-            if constexpr (kQ8) *(v4i *)at = codes_f16(lc[i]);
-            else put(at, la + LV * i);
+            if constexpr (kQ8) *(v4i *)at = codes_f16(f.lc[i]);
+            else put(at, f.la + LV * i);
+            return;
         }
 #pragma unroll
-        for (int i = 0; i < NK; ++i)
-            if (NT <= 256 || tid < 256) put(buf + sk + i * (NT / 8) * 128, ka + KV * i);
+        for (int q = 0; q < NK; ++q) {
+            if constexpr (KE == 4) {
+                int2 hi, lo;
+                th_split4<false>(__builtin_bit_cast(v4f, f.kf[q]), hi, lo);
+                *(int2 *)(buf + sk + q * (NT / 16) * 128) = hi;
+                *(int2 *)(buf + Sh::PlaneB + sk + q * (NT / 16) * 128) = lo;
+            } else {
+                *(v2i *)(buf + sk + q * (NT / 16) * 128) = f.kb[q];
+            }
+        }
         if constexpr (kQ8) {
             if (tid < kThCh) {
                 float *sc = (float *)(buf + NP * Sh::PlaneB);
-                sc[tid] = rsc;
-                sc[kThCh + tid] = __log2f(fmaxf(fabsf(rsc), 1e-35f));
+                sc[tid] = f.rsc;
+                sc[kThCh + tid] = __builtin_amdgcn_logf(fmaxf(fabsf(f.rsc), 1e-35f));
             }
         }
     };
+    auto stage_all = [&](uint8_t *buf, const Held &f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i <= NL; ++i) stage(buf, f, i);
+    };
 
-    fetch(0);
+    Held held, ahead;  // the first two chunks are requested together
+    fetch(0, ahead);
+    fetch(1, held);
     // ---- queries: A operand of the scores, head n of node m: columns 32 kb + 8 g .. of the eight
     // latent blocks kb = 8 kh + j and of the key block kh (j = 8). Scores are in units of log2.
     const int m = w % NM, kh = w / NM;
@@ -389,10 +403,11 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(qv[j][e]));
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            // 2^(10 - e) with 2^(e - 1) <= mx < 2^e, kept within the normal exponents
-            const int e = mx > 0.f && mx < INFINITY ? min(max(ilogbf(mx) + 1, -100), 100) : 10;
-            qs = ldexpf(1.0f, 10 - e);
-            const float qi = ldexpf(1.0f, e - 10);
+            // 2^(10 - e) with 2^(e - 1) <= mx < 2^e, from the exponent's bits, kept within 2^+-100 (zero and
+            // values that are not finite among them)
+            const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255) - 126, -90), 100);
+            qs = __uint_as_float((uint32_t)(137 - e) << 23);
+            const float qi = __uint_as_float((uint32_t)(117 + e) << 23);
 #pragma unroll
             for (int i = 0; i < 4; ++i) qd[i] = __shfl(qi, 4 * g + i);
         }
@@ -400,8 +415,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         for (int j = 0; j < 8; ++j) th_split<kQ8>(qv[2 * j] * qs, qv[2 * j + 1] * qs, qh[j], ql[j]);
         th_split<false>(qv[16], qv[17], qh[8], ql[8]);
     }
-    stage(smem);
-    if (nch > 1) fetch(1);
+    stage_all(smem, ahead);
 
     // score operands: row n of a 16-row half (16 KB / 2 KB apart), block j at bofs[j % 4] + 256 (j / 4)
     int bofs[4];
@@ -418,7 +432,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             tro[h][t] = row * 1024 + 16 * ((2 * (NC * w + t) + ((n >> 1) & 1)) ^ th_swz(row)) + 8 * (n & 1);
     }
     const int sq = tid >> 3, sr = 4 * (tid & 7);  // softmax: this thread's query and rows
-    float m_run = -INFINITY, l_run = 0.f;
+    float m_run = -1e30f, l_run = 0.f;  // (a maximum of -inf would make its own rows' weights NaN)
     v4f acc[NM][NC];
 #pragma unroll
     for (int i = 0; i < NM; ++i)
@@ -426,13 +440,13 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         for (int t = 0; t < NC; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
     lds_barrier();
 
-    // The operand reads of a product run W reads ahead of it: the order of reads and products below is
-    // kept as it is written (left to itself the compiler reads each operand right before its use and waits
-    // for LDS every time); vector instructions may move across.
+    // The operand reads of a product run W reads ahead of it. The order below is kept as it is written: left
+    // to itself the compiler reads each operand right before its use and waits for LDS every time.
     const int spw = Sh::SpOff + 4 * (kh * Sh::SpH + th_sp(16 * m + 4 * g) + n), spr = Sh::SpOff + 4 * (th_sp(sq) + sr);
-    auto scores = [&](const uint8_t *buf, int c) __attribute__((always_inline)) {
+    // between(i): other work after read i's products
+    auto scores = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
         float *sp = (float *)(smem + spw + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
-        constexpr int N = 18 * NP, W = 6;  // read i: plane i % NP of rows 16 (i / NP % 2) of block i / NP / 2
+        constexpr int N = 18 * NP, W = NP == 2 ? 4 : 6;  // read i: plane i % NP of rows 16 (i / NP % 2) of block i / NP / 2
         auto get = [&](int i) __attribute__((always_inline)) {
             const int j = i / (2 * NP), rb = i / NP % 2;
             return *(const v4i *)(buf + (i % NP) * Sh::PlaneB + (j < 8 ? bofs[j & 3] + 256 * (j >> 2) + 16384 * rb : kofs + 2048 * rb));
@@ -447,7 +461,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
 #pragma unroll
         for (int i = 0; i < W; ++i) bv[i] = get(i);
-        __builtin_amdgcn_sched_barrier(kThFree);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const int j = i / (2 * NP), rb = i / NP % 2;
@@ -460,7 +474,8 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 if (i % NP == 0) d[rb] = th_mfma<FMT>(ql[j], v, d[rb]);  // not lo . lo
             }
             if (i + W < N) bv[i % W] = get(i + W);
-            __builtin_amdgcn_sched_barrier(kThFree);
+            between(i);
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int rb = 0; rb < 2; ++rb) {
@@ -471,8 +486,10 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             for (int i = 0; i < 4; ++i) sp[32 * i + 16 * rb] = d[rb][i];
         }
     };
-    // softmax of a chunk: its reads, then (after other work) its arithmetic and writes
-    v4f sx, st, sr4;
+    // softmax of a chunk: its reads, then its arithmetic and writes in five pieces
+    v4f sx, st, sr4, sp4;
+    float cm, alpha;
+    bool moved;
     auto softmax_read = [&](const uint8_t *buf, int c) __attribute__((always_inline)) {
         const float *scl = (const float *)(buf + NP * Sh::PlaneB);
         const float *sp = (const float *)(smem + spr + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
@@ -483,36 +500,41 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
         sx = s0 + s1;
     };
-    auto softmax = [&](int c) __attribute__((always_inline)) {
-        const int nv = r1 - (r0 + c * kThCh) - sr;  // of this thread's rows, the ones in the split
-        v4f x, t;
+    auto softmax = [&](int c, int piece) __attribute__((always_inline)) {
+        if (piece == 0) {
+            // of this thread's rows, the ones in the split; none before the first chunk
+            const int nv = (c < 0 ? 0 : r1 - (r0 + c * kThCh)) - sr;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) x[e] = e < nv ? sx[e] : -INFINITY;
-        t = x;
-        if constexpr (kQ8) t += st;
-        float cm = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-        cm = fmaxf(cm, dpp_f32<0xB1>(cm));
-        cm = fmaxf(cm, dpp_f32<0x4E>(cm));
-        cm = fmaxf(cm, dpp_f32<0x141>(cm));  // row_half_mirror: the other four of the eight
-        const bool mv = cm > m_run + 2.0f;
-        const bool any = __any(mv);
-        const float alpha = mv ? __builtin_amdgcn_exp2f(m_run - cm) : 1.0f;
-        m_run = mv ? cm : m_run;
-        l_run *= alpha;
-        v4f p;
+            for (int e = 0; e < 4; ++e) sx[e] = e < nv ? sx[e] : -INFINITY;
+            v4f t = sx;
+            if constexpr (kQ8) t += st;
+            cm = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            cm = fmaxf(cm, dpp_f32<0xB1>(cm));
+        } else if (piece == 1) {
+            cm = fmaxf(cm, dpp_f32<0x4E>(cm));
+            cm = fmaxf(cm, dpp_f32<0x141>(cm));  // row_half_mirror: the other four of the eight
+            const bool mv = cm > m_run + 2.0f;
+            moved = __any(mv);
+            alpha = mv ? __builtin_amdgcn_exp2f(m_run - cm) : 1.0f;
+            m_run = mv ? cm : m_run;
+        } else if (piece == 2) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = __builtin_amdgcn_exp2f(x[e] - m_run);
-        l_run += (p[0] + p[1]) + (p[2] + p[3]);  // this thread's rows; the eight threads' sums are added at the end
-        if constexpr (kQ8) p *= sr4;
-        int2 hi, lo;
-        th_split4<kQ8>(p, hi, lo);
-        uint8_t *pw = smem + Sh::PwOff + th_pw(sq, sr >> 3) + 2 * (sr & 4);
-        *(int2 *)pw = hi;
-        *(int2 *)(pw + Sh::PwB) = lo;
-        if ((tid & 7) == 0) *(float *)(smem + Sh::AlOff + 4 * sq) = alpha;
-        if (l == 0) *(int *)(smem + Sh::FlOff + 32 * (c & 1) + 4 * w) = any ? 1 : 0;
+            for (int e = 0; e < 4; ++e) sp4[e] = __builtin_amdgcn_exp2f(sx[e] - m_run);
+        } else if (piece == 3) {
+            // this thread's rows; the eight threads' sums are added at the end
+            l_run = fmaf(l_run, alpha, (sp4[0] + sp4[1]) + (sp4[2] + sp4[3]));
+            if constexpr (kQ8) sp4 *= sr4;
+        } else {
+            int2 hi, lo;
+            th_split4<kQ8>(sp4, hi, lo);
+            uint8_t *pw = smem + Sh::PwOff + th_pw(sq, sr >> 3) + 2 * (sr & 4);
+            *(int2 *)pw = hi;
+            *(int2 *)(pw + Sh::PwB) = lo;
+            if ((tid & 7) == 0) *(float *)(smem + Sh::AlOff + 4 * sq) = alpha;
+            if (l == 0) *(int *)(smem + Sh::FlOff + 32 * (c & 1) + 4 * w) = moved ? 1 : 0;
+        }
     };
-    auto mix = [&](const uint8_t *buf, int c) __attribute__((always_inline)) {
+    auto mix = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
         v4i f[NW / 4], ph[NM], pl[NM], bt[2][NP];
 #pragma unroll
         for (int i = 0; i < NW / 4; ++i) f[i] = *(const v4i *)(smem + Sh::FlOff + 32 * (c & 1) + 16 * i);
@@ -541,7 +563,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 for (int t = 0; t < NC; ++t) acc[i][t] *= al;
             }
         }
-        __builtin_amdgcn_sched_barrier(kThFree);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
 #pragma unroll
@@ -552,27 +574,35 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
             for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(pl[i], bt[t & 1][0], acc[i][t]);
             if (t + 2 < NC) get(t + 2);
-            __builtin_amdgcn_sched_barrier(kThFree);
+            between(t);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
 
     if constexpr (Sh::Pipe) {
-        // Two barriers a chunk. Between them the waves hold a product and vector work that do not depend
-        // on each other: scores of chunk c + 1 beside the softmax of chunk c, then the mix of chunk c
-        // beside the staging of chunk c + 2. (The scores of the chunk past the last are not used.)
-        uint8_t *cur = smem, *next = smem + Sh::Slot, *then = smem + 2 * Sh::Slot;
-        if (nch > 1) stage(next);
-        if (nch > 2) fetch(2);
-        scores(cur, 0);
-        lds_barrier();
-        for (int c = 0; c < nch; ++c) {
+        // Two barriers a chunk. Between them a wave holds a product and vector work that do not depend on each
+        // other, the vector work laid between the products: scores of chunk c + 1 with the softmax of chunk
+        // c, then the mix of chunk c with the staging of chunk c + 2. The pass c = -1 fills the pipe (its
+        // softmax has no rows, its sums are dropped); what the last passes stage and score is not used.
+        static_assert(NL <= NC, "a latent item per column block");
+        uint8_t *cur = smem + 2 * Sh::Slot, *next = smem, *then = smem + Sh::Slot;
+        for (int c = -1; c < nch; ++c) {
             softmax_read(cur, c);
-            scores(next, c + 1);
-            softmax(c);
+            scores(next, c + 1, [&](int i) __attribute__((always_inline)) {
+                if (i >= 4 && i <= 12 && i % 2 == 0) softmax(c, (i - 4) / 2);
+            });
             lds_barrier();
-            mix(cur, c);
-            if (c + 2 < nch) stage(then);
-            if (c + 3 < nch) fetch(c + 3);
+            mix(cur, c, [&](int t) __attribute__((always_inline)) {
+                stage(then, held, t);
+                if (t == NC - 1) stage(then, held, NL);
+            });
+            fetch(c + 3, held);
+            if (c < 0) {
+#pragma unroll
+                for (int i = 0; i < NM; ++i)
+#pragma unroll
+                    for (int t = 0; t < NC; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
+            }
             lds_barrier();
             uint8_t *t = cur;
             cur = next;
@@ -581,16 +611,17 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
     } else {
         for (int c = 0; c < nch; ++c) {
-            scores(smem, c);
+            scores(smem, c, [](int) {});
             lds_barrier();  // both halves of every score are in LDS
             softmax_read(smem, c);
-            softmax(c);
+#pragma unroll
+            for (int i = 0; i < 5; ++i) softmax(c, i);
             lds_barrier();  // the weights are in LDS
-            mix(smem, c);
+            mix(smem, c, [](int) {});
             if (c + 1 < nch) {
                 lds_barrier();  // every wave is done with the chunk
-                stage(smem);
-                if (c + 2 < nch) fetch(c + 2);
+                stage_all(smem, held);
+                fetch(c + 2, held);
                 lds_barrier();
             }
         }
@@ -837,7 +868,7 @@ __global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
 // workgroups (ceil(count / nm) per split) on the CUs takes about k (r / kThCh + kThStart) chunks' time, the
 // start of a workgroup (its queries, its first chunk) being worth kThStart chunks: for each k up to
 // kThRounds the fewest rows that make k rounds, and of these the shortest.
-constexpr int kThMin = 64, kThStart = 4, kThRounds = 4;
+constexpr int kThMin = 64, kThMax = 1 << 19, kThStart = 4, kThRounds = 4;
 int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
     const bool kimi = d.NH == 16 && d.R == 512 && d.DR == 64 && d.DV == 128;
     int most = 0, longest = 0;
@@ -855,9 +886,9 @@ int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
             for (int b = 0; b < t.n; ++b) n += (t.s[b].count + t.nm - 1) / t.nm * splits(t.s[b].ctx, chunks * kThCh);
             return n;
         };
-        // the combine's table of a node's splits; also keeps offsets within a split below 2^31 bytes
-        const long least = std::max<long>(kThMin / kThCh, splits(splits(longest, kMaxSplits), kThCh));
-        long cost = LONG_MAX, hi = std::max(least, splits(longest, kThCh));
+        // at most kThMax rows: offsets within a split stay below 2^31 bytes
+        const long least = kThMin / kThCh;
+        long cost = LONG_MAX, hi = std::max(least, std::min<long>(splits(longest, kThCh), kThMax / kThCh));
         for (int k = 1; k <= kThRounds; ++k) {
             long lo = least, up = hi;
             while (lo < up) {  // groups() does not increase with the chunks
