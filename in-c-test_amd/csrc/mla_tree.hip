@@ -649,6 +649,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
 // ---- the nodes' own rows, the merge and W_UV (Kimi shapes, DV = 128) --------------------------------
 
 constexpr int kTcNodes = 4;  // nodes of a combine workgroup (at most)
+constexpr int kTcAhead = 6;  // splits whose loads a wave has in flight
 struct TreeCombArgs {
     TreeRowsTable t;
     TreeNodes nd;
@@ -694,121 +695,142 @@ __global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
     constexpr size_t stride = NH * (R + 2);
     const float *Pm = P + NH * R + h, *Pa = P + h * R + 4 * l;
 
-    // ---- the history's splits: maximum, denominator, this wave's share of the sum
+    // ---- the path's requests (the node's first wave): the head's query, the first four rows
+    const uint32_t mlo = (uint32_t)tree_lane((int)(uint32_t)lane_path, k), mhi = (uint32_t)tree_lane((int)(uint32_t)(lane_path >> 32), k);
+    const uint64_t mask = ((uint64_t)mhi << 32) | mlo;
+    const int np = __builtin_popcountll(mask);
+    struct Row {  // four + four latents and a key element of a row, as stored
+        v4f f0, f1;
+        uint2 h0, h1;
+        int q0, q1;
+        float sc, key;
+    };
+    auto ask = [&](size_t row, Row &x) __attribute__((always_inline)) {
+        if constexpr (FMT == kFmtQ8) {
+            const int8_t *p = (const int8_t *)s.a + row * R + 4 * l;
+            x.q0 = *(const int *)p;
+            x.q1 = *(const int *)(p + 256);
+            x.sc = ((const float *)s.b)[row];
+        } else if constexpr (FMT == kFmtF32) {
+            const float *p = (const float *)s.a + row * R + 4 * l;
+            x.f0 = *(const v4f *)p;
+            x.f1 = *(const v4f *)(p + 256);
+        } else {
+            const uint16_t *p = (const uint16_t *)s.a + row * R + 4 * l;
+            x.h0 = *(const uint2 *)p;
+            x.h1 = *(const uint2 *)(p + 256);
+        }
+        x.key = tree_key<FMT>(s, row, DR, l);
+    };
+    auto lat = [&](const Row &x, v4f &x0, v4f &x1) __attribute__((always_inline)) {
+        if constexpr (FMT == kFmtQ8) {
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                x0[z] = (float)(int8_t)(x.q0 >> (8 * z)) * x.sc;
+                x1[z] = (float)(int8_t)(x.q1 >> (8 * z)) * x.sc;
+            }
+        } else if constexpr (FMT == kFmtF32) {
+            x0 = x.f0;
+            x1 = x.f1;
+        } else {
+            auto up = [](uint2 h) { return v4f{__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u), __uint_as_float(h.y << 16), __uint_as_float(h.y & 0xffff0000u)}; };
+            x0 = up(x.h0);
+            x1 = up(x.h1);
+        }
+    };
+    // four rows of the path at a time; behind its end its last row again
+    int lastrow = 0;
+    auto four = [&](uint64_t &m, Row *x) __attribute__((always_inline)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (m) lastrow = __builtin_ctzll(m);
+            m &= m - 1;
+            ask((size_t)s.ctx + lastrow, x[r]);
+        }
+    };
+    Row x[4];
+    v4f q0, q1;
+    float qk = 0.f;
+    uint64_t left = mask;
+    if (u == 0) {
+        const float *qr = a.qf + ((size_t)(a.nd.first + k) * NH + h) * (R + DR);
+        q0 = *(const v4f *)(qr + 4 * l);
+        q1 = *(const v4f *)(qr + 256 + 4 * l);
+        qk = qr[R + l];
+        four(left, x);
+    }
+    // ---- the history's splits, 64 at a time (split s0 + l's maximum and sum in lane l), running maximum
     float mh = -INFINITY, den = 0.f;
-    for (int s0 = 0; s0 < ns; s0 += 64) mh = fmaxf(mh, s0 + l < ns ? Pm[(size_t)(s0 + l) * stride] : -INFINITY);
-    mh = wave_max(mh);
     v4f c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
     for (int s0 = 0; s0 < ns; s0 += 64) {
-        float e = 0.f, ls = 0.f;
-        if (s0 + l < ns) {
-            e = __expf(Pm[(size_t)(s0 + l) * stride] - mh);
-            ls = Pm[(size_t)(s0 + l) * stride + NH];
-        }
-        den = fmaf(ls, e, den);
         const int top = min(64, ns - s0);
-        for (int t = u; t < top; t += 4 * wpn) {
-            v4f x0[4], x1[4];
+        const float *pm = Pm + (size_t)(s0 + min(l, top - 1)) * stride;
+        const float ms = pm[0], ls = pm[NH];
+        auto get = [&](int t, v4f *y0, v4f *y1) __attribute__((always_inline)) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < kTcAhead; ++r) {
                 const float *p = Pa + (size_t)(s0 + min(t + r * wpn, top - 1)) * stride;
-                x0[r] = *(const v4f *)p;
-                x1[r] = *(const v4f *)(p + 256);
+                y0[r] = *(const v4f *)p;
+                y1[r] = *(const v4f *)(p + 256);
             }
+        };
+        v4f y0[kTcAhead], y1[kTcAhead];
+        get(u, y0, y1);
+        const float mn = fmaxf(mh, wave_max(ms));
+        const float al = __expf(mh - mn), e = l < top ? __expf(ms - mn) : 0.f;
+        mh = mn;
+        den = fmaf(den, al, ls * e);
+        c0 *= al;
+        c1 *= al;
+        for (int t = u; t < top; t += kTcAhead * wpn) {
+            if (t != u) get(t, y0, y1);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
+            for (int r = 0; r < kTcAhead; ++r) {
                 if (t + r * wpn >= top) break;
                 const float wt = lane_f32(e, t + r * wpn);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                    c0[z] = fmaf(x0[r][z], wt, c0[z]);
-                    c1[z] = fmaf(x1[r][z], wt, c1[z]);
+                    c0[z] = fmaf(y0[r][z], wt, c0[z]);
+                    c1[z] = fmaf(y1[r][z], wt, c1[z]);
                 }
             }
         }
     }
     den = wave_sum(den);
-    // ---- the path (the node's first wave)
+    // ---- the path
     float mp = -INFINITY, lp = 0.f;
     v4f p0 = {0.f, 0.f, 0.f, 0.f}, p1 = p0;
     if (u == 0) {
-        const uint32_t mlo = (uint32_t)tree_lane((int)(uint32_t)lane_path, k), mhi = (uint32_t)tree_lane((int)(uint32_t)(lane_path >> 32), k);
-        const uint64_t mask = ((uint64_t)mhi << 32) | mlo;
-        const float *qr = a.qf + ((size_t)(a.nd.first + k) * NH + h) * (R + DR);
-        const v4f q0 = *(const v4f *)(qr + 4 * l) * a.smscale, q1 = *(const v4f *)(qr + 256 + 4 * l) * a.smscale;
-        const float qk = qr[R + l] * a.smscale;
-        auto lat = [&](size_t row, v4f &x0, v4f &x1) __attribute__((always_inline)) {
-            if constexpr (FMT == kFmtQ8) {
-                const int8_t *p = (const int8_t *)s.a + row * R + 4 * l;
-                const int a0 = *(const int *)p, a1 = *(const int *)(p + 256);
-                const float sc = ((const float *)s.b)[row];
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    x0[z] = (float)(int8_t)(a0 >> (8 * z)) * sc;
-                    x1[z] = (float)(int8_t)(a1 >> (8 * z)) * sc;
-                }
-            } else if constexpr (FMT == kFmtF32) {
-                const float *p = (const float *)s.a + row * R + 4 * l;
-                x0 = *(const v4f *)p;
-                x1 = *(const v4f *)(p + 256);
-            } else {
-                const uint16_t *p = (const uint16_t *)s.a + row * R + 4 * l;
-                const uint2 a0 = *(const uint2 *)p, a1 = *(const uint2 *)(p + 256);
-                x0 = v4f{__uint_as_float(a0.x << 16), __uint_as_float(a0.x & 0xffff0000u), __uint_as_float(a0.y << 16), __uint_as_float(a0.y & 0xffff0000u)};
-                x1 = v4f{__uint_as_float(a1.x << 16), __uint_as_float(a1.x & 0xffff0000u), __uint_as_float(a1.y << 16), __uint_as_float(a1.y & 0xffff0000u)};
-            }
-        };
-        const int np = __builtin_popcountll(mask);
-        // four rows at a time; rows past the path's end repeat its last
-        auto four = [&](uint64_t &m, size_t *row) __attribute__((always_inline)) {
-            int last = 0;
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                if (m) last = __builtin_ctzll(m);
-                m &= m - 1;
-                row[r] = (size_t)s.ctx + last;
-            }
-        };
         float sc = -INFINITY;
-        uint64_t m = mask;
         for (int t = 0; t < np; t += 4) {
-            size_t row[4];
-            four(m, row);
-            float v[4];
-            v4f x0[4], x1[4];
-            float xk[4];
+            if (t > 0) four(left, x);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                lat(row[r], x0[r], x1[r]);
-                xk[r] = tree_key<FMT>(s, row[r], DR, l);
-            }
+                v4f x0, x1;
+                lat(x[r], x0, x1);
+                float v = qk * x[r].key;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                v[r] = qk * xk[r];
-#pragma unroll
-                for (int z = 0; z < 4; ++z) v[r] = fmaf(q1[z], x1[r][z], fmaf(q0[z], x0[r][z], v[r]));
-                v[r] = wave_sum(v[r]);
-                if (l == t + r && t + r < np) sc = v[r];
+                for (int z = 0; z < 4; ++z) v = fmaf(q1[z], x1[z], fmaf(q0[z], x0[z], v));
+                v = wave_sum(v) * a.smscale;
+                if (l == t + r && t + r < np) sc = v;
             }
         }
         mp = wave_max(sc);
         const float e = l < np ? __expf(sc - mp) : 0.f;
         lp = wave_sum(e);
-        m = mask;
+        left = mask;
         for (int t = 0; t < np; t += 4) {
-            size_t row[4];
-            four(m, row);
-            v4f x0[4], x1[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) lat(row[r], x0[r], x1[r]);
+            if (np > 4) four(left, x);  // four rows or fewer are still here
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if (t + r >= np) break;
+                v4f x0, x1;
+                lat(x[r], x0, x1);
                 const float wt = lane_f32(e, t + r);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
-                    p0[z] = fmaf(x0[r][z], wt, p0[z]);
-                    p1[z] = fmaf(x1[r][z], wt, p1[z]);
+                    p0[z] = fmaf(x0[z], wt, p0[z]);
+                    p1[z] = fmaf(x1[z], wt, p1[z]);
                 }
             }
         }
