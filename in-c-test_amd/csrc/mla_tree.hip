@@ -134,10 +134,10 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 // ---- the history (Kimi shapes) ------------------------------------------------------------------
 
 // A workgroup takes NM nodes of one tree (16 NM queries) over one split of the history, in chunks of 32
-// rows that all its waves share in LDS: 2 NM waves,
-//   scores: wave (m, kh) = node m's 16 heads x 32 rows over half kh of the 576 columns, the queries held
+// rows (FP32: 16) that all its waves share in LDS: 2 NM waves,
+//   scores: wave (m, kh) = node m's 16 heads x the rows over half kh of the 576 columns, the queries held
 //     in registers; the two halves are added through LDS;
-//   softmax: 8 threads per query, 4 rows each, running maximum (moved only when a chunk exceeds it by
+//   softmax: 8 threads per query, 4 rows (FP32: 2) each, running maximum (moved only when a chunk exceeds it by
 //     more than ln 4) and sum in registers; weights to LDS as the next product's operand;
 //   mix: every wave 512 / (2 NM) latent columns of all 16 NM queries, the rows read transposed.
 // Operands are 16 bits wide, sums 32: the 32-bit query and weight enter as hi + lo (two products), the
@@ -147,15 +147,16 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 // bits. A Q8 row's scale multiplies its latent score and its weight; to keep the weights within fp16
 // whatever the scales, the running maximum is that of score + ln(scale), so that weight times scale stays
 // <= 4.
-constexpr int kThCh = 32;       // rows of a chunk
+constexpr int kThCh = 32;  // rows of a chunk (FP32: of two)
 template <int FMT, int NM>
 struct ThShape {
     static constexpr int NW = 2 * NM, NT = 64 * NW, NQ = 16 * NM;
     static constexpr int NP = FMT == kFmtF32 ? 2 : 1;  // planes of a row
-    static constexpr int LatB = kThCh * 1024, KeyB = kThCh * 128, PlaneB = LatB + KeyB;
-    static constexpr int ScB = FMT == kFmtQ8 ? 2 * kThCh * 4 : 0;  // scales, their logarithms
+    static constexpr int Ch = kThCh / NP;              // rows of a chunk
+    static constexpr int LatB = Ch * 1024, KeyB = Ch * 128, PlaneB = LatB + KeyB;
+    static constexpr int ScB = FMT == kFmtQ8 ? 2 * Ch * 4 : 0;  // scales, their logarithms
     static constexpr int Slot = NP * PlaneB + ScB;
-    static constexpr int Ring = FMT == kFmtF32 || NM < 4 ? 1 : 3;
+    static constexpr int Ring = NM < 4 ? 1 : 3;
     static constexpr bool Pipe = Ring == 3;
     static constexpr int SpOff = Ring * Slot;
     static constexpr int SpH = NQ * 36;  // floats of a half of the scores (th_sp)
@@ -282,7 +283,7 @@ __device__ __forceinline__ void th_split4(const v4f &x, int2 &hi, int2 &lo) {
 template <int FMT, int NM>
 __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_tree_hist(TreeArgs a) {
     using Sh = ThShape<FMT, NM>;
-    constexpr int NT = Sh::NT, NW = Sh::NW, NP = Sh::NP;
+    constexpr int NT = Sh::NT, NW = Sh::NW, NP = Sh::NP, Ch = Sh::Ch, RB = Ch / 16;
     constexpr int NC = 512 / NW / 16;  // 16-column blocks of a wave in the mix
     constexpr bool kQ8 = FMT == kFmtQ8;
     __shared__ __attribute__((aligned(16))) uint8_t smem[Sh::Smem];
@@ -292,29 +293,30 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     if (!tree_unit(a.t, s)) return;
     const int split = s.split, tile = s.tile;
     const int r0 = split * s.rps, r1 = split == s.ns - 1 ? s.ctx : r0 + s.rps;
-    const int nch = (r1 - r0 + kThCh - 1) / kThCh;
+    const int nch = (r1 - r0 + Ch - 1) / Ch;
     const int first = tile * NM, live = min(NM, s.count - first);  // nodes of this tile
 
     // ---- staging: a chunk's rows from memory to registers, and from there to an LDS slot. A thread
-    // takes eight values of a latent row (word tid % 64 of rows tid / 64 + NW i) and four of a key row (half a
-    // word: tid % 16 of rows tid / 16 + NT / 16 i).
-    constexpr int NL = kThCh / NW, NK = 512 / NT;
+    // takes eight values of a latent row (word tid % 64 of rows tid / 64 + NW i) and eight bytes of a key row
+    // (tid % 16 of rows tid / 16 + NT / 16 i; FP32: tid % 32 of rows tid / 32).
+    constexpr int NL = Ch / NW, NK = 512 / NT;
     constexpr int LE = kQ8 ? 1 : FMT == kFmtF32 ? 4 : 2, KE = FMT == kFmtF32 ? 4 : 2;  // bytes of an element
     constexpr int LV = LE == 4 ? 2 : 1;
     struct Held {
-        v4i la[kQ8 ? 1 : NL * LV], kf[KE == 4 ? NK : 1];
-        v2i lc[kQ8 ? NL : 1], kb[KE == 4 ? 1 : NK];
+        v4i la[kQ8 ? 1 : NL * LV];
+        v2i lc[kQ8 ? NL : 1], kb[NK];
         float rsc;
     };
-    const int lrow = tid >> 6, krow = tid >> 4;
+    static_assert(KE == 2 || NK == 1, "FP32 rows: eight waves");
+    const int lrow = tid >> 6;
     // the split's rows as buffers: a read past the last row gives zeros (its score is masked)
     const int nrow = r1 - r0;
     const auto ba = __builtin_amdgcn_make_buffer_rsrc(s.a + (size_t)r0 * (512 * LE), 0, nrow * (512 * LE), 0x00027000);
     const auto bk = __builtin_amdgcn_make_buffer_rsrc((kQ8 ? s.c : s.b) + (size_t)r0 * (64 * KE), 0, nrow * (64 * KE), 0x00027000);
     const auto bs = __builtin_amdgcn_make_buffer_rsrc(s.b + (size_t)r0 * 4, 0, kQ8 ? nrow * 4 : 0, 0x00027000);
-    const int va = tid * (8 * LE), vk = tid * (4 * KE);  // rows lie one after another, so do the threads' words
+    const int va = tid * (8 * LE), vk = tid * 8;  // rows lie one after another, so do the threads' words
     auto fetch = [&](int c, Held &f) __attribute__((always_inline)) {
-        const int oa = va + c * (kThCh * 512 * LE), ok = vk + c * (kThCh * 64 * KE);
+        const int oa = va + c * (Ch * 512 * LE), ok = vk + c * (Ch * 64 * KE);
 #pragma unroll
         for (int i = 0; i < NL; ++i) {
             if constexpr (kQ8)
@@ -325,12 +327,9 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                     f.la[LV * i + v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ba, oa + i * (NT * 8 * LE) + 16 * v, 0, 0));
         }
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            if constexpr (KE == 4) f.kf[i] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(bk, ok + i * (NT * 4 * KE), 0, 0));
-            else f.kb[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(bk, ok + i * (NT * 4 * KE), 0, 0));
-        }
+        for (int i = 0; i < NK; ++i) f.kb[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(bk, ok + i * (NT * 8), 0, 0));
         if constexpr (kQ8)
-            f.rsc = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(bs, 4 * (c * kThCh + (tid & 31)), 0, 0));
+            f.rsc = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(bs, 4 * (c * Ch + (tid & 31)), 0, 0));
     };
     auto put = [&](uint8_t *at, const v4i *v) __attribute__((always_inline)) {
         if constexpr (NP == 2) {
@@ -342,7 +341,8 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             *(v4i *)at = v[0];
         }
     };
-    const int sa = lrow * 1024 + 16 * (l ^ th_swz(lrow)), sk = Sh::LatB + th_key(krow, (tid & 15) >> 1) + 8 * (tid & 1);
+    const int sa = lrow * 1024 + 16 * (l ^ th_swz(lrow));
+    const int sk = Sh::LatB + (KE == 4 ? th_key(tid >> 5, (tid >> 2) & 7) + 4 * (tid & 3) : th_key(tid >> 4, (tid >> 1) & 7) + 8 * (tid & 1));
     // piece i < NL: a latent item; the last piece: the key items and the scales
     auto stage = [&](uint8_t *buf, const Held &f, int i) __attribute__((always_inline)) {
         if (i < NL) {
@@ -355,19 +355,20 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int q = 0; q < NK; ++q) {
             if constexpr (KE == 4) {
-                int2 hi, lo;
-                th_split4<false>(__builtin_bit_cast(v4f, f.kf[q]), hi, lo);
-                *(int2 *)(buf + sk + q * (NT / 16) * 128) = hi;
-                *(int2 *)(buf + Sh::PlaneB + sk + q * (NT / 16) * 128) = lo;
+                const v2f x = __builtin_bit_cast(v2f, f.kb[q]);
+                const v2bf hi = __builtin_convertvector(x, v2bf);
+                const v2bf lo = __builtin_convertvector((v2f{x.x - (float)hi.x, x.y - (float)hi.y}), v2bf);
+                *(int *)(buf + sk) = __builtin_bit_cast(int, hi);
+                *(int *)(buf + Sh::PlaneB + sk) = __builtin_bit_cast(int, lo);
             } else {
                 *(v2i *)(buf + sk + q * (NT / 16) * 128) = f.kb[q];
             }
         }
         if constexpr (kQ8) {
-            if (tid < kThCh) {
+            if (tid < Ch) {
                 float *sc = (float *)(buf + NP * Sh::PlaneB);
                 sc[tid] = f.rsc;
-                sc[kThCh + tid] = __builtin_amdgcn_logf(fmaxf(fabsf(f.rsc), 1e-35f));
+                sc[Ch + tid] = __builtin_amdgcn_logf(fmaxf(fabsf(f.rsc), 1e-35f));
             }
         }
     };
@@ -422,16 +423,18 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
     for (int j = 0; j < 4; ++j) bofs[j] = n * 1024 + 16 * ((4 * (8 * kh + j) + g) ^ th_swz(n));
     const int kofs = Sh::LatB + th_key(n, 4 * kh + g);
-    // transposed reads of column block NC w + t: rows 8 g + 4 h + (n >> 2), see lds_read_tr16
+    // transposed reads of column block NC w + t (lds_read_tr16): rows 8 g + 4 h + (n >> 2); of the FP32 planes
+    // the 16 hi rows for g = 0, 1 and the 16 lo rows for g = 2, 3
     int tro[2][NC];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const int row = 8 * g + 4 * h + (n >> 2);
+        const int row = 8 * (NP == 2 ? g & 1 : g) + 4 * h + (n >> 2);
 #pragma unroll
         for (int t = 0; t < NC; ++t)
-            tro[h][t] = row * 1024 + 16 * ((2 * (NC * w + t) + ((n >> 1) & 1)) ^ th_swz(row)) + 8 * (n & 1);
+            tro[h][t] = (NP == 2 ? (g >> 1) * Sh::PlaneB : 0) + row * 1024 + 16 * ((2 * (NC * w + t) + ((n >> 1) & 1)) ^ th_swz(row)) + 8 * (n & 1);
     }
-    const int sq = tid >> 3, sr = 4 * (tid & 7);  // softmax: this thread's query and rows
+    constexpr int SR = Ch / 8;                      // softmax: rows of a thread,
+    const int sq = tid >> 3, sr = SR * (tid & 7);  // its query and first row
     float m_run = -1e30f, l_run = 0.f;  // (a maximum of -inf would make its own rows' weights NaN)
     v4f acc[NM][NC];
 #pragma unroll
@@ -446,39 +449,49 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     // between(i): other work after read i's products
     auto scores = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
         float *sp = (float *)(smem + spw + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
-        constexpr int N = 18 * NP, W = NP == 2 ? 4 : 6;  // read i: plane i % NP of rows 16 (i / NP % 2) of block i / NP / 2
+        // read i: plane i % NP of rows 16 (i / NP % RB) of block i / NP / RB
+        constexpr int N = 9 * NP * RB, W = 6;
         auto get = [&](int i) __attribute__((always_inline)) {
-            const int j = i / (2 * NP), rb = i / NP % 2;
+            const int j = i / (NP * RB), rb = i / NP % RB;
             return *(const v4i *)(buf + (i % NP) * Sh::PlaneB + (j < 8 ? bofs[j & 3] + 256 * (j >> 2) + 16384 * rb : kofs + 2048 * rb));
         };
+        // sums: d over the latents by rows (FP32: by hi . hi and lo . hi), dk over the key (FP32: hi . lo)
         v4f d[2], dk[2];
         v4i bv[W];
-        float x[2] = {1.f, 1.f};
+        float x[RB];
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-            d[rb] = dk[rb] = v4f{0.f, 0.f, 0.f, 0.f};
-            if constexpr (kQ8) x[rb] = *(const float *)(buf + NP * Sh::PlaneB + 4 * (16 * rb + n));
-        }
+        for (int z = 0; z < 2; ++z) d[z] = dk[z] = v4f{0.f, 0.f, 0.f, 0.f};
+        if constexpr (kQ8)
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) x[rb] = *(const float *)(buf + NP * Sh::PlaneB + 4 * (16 * rb + n));
 #pragma unroll
         for (int i = 0; i < W; ++i) bv[i] = get(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int j = i / (2 * NP), rb = i / NP % 2;
+            const int j = i / (NP * RB), rb = i / NP % RB;
             const v4i v = bv[i % W];
-            if (kQ8 && j == 8) {
+            if constexpr (NP == 2) {  // not lo . lo
+                if (i % 2 == 0) {
+                    d[0] = th_mfma<FMT>(qh[j], v, d[0]);
+                    d[1] = th_mfma<FMT>(ql[j], v, d[1]);
+                } else {
+                    dk[0] = th_mfma<FMT>(qh[j], v, dk[0]);
+                }
+            } else if (kQ8 && j == 8) {
                 dk[rb] = th_mfma<kFmtBF16>(qh[j], v, dk[rb]);
                 dk[rb] = th_mfma<kFmtBF16>(ql[j], v, dk[rb]);
             } else {
                 d[rb] = th_mfma<FMT>(qh[j], v, d[rb]);
-                if (i % NP == 0) d[rb] = th_mfma<FMT>(ql[j], v, d[rb]);  // not lo . lo
+                d[rb] = th_mfma<FMT>(ql[j], v, d[rb]);
             }
             if (i + W < N) bv[i % W] = get(i + W);
             between(i);
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (NP == 2) d[0] += d[1] + dk[0];
 #pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
+        for (int rb = 0; rb < RB; ++rb) {
             if constexpr (kQ8)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) d[rb][i] = fmaf(d[rb][i], qd[i] * x[rb], dk[rb][i]);
@@ -487,28 +500,30 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         }
     };
     // softmax of a chunk: its reads, then its arithmetic and writes in five pieces
-    v4f sx, st, sr4, sp4;
+    typedef float vsr __attribute__((ext_vector_type(SR)));
+    vsr sx, st, sr4, sp4;
     float cm, alpha;
     bool moved;
     auto softmax_read = [&](const uint8_t *buf, int c) __attribute__((always_inline)) {
         const float *scl = (const float *)(buf + NP * Sh::PlaneB);
         const float *sp = (const float *)(smem + spr + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
-        const v4f s0 = *(const v4f *)sp, s1 = *(const v4f *)(sp + Sh::SpH);
+        const vsr s0 = *(const vsr *)sp, s1 = *(const vsr *)(sp + Sh::SpH);
         if constexpr (kQ8) {
-            sr4 = *(const v4f *)(scl + sr);
-            st = *(const v4f *)(scl + kThCh + sr);
+            sr4 = *(const vsr *)(scl + sr);
+            st = *(const vsr *)(scl + Ch + sr);
         }
         sx = s0 + s1;
     };
     auto softmax = [&](int c, int piece) __attribute__((always_inline)) {
         if (piece == 0) {
             // of this thread's rows, the ones in the split; none before the first chunk
-            const int nv = (c < 0 ? 0 : r1 - (r0 + c * kThCh)) - sr;
+            const int nv = (c < 0 ? 0 : r1 - (r0 + c * Ch)) - sr;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sx[e] = e < nv ? sx[e] : -INFINITY;
-            v4f t = sx;
+            for (int e = 0; e < SR; ++e) sx[e] = e < nv ? sx[e] : -INFINITY;
+            vsr t = sx;
             if constexpr (kQ8) t += st;
-            cm = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+            cm = fmaxf(t[0], t[1]);
+            if constexpr (SR == 4) cm = fmaxf(cm, fmaxf(t[2], t[3]));
             cm = fmaxf(cm, dpp_f32<0xB1>(cm));
         } else if (piece == 1) {
             cm = fmaxf(cm, dpp_f32<0x4E>(cm));
@@ -519,37 +534,44 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             m_run = mv ? cm : m_run;
         } else if (piece == 2) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sp4[e] = __builtin_amdgcn_exp2f(sx[e] - m_run);
+            for (int e = 0; e < SR; ++e) sp4[e] = __builtin_amdgcn_exp2f(sx[e] - m_run);
         } else if (piece == 3) {
             // this thread's rows; the eight threads' sums are added at the end
-            l_run = fmaf(l_run, alpha, (sp4[0] + sp4[1]) + (sp4[2] + sp4[3]));
+            float sum = sp4[0] + sp4[1];
+            if constexpr (SR == 4) sum += sp4[2] + sp4[3];
+            l_run = fmaf(l_run, alpha, sum);
             if constexpr (kQ8) sp4 *= sr4;
         } else {
-            int2 hi, lo;
-            th_split4<kQ8>(sp4, hi, lo);
-            uint8_t *pw = smem + Sh::PwOff + th_pw(sq, sr >> 3) + 2 * (sr & 4);
-            *(int2 *)pw = hi;
-            *(int2 *)(pw + Sh::PwB) = lo;
+            if constexpr (SR == 4) {
+                int2 hi, lo;
+                th_split4<kQ8>(sp4, hi, lo);
+                uint8_t *pw = smem + Sh::PwOff + th_pw(sq, sr >> 3) + 2 * (sr & 4);
+                *(int2 *)pw = hi;
+                *(int2 *)(pw + Sh::PwB) = lo;
+            } else {  // the hi weights in words 0, 1, the lo weights in words 2, 3
+                const v2bf hi = __builtin_convertvector((v2f{sp4[0], sp4[1]}), v2bf);
+                const v2bf lo = __builtin_convertvector((v2f{sp4[0] - (float)hi.x, sp4[1] - (float)hi.y}), v2bf);
+                *(int *)(smem + Sh::PwOff + th_pw(sq, sr >> 3) + 2 * (sr & 7)) = __builtin_bit_cast(int, hi);
+                *(int *)(smem + Sh::PwOff + th_pw(sq, 2 + (sr >> 3)) + 2 * (sr & 7)) = __builtin_bit_cast(int, lo);
+            }
             if ((tid & 7) == 0) *(float *)(smem + Sh::AlOff + 4 * sq) = alpha;
             if (l == 0) *(int *)(smem + Sh::FlOff + 32 * (c & 1) + 4 * w) = moved ? 1 : 0;
         }
     };
     auto mix = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
-        v4i f[NW / 4], ph[NM], pl[NM], bt[2][NP];
+        // FP32: an operand holds 16 rows twice, for the hi and for the lo plane: ph . (hi | lo) + pl . (hi | lo)
+        v4i f[NW / 4], ph[NM], pl[NM], bt[2];
 #pragma unroll
         for (int i = 0; i < NW / 4; ++i) f[i] = *(const v4i *)(smem + Sh::FlOff + 32 * (c & 1) + 16 * i);
         auto get = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-            for (int z = 0; z < NP; ++z)
-                bt[t & 1][z] = __builtin_bit_cast(v4i, __builtin_shufflevector(lds_read_tr16(buf + z * Sh::PlaneB + tro[0][t]),
-                                                                               lds_read_tr16(buf + z * Sh::PlaneB + tro[1][t]), 0,
-                                                                               1, 2, 3, 4, 5, 6, 7));
+            bt[t & 1] = __builtin_bit_cast(
+                v4i, __builtin_shufflevector(lds_read_tr16(buf + tro[0][t]), lds_read_tr16(buf + tro[1][t]), 0, 1, 2, 3, 4, 5, 6, 7));
         };
 #pragma unroll
         for (int i = 0; i < NM; ++i) {
-            ph[i] = *(const v4i *)(smem + Sh::PwOff + th_pw(16 * i + n, g));
+            ph[i] = *(const v4i *)(smem + Sh::PwOff + th_pw(16 * i + n, NP == 2 ? g & 1 : g));
             if (i == 0) get(0);
-            pl[i] = *(const v4i *)(smem + Sh::PwOff + Sh::PwB + th_pw(16 * i + n, g));
+            pl[i] = *(const v4i *)(smem + Sh::PwOff + (NP == 2 ? th_pw(16 * i + n, 2 + (g & 1)) : Sh::PwB + th_pw(16 * i + n, g)));
         }
         get(1);
         int any = 0;
@@ -567,12 +589,9 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
         for (int t = 0; t < NC; ++t) {
 #pragma unroll
-            for (int i = 0; i < NM; ++i) {
-                acc[i][t] = th_mfma<FMT>(ph[i], bt[t & 1][0], acc[i][t]);
-                if constexpr (NP == 2) acc[i][t] = th_mfma<FMT>(ph[i], bt[t & 1][1], acc[i][t]);
-            }
+            for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(ph[i], bt[t & 1], acc[i][t]);
 #pragma unroll
-            for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(pl[i], bt[t & 1][0], acc[i][t]);
+            for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(pl[i], bt[t & 1], acc[i][t]);
             if (t + 2 < NC) get(t + 2);
             between(t);
             __builtin_amdgcn_sched_barrier(0);
@@ -593,7 +612,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             });
             lds_barrier();
             mix(cur, c, [&](int t) __attribute__((always_inline)) {
-                stage(then, held, t);
+                if (t < NL) stage(then, held, t);
                 if (t == NC - 1) stage(then, held, NL);
             });
             fetch(c + 3, held);
