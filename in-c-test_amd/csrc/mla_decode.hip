@@ -14,6 +14,7 @@
 #include "mla_device.h"
 #include "mla_internal.h"
 
+#include <string.h>
 #include <math.h>
 
 #include <algorithm>
@@ -351,10 +352,13 @@ hipError_t launch_gemv_ksplit(hipStream_t st, float *Y, size_t pstride, int ldy,
 struct KvaTokArgs {
     float *Y;                  // partial kq at Y + kq * pstride, [S, ldy]
     const uint16_t *XH, *XL;   // [S, in] bf16 hi / lo planes
-    const uint16_t *W;         // [out, in]
+    const uint16_t *W, *W1;    // rows [0, out0) of W, then [0, out - out0) of W1, of length in
     size_t pstride;
-    int ldy, S, out, in;
+    int ldy, S, out0, out, in;
 };
+__device__ __forceinline__ const uint16_t *kva_row(const KvaTokArgs &a, int row) {
+    return row < a.out0 ? a.W + (size_t)row * a.in : a.W1 + (size_t)(row - a.out0) * a.in;
+}
 
 template <int KPW>
 __global__ __launch_bounds__(256) void k_kva_tok(KvaTokArgs a) {
@@ -362,7 +366,7 @@ __global__ __launch_bounds__(256) void k_kva_tok(KvaTokArgs a) {
     const int kq = blockIdx.y, row0 = blockIdx.x * 64, tok0 = blockIdx.z * 128 + 32 * w;
     const uint16_t *wr[4], *xh[2], *xl[2];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) wr[t] = a.W + (size_t)min(row0 + 16 * t + n, a.out - 1) * a.in;
+    for (int t = 0; t < 4; ++t) wr[t] = kva_row(a, min(row0 + 16 * t + n, a.out - 1));
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const size_t tok = (size_t)min(tok0 + 16 * u + n, a.S - 1);
@@ -481,7 +485,7 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
             rp = (p < BT * 4 ? a.XH : a.XL) + (size_t)min(tok0 + xrow, a.S - 1) * a.in;
             s = (p & 3) ^ swz(xrow);
         } else {
-            rp = a.W + (size_t)min(row0 + wrow, a.out - 1) * a.in;
+            rp = kva_row(a, min(row0 + wrow, a.out - 1));
             s = (p & 3) ^ swz(wrow);
         }
         src[i] = (const uint8_t *)(rp + kq * 512 + 8 * s);
@@ -567,12 +571,14 @@ static hipError_t kva_gemm_launch(hipStream_t st, const KvaTokArgs &a) {
 }
 
 hipError_t launch_kva_tok(hipStream_t st, float *Y, size_t pstride, int ldy, const uint16_t *XH,
-                          const uint16_t *XL, int S, const uint16_t *W, int out, int in) {
-    if (!gemv_ksplit_ok(in, in) || S < 1 || out <= 0 || ldy < out || (S + 127) / 128 > 65535 ||
+                          const uint16_t *XL, int S, const uint16_t *W, int out0, int in, const uint16_t *W1,
+                          int out1) {
+    const int out = out0 + out1;
+    if (!gemv_ksplit_ok(in, in) || S < 1 || out0 <= 0 || out1 < 0 || ldy < out || (out1 > 0 && ((uintptr_t)W1 % 16 != 0 || !W1)) || (S + 127) / 128 > 65535 ||
         ((uintptr_t)XH % 16) != 0 || ((uintptr_t)XL % 16) != 0 || ((uintptr_t)W % 16) != 0 ||
         ((uintptr_t)Y % 16) != 0 || pstride % 4 != 0)
         return hipErrorInvalidValue;
-    KvaTokArgs a{Y, XH, XL, W, pstride, ldy, S, out, in};
+    KvaTokArgs a{Y, XH, XL, W, W1, pstride, ldy, S, out0, out, in};
     if (in == 2048) {
         // Small tiles while they do not outnumber the places for them, so that a short prompt spreads
         // over the CUs: first with a ring that holds all 16 k steps (one block per CU; a block then waits
@@ -855,91 +861,97 @@ __global__ __launch_bounds__(256) void k_append(SeqTable t, Dims d, AppendArgs a
 // k_append waited through four dependent phases per row. Fills of a state on the device, where nobody
 // reads the copy: 16000 BF16 rows 57 -> 41 us (165 MB, most of it the four partials), 1181 Q8 rows
 // 7.2 -> 5.2.
+// One row by one wave: input row ky (np partials), RoPE at position pos, stored at history row hrow of the
+// arrays sa, sb, sc and (row_out not null) staged. nw: the norm weights of columns l + 64 q.
+template <int FMT>
+__device__ __forceinline__ void append_row_wave(void *sa, void *sb, void *sc, size_t hrow, int pos, const float *ky,
+                                                const AppendArgs &a, const float *nw, uint8_t *row_out) {
+    constexpr int R = 512, DR = 64;
+    const int l = threadIdx.x & 63;
+    float kv[9];
+#pragma unroll
+    for (int q = 0; q < 9; ++q) kv[q] = sum_parts(ky + l + 64 * q, kGemvKs, a.pstride);
+    const float2 cs = a.cs[(size_t)pos * 32 + (l & 31)];
+    double sw[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const double v0 = (double)kv[i], v1 = (double)kv[i + 4];
+        double ss = v0 * v0;
+        ss += v1 * v1;
+        sw[i] = wave_sum_f64(ss);
+    }
+    const float mean_sq = (float)(((sw[0] + sw[1]) + (sw[2] + sw[3])) / (double)R);
+    const float inv = 1.0f / sqrtf(mean_sq + a.eps);
+    float lat[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const float t = kv[q] * inv;
+        lat[q] = t * nw[q];
+    }
+    // rotated key: lane i < 32 takes pair i
+    const float ev = __shfl(kv[8], 2 * (l & 31)), od = __shfl(kv[8], 2 * (l & 31) + 1);
+    const float ec = ev * cs.x, os = od * cs.y, oc = od * cs.x, es = ev * cs.y;
+    const float key = l < 32 ? ec - os : oc + es;  // element l
+    if constexpr (FMT == kFmtQ8) {
+        float m = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) m = fmaxf(m, fabsf(lat[q]));  // drops NaN, as k_append's
+        const float amax = wave_max(m);
+        int8_t *codes = (int8_t *)sa + hrow * R;
+        const bool zero = !(amax > 0.0f) || !isfinite(amax);
+        const float scale = zero ? 1.0f : amax / 127.0f;
+        const float qi = zero ? 0.0f : 1.0f / scale;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            int8_t c = 0;
+            if (!zero) {
+                float v = roundf(lat[q] * qi);
+                v = v > 127.0f ? 127.0f : v;
+                v = v < -127.0f ? -127.0f : v;
+                c = (int8_t)v;
+            }
+            codes[l + 64 * q] = c;
+            if (row_out) row_out[l + 64 * q] = (uint8_t)c;
+        }
+        const uint16_t h = f32_to_bf16_rne(key);
+        ((uint16_t *)sc)[hrow * DR + l] = h;
+        if (row_out) ((uint16_t *)(row_out + R + 4))[l] = h;
+        if (l == 0) {
+            ((float *)sb)[hrow] = scale;
+            if (row_out) *(float *)(row_out + R) = scale;
+        }
+    } else if constexpr (FMT == kFmtF32) {
+        float *dst = (float *)sa + hrow * R;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            dst[l + 64 * q] = lat[q];
+            if (row_out) ((float *)row_out)[l + 64 * q] = lat[q];
+        }
+        ((float *)sb)[hrow * DR + l] = key;
+        if (row_out) ((float *)row_out)[R + l] = key;
+    } else {
+        uint16_t *dst = (uint16_t *)sa + hrow * R;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            const uint16_t h = f32_to_bf16_rne(lat[q]);
+            dst[l + 64 * q] = h;
+            if (row_out) ((uint16_t *)row_out)[l + 64 * q] = h;
+        }
+        const uint16_t h = f32_to_bf16_rne(key);
+        ((uint16_t *)sb)[hrow * DR + l] = h;
+        if (row_out) ((uint16_t *)row_out)[R + l] = h;
+    }
+}
+
 template <int FMT>
 __global__ __launch_bounds__(256) void k_append_rows(SeqDesc s, AppendArgs a, int nrows, int stage) {
-    constexpr int R = 512, DR = 64;
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
     float nw[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) nw[q] = bf16_to_f32(a.norm[l + 64 * q]);
-    for (int b = blockIdx.x * 4 + w; b < nrows; b += gridDim.x * 4) {
-        const int pos = s.pos + b;
-        const float *ky = a.y + (size_t)b * a.ldy + a.koff + l;
-        float kv[9];
-#pragma unroll
-        for (int q = 0; q < 9; ++q) kv[q] = sum_parts(ky + 64 * q, kGemvKs, a.pstride);
-        const float2 cs = a.cs[(size_t)pos * 32 + (l & 31)];
-        double sw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double v0 = (double)kv[i], v1 = (double)kv[i + 4];
-            double ss = v0 * v0;
-            ss += v1 * v1;
-            sw[i] = wave_sum_f64(ss);
-        }
-        const float mean_sq = (float)(((sw[0] + sw[1]) + (sw[2] + sw[3])) / (double)R);
-        const float inv = 1.0f / sqrtf(mean_sq + a.eps);
-        float lat[8];
-#pragma unroll
-        for (int q = 0; q < 8; ++q) {
-            const float t = kv[q] * inv;
-            lat[q] = t * nw[q];
-        }
-        // rotated key: lane i < 32 takes pair i
-        const float ev = __shfl(kv[8], 2 * (l & 31)), od = __shfl(kv[8], 2 * (l & 31) + 1);
-        const float ec = ev * cs.x, os = od * cs.y, oc = od * cs.x, es = ev * cs.y;
-        const float key = l < 32 ? ec - os : oc + es;  // element l
-        uint8_t *row_out = a.rows + (size_t)b * a.row_bytes;
-        if constexpr (FMT == kFmtQ8) {
-            float m = 0.f;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) m = fmaxf(m, fabsf(lat[q]));  // drops NaN, as k_append's
-            const float amax = wave_max(m);
-            int8_t *codes = (int8_t *)s.a + (size_t)pos * R;
-            const bool zero = !(amax > 0.0f) || !isfinite(amax);
-            const float scale = zero ? 1.0f : amax / 127.0f;
-            const float qi = zero ? 0.0f : 1.0f / scale;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                int8_t c = 0;
-                if (!zero) {
-                    float v = roundf(lat[q] * qi);
-                    v = v > 127.0f ? 127.0f : v;
-                    v = v < -127.0f ? -127.0f : v;
-                    c = (int8_t)v;
-                }
-                codes[l + 64 * q] = c;
-                if (stage) row_out[l + 64 * q] = (uint8_t)c;
-            }
-            const uint16_t h = f32_to_bf16_rne(key);
-            ((uint16_t *)s.c)[(size_t)pos * DR + l] = h;
-            if (stage) ((uint16_t *)(row_out + R + 4))[l] = h;
-            if (l == 0) {
-                ((float *)s.b)[pos] = scale;
-                if (stage) *(float *)(row_out + R) = scale;
-            }
-        } else if constexpr (FMT == kFmtF32) {
-            float *dst = (float *)s.a + (size_t)pos * R;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                dst[l + 64 * q] = lat[q];
-                if (stage) ((float *)row_out)[l + 64 * q] = lat[q];
-            }
-            ((float *)s.b)[(size_t)pos * DR + l] = key;
-            if (stage) ((float *)row_out)[R + l] = key;
-        } else {
-            uint16_t *dst = (uint16_t *)s.a + (size_t)pos * R;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) {
-                const uint16_t h = f32_to_bf16_rne(lat[q]);
-                dst[l + 64 * q] = h;
-                if (stage) ((uint16_t *)row_out)[l + 64 * q] = h;
-            }
-            const uint16_t h = f32_to_bf16_rne(key);
-            ((uint16_t *)s.b)[(size_t)pos * DR + l] = h;
-            if (stage) ((uint16_t *)row_out)[R + l] = h;
-        }
-    }
+    for (int b = blockIdx.x * 4 + w; b < nrows; b += gridDim.x * 4)
+        append_row_wave<FMT>(s.a, s.b, s.c, (size_t)(s.pos + b), s.pos + b, a.y + (size_t)b * a.ldy + a.koff, a, nw,
+                             stage ? a.rows + (size_t)b * a.row_bytes : nullptr);
 }
 
 static AppendArgs append_args(int fmt, const Dims &d, const float *y, int ldy, int koff,
@@ -1308,12 +1320,13 @@ __device__ __forceinline__ void qprep_body(const SeqTable &t, const Dims &d, con
 // same product chain as in qprep_body (hi column + lo column, k-steps in order), so the rows
 // are bit-identical to it. Wave w owns latent columns 128 qq + 32 w .. + 31 (W_UK^T fragments
 // (h, qq, 2w + t, ks)). The quarter-0 blocks also rotate q_rope (one pair per thread).
-__device__ __forceinline__ void qprep_quarter(const SeqTable &t, const QprepArgs &a, int blk, int NH) {
+// n sequences; pos(b): the position of sequence b, called by whole waves (b may differ between the lanes).
+template <class Pos>
+__device__ __forceinline__ void qprep_quarter(int n_, const Pos &pos, const QprepArgs &a, int blk, int NH) {
     __shared__ __attribute__((aligned(16))) float qn8[8][132];  // q_nope of the 8 sequences
-    const DescLane dl = desc_lane(t);
     const int g8 = blk / (NH * 4), h = (blk / 4) % NH, qq = blk & 3;
     const int tid = threadIdx.x, w = tid >> 6, l = tid & 63, n = l & 15, g = l >> 4;
-    const int nseq = min(8, t.n - 8 * g8);
+    const int nseq = min(8, n_ - 8 * g8);
     v8bf wa[2][4];
     {
         const uint16_t *ut = a.ukt + ((size_t)((h * 4 + qq) * 8 + 2 * w) * 4 * 64 + l) * 8;
@@ -1344,7 +1357,7 @@ __device__ __forceinline__ void qprep_quarter(const SeqTable &t, const QprepArgs
         const int i = tid & 31;
         ev = sum_parts(qh + 128 + 2 * i, a.np, a.pstride);
         od = sum_parts(qh + 128 + 2 * i + 1, a.np, a.pstride);
-        cs = a.cs[(size_t)__shfl(dl.pos, b) * 32 + i];  // b differs between the wave's halves
+        cs = a.cs[(size_t)pos(b) * 32 + i];  // b differs between the wave's halves
     }
     __syncthreads();
     // B operand: column n = hi (n < 8) or lo (n >= 8) of sequence n & 7, k = 32 ks + 8 g .. + 7
@@ -1394,7 +1407,10 @@ __global__ __launch_bounds__(256) void k_qprep(SeqTable t, Dims d, QprepArgs a) 
 // read different parts of the same projection and are independent.
 __global__ __launch_bounds__(256) void k_append_qprep(SeqTable t, Dims d, AppendArgs aa, QprepArgs qa, int na) {
     if ((int)blockIdx.x < na) append_body(t, d, aa, blockIdx.x);
-    else if (qa.quarter) qprep_quarter(t, qa, blockIdx.x - na, d.NH);
+    else if (qa.quarter) {
+        const int lane_pos = t.s[threadIdx.x & 63].pos;
+        qprep_quarter(t.n, [&](int b) { return __shfl(lane_pos, b); }, qa, blockIdx.x - na, d.NH);
+    }
     else qprep_body(t, d, qa, blockIdx.x - na);
 }
 
@@ -1443,6 +1459,65 @@ hipError_t launch_append_qprep(hipStream_t st, int fmt, const SeqTable &t, const
                  ukt != nullptr ? 1 : 0;
     const int nq = qa.quarter ? (t.n + 7) / 8 * d.NH * 4 : t.n * d.NH;
     hipLaunchKernelGGL(k_append_qprep, dim3(t.n + nq), dim3(256), 0, st, t, d, aa, qa, t.n);
+    return hipGetLastError();
+}
+
+// The rows and the queries of a tree launch group (R = 512, DN = 128, DR = 64): blocks [0, na) append four
+// rows each, a wave per row, the rest prepare the queries of eight nodes. Node k: row ctx + i of its
+// sequence, i = k - node0, at position ctx + depth.
+struct TreePrepArgs {
+    TreeRowsTable t;
+    uint8_t seq[kTreeGroup], depth[kTreeGroup];
+    AppendArgs aa;
+    QprepArgs qa;
+    int n, na, NH;
+};
+static_assert(sizeof(TreePrepArgs) <= 4096 && kTreeGroup <= 4 * 64, "kernel arguments; four nodes per lane");
+template <int FMT>
+__global__ __launch_bounds__(256) void k_tree_prep(TreePrepArgs a) {
+    const int l = threadIdx.x & 63;
+    const TreeRows q = a.t.s[l];
+    const uint32_t seq4 = ((const uint32_t *)a.seq)[l], depth4 = ((const uint32_t *)a.depth)[l];
+    if ((int)blockIdx.x >= a.na) {
+        auto pos = [&](int b) {
+            const int sh = 8 * (b & 3);
+            return __shfl(q.ctx, (__shfl((int)seq4, b >> 2) >> sh) & 255) + ((__shfl((int)depth4, b >> 2) >> sh) & 255);
+        };
+        qprep_quarter(a.n, pos, a.qa, blockIdx.x - a.na, a.NH);
+        return;
+    }
+    const int k = __builtin_amdgcn_readfirstlane((int)blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (k >= a.n) return;
+    float nw[8];
+#pragma unroll
+    for (int c = 0; c < 8; ++c) nw[c] = bf16_to_f32(a.aa.norm[l + 64 * c]);
+    const int b = (lane_pick((int)seq4, k >> 2) >> (8 * (k & 3))) & 255, dep = (lane_pick((int)depth4, k >> 2) >> (8 * (k & 3))) & 255;
+    const int ctx = lane_pick(q.ctx, b), i = k - lane_pick(q.node0, b);
+    append_row_wave<FMT>(lane_pick(q.a, b), lane_pick(q.b, b), lane_pick(q.c, b), (size_t)ctx + i, ctx + dep,
+                         a.aa.y + (size_t)k * a.aa.ldy + a.aa.koff, a.aa, nw, a.aa.rows + (size_t)k * a.aa.row_bytes);
+}
+
+bool tree_prep_ok(const Dims &d, int ynp, const uint16_t *ukt) {
+    return d.R == 512 && d.DN == 128 && d.DR == 64 && d.QD == 192 && ynp == kGemvKs && ukt != nullptr;
+}
+hipError_t launch_tree_prep(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
+                            const uint16_t *kv_a_norm, float eps, const float2 *rope_cs, const uint16_t *kv_b,
+                            const uint16_t *ukt, const DecodeWork &w) {
+    if (!tree_prep_ok(d, w.ynp, ukt) || t.nodes < 1 || t.nodes > kTreeGroup || t.n < 1 || t.n > kMaxBatch) return hipErrorInvalidValue;
+    TreePrepArgs a;
+    a.t = tree_rows(t);
+    memcpy(a.seq, nd.seq, sizeof a.seq);
+    memcpy(a.depth, nd.depth, sizeof a.depth);
+    a.aa = append_args(fmt, d, w.y, d.QO + d.KVO, d.QO, w.ynp, w.ypstride, kv_a_norm, eps, rope_cs, w, false, 0);
+    a.qa = qprep_args(fmt, d, kv_b, ukt, rope_cs, w, false);
+    a.n = t.nodes;
+    a.na = (t.nodes + 3) / 4;
+    a.NH = d.NH;
+    const dim3 grid((unsigned)(a.na + (t.nodes + 7) / 8 * d.NH * 4));
+    if (fmt == kFmtQ8) hipLaunchKernelGGL(k_tree_prep<kFmtQ8>, grid, dim3(256), 0, st, a);
+    else if (fmt == kFmtF32) hipLaunchKernelGGL(k_tree_prep<kFmtF32>, grid, dim3(256), 0, st, a);
+    else if (fmt == kFmtBF16) hipLaunchKernelGGL(k_tree_prep<kFmtBF16>, grid, dim3(256), 0, st, a);
+    else return hipErrorInvalidValue;
     return hipGetLastError();
 }
 

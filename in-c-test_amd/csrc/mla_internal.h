@@ -95,9 +95,11 @@ hipError_t launch_gemv_ksplit(hipStream_t st, float *Y, size_t pstride, int ldy,
                               int out1, int in, unsigned *zero_flags = nullptr, int nzero = 0);
 // The same kGemvKs partials (bit for bit) for S tokens given as bf16 planes XH, XL [S, in]
 // (k_split's rounding), tiled over 128 tokens so a weight tile serves many of them: the
-// prefill's kv_a projection and the state prefill. Shapes as launch_gemv_ksplit.
+// prefill's kv_a projection and the state prefill. The output rows are the concatenation of W (out0 rows)
+// and W1 (out1 rows, may be 0). Shapes as launch_gemv_ksplit.
 hipError_t launch_kva_tok(hipStream_t st, float *Y, size_t pstride, int ldy, const uint16_t *XH,
-                          const uint16_t *XL, int S, const uint16_t *W, int out, int in);
+                          const uint16_t *XL, int S, const uint16_t *W, int out0, int in,
+                          const uint16_t *W1 = nullptr, int out1 = 0);
 // Y[b, o] (+)= sum_k W[o, k] x[b, k] with x given as bf16 planes XS[2][B][in] (hi, lo), as
 // launch_combine writes them (DecodeWork::hos). Shapes when gemv_xs_ok (in = 2048 or 4096),
 // any B.
@@ -241,8 +243,7 @@ hipError_t launch_empty(hipStream_t st);
 
 // ---- trees and rows (mla_tree.hip) ----
 // A tree decode: the nodes of one or more sequences' drafts, each node attending its sequence's
-// history, its ancestors and itself. A launch group: up to kMaxBatch sequences and kTreeGroup nodes; what
-// is told per node travels in kernel arguments for kTreeNodes nodes at a time.
+// history, its ancestors and itself. A launch group: up to kMaxBatch sequences and kTreeGroup nodes.
 constexpr int kTreeNodes = 64;   // nodes of one tree
 constexpr int kTreeGroup = 256;
 struct TreeSeq {
@@ -260,11 +261,30 @@ struct TreeTable {
     int units;  // history workgroups
     int nm;  // nodes per history workgroup (2 or 4); 0: the route for any dims (every row in one partial)
 };
-struct TreeNodes {  // nodes first .. first + n - 1 of the group
-    uint64_t path[kTreeNodes];  // the node and its ancestors: bit i = node i of its tree
-    uint8_t seq[kTreeNodes];    // its sequence
-    int first, n;
+// What the kernels that go by node need of a sequence (kernel arguments stay below 4 KB).
+struct TreeRows {
+    void *a, *b, *c;
+    int ctx, node0, part0, ns;
 };
+struct TreeRowsTable {
+    TreeRows s[kMaxBatch];
+};
+inline TreeRowsTable tree_rows(const TreeTable &t) {
+    TreeRowsTable r{};
+    for (int b = 0; b < t.n; ++b) r.s[b] = {t.s[b].a, t.s[b].b, t.s[b].c, t.s[b].ctx, t.s[b].node0, t.s[b].part0, t.s[b].ns};
+    return r;
+}
+struct TreeNodes {  // of every node of the group
+    uint8_t seq[kTreeGroup];     // its sequence
+    int8_t parent[kTreeGroup];   // its parent within its tree, or -1
+    uint8_t depth[kTreeGroup];   // 0: a child of the history
+};
+// The nodes' rows (w.y's kv_a part: appended to the histories, copies at w.rows) and queries (w.qf), where
+// tree_prep_ok: launch_append_qprep's results bit for bit.
+bool tree_prep_ok(const Dims &d, int ynp, const uint16_t *ukt);
+hipError_t launch_tree_prep(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
+                            const uint16_t *kv_a_norm, float eps, const float2 *rope_cs, const uint16_t *kv_b,
+                            const uint16_t *ukt, const DecodeWork &w);
 // The plan of a group (t.n, t.nodes, t.s[].ctx, count, node0 given): nm, the splits and the partials;
 // returns the number of partials.
 int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu);
@@ -274,6 +294,8 @@ hipError_t launch_tree_history(hipStream_t st, int fmt, const TreeTable &t, cons
 // t.nodes * HO (nm != 0).
 hipError_t launch_tree_combine(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
                                const uint16_t *kv_b, const DecodeWork &w);
+// Y[b, o] (+)= the kGemvKs partials' sum in their order, [n] values pstride apart (n % 4 == 0, 16-byte aligned).
+hipError_t launch_tree_sum(hipStream_t st, float *Y, const float *P, size_t pstride, size_t n, bool accumulate);
 // Attention of the nodes over all their rows into w.part (nm == 0).
 hipError_t launch_tree_generic(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
                                const DecodeWork &w);

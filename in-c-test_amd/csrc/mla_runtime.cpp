@@ -1934,6 +1934,9 @@ size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &t
     return (size_t)plan_tree(fmt, d, tt, ctx().ncu) * d.NH * (d.R + 2) * sizeof(float);
 }
 
+// Nodes from which on a group's projections are products over LDS tiles instead of the decode's GEMVs.
+constexpr int kTreeGemm = 64;
+
 // One tree decode of a launch group: the steps of decode_group with the group's nodes as its
 // members, each member's row at history row ctx + i and its rotation at position ctx + depth.
 // Everything it needs has been acquired (tree_prepare).
@@ -1954,71 +1957,84 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         HIP_TRY(launch_rmsnorm(st, in_norm->buf, d_x, in_norm->w, d.H, N, eps));
         d_x = in_norm->buf;
     }
+    // The projections of many nodes as products over LDS tiles, the same partials bit for bit (launch_kva_tok);
+    // the planes of x take the place of kv, which only the expanded format uses.
+    const bool many = N > kTreeGemm && gemv_ksplit_ok(d.H, d.H) && d.KVB >= d.H;
     if (gemv_ksplit_ok(d.H, d.H)) {
-        if (((uintptr_t)d_x % 16) != 0) {  // the kernel reads 16-byte vectors
+        if (((uintptr_t)d_x % 16) != 0) {  // the kernels read 16-byte vectors
             HIP_TRY(hipMemcpyAsync(w.x, d_x, (size_t)N * d.H * sizeof(float), hipMemcpyDeviceToDevice, st));
             d_x = w.x;
         }
         w.ynp = kGemvKs;
         w.ypstride = (size_t)N * ldy;
-        HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
+        if (many) {
+            uint16_t *xh = (uint16_t *)w.kv, *xl = xh + (size_t)N * d.H;
+            HIP_TRY(launch_split(st, d_x, d.H, xh, xl, d.H, N, d.H));
+            HIP_TRY(launch_kva_tok(st, w.y, w.ypstride, ldy, xh, xl, N, dw.q, d.QO, d.H, dw.kva, d.KVO));
+        } else {
+            HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
+        }
     } else {
         w.ynp = 1;
         w.ypstride = 0;
         HIP_TRY(launch_gemv(st, w.y, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H, false));
     }
-    // What is told per node goes kTreeNodes nodes at a time.
-    const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0), qs = (size_t)std::max(d.R + d.DR, d.QD);
-    const float2 *cs = nullptr;
-    TreeNodes nds[(kTreeGroup + kTreeNodes - 1) / kTreeNodes];
-    int b = 0, i = 0, dep[kTreeNodes];
-    uint64_t path[kTreeNodes];
-    for (int k0 = 0, z = 0; k0 < N; k0 += kTreeNodes, ++z) {
-        TreeNodes &nd = nds[z];
-        SeqTable t;
-        memset(&t, 0, sizeof t);
-        memset(&nd, 0, sizeof nd);
-        nd.first = k0;
-        nd.n = t.n = std::min(kTreeNodes, N - k0);
-        int maxpos = 0;
-        for (int k = 0; k < t.n; ++k, ++i) {
-            while (i == seqs[b].count) {
-                i = 0;
-                ++b;
-            }
-            const TreeIn &q = seqs[b];
-            const int p = q.parents[i];
-            dep[i] = p < 0 ? 0 : dep[p] + 1;
-            path[i] = (p < 0 ? 0 : path[p]) | (uint64_t)1 << i;
-            nd.path[k] = path[i];
+    TreeNodes nd;
+    memset(&nd, 0, sizeof nd);
+    int maxpos = 0;
+    for (int b = 0, k = 0; b < n; ++b) {
+        const int k0 = k;
+        for (int i = 0; i < seqs[b].count; ++i, ++k) {
+            const int p = seqs[b].parents[i];
             nd.seq[k] = (uint8_t)b;
-            SeqDesc &s = t.s[k];
-            s.a = q.m->a;
-            s.b = q.m->b;
-            s.c = q.m->c;
-            s.pos = q.ctx + dep[i];
-            s.roff = i - dep[i];
-            maxpos = std::max(maxpos, s.pos);
+            nd.parent[k] = (int8_t)p;
+            nd.depth[k] = (uint8_t)(p < 0 ? 0 : nd.depth[k0 + p] + 1);
+            maxpos = std::max(maxpos, seqs[b].ctx + nd.depth[k]);
         }
-        if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
-        DecodeWork wk = w;
-        wk.y += (size_t)k0 * ldy;
-        wk.qf += (size_t)k0 * d.NH * qs;
-        wk.rows += (size_t)k0 * rb;
-        HIP_TRY(launch_append_qprep(st, fmt, t, d, wk.y, ldy, d.QO, w.ynp, w.ypstride, dw.norm, eps, cs, dw.kvb,
-                                    dw.ukt, wk, false));
+    }
+    const float2 *cs = nullptr;
+    if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
+    if (tree_prep_ok(d, w.ynp, dw.ukt)) {
+        HIP_TRY(launch_tree_prep(st, fmt, tt, nd, d, dw.norm, eps, cs, dw.kvb, dw.ukt, w));
+    } else {
+        const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0);
+        for (int k0 = 0; k0 < N; k0 += kMaxBatch) {
+            SeqTable t;
+            memset(&t, 0, sizeof t);
+            t.n = std::min(kMaxBatch, N - k0);
+            for (int k = 0; k < t.n; ++k) {
+                const TreeSeq &q = tt.s[nd.seq[k0 + k]];
+                t.s[k].a = q.a;
+                t.s[k].b = q.b;
+                t.s[k].c = q.c;
+                t.s[k].pos = q.ctx + nd.depth[k0 + k];
+                t.s[k].roff = k0 + k - q.node0 - nd.depth[k0 + k];
+            }
+            DecodeWork wk = w;
+            wk.y += (size_t)k0 * ldy;
+            wk.qf += (size_t)k0 * d.NH * std::max(d.R + d.DR, d.QD);
+            wk.rows += (size_t)k0 * rb;
+            HIP_TRY(launch_append_qprep(st, fmt, t, d, wk.y, ldy, d.QO, w.ynp, w.ypstride, dw.norm, eps, cs, dw.kvb, dw.ukt, wk,
+                                        false));
+        }
     }
     if (tt.nm) {
         HIP_TRY(launch_tree_history(st, fmt, tt, d, w));
-        for (int k0 = 0, z = 0; k0 < N; k0 += kTreeNodes, ++z) HIP_TRY(launch_tree_combine(st, fmt, tt, nds[z], d, dw.kvb, w));
-        HIP_TRY(launch_gemv_xs(st, d_out, d.H, w.hos, N, dw.o, d.H, d.HO, residual));
+        HIP_TRY(launch_tree_combine(st, fmt, tt, nd, d, dw.kvb, w));
+        if (many && d.H <= ldy && d.H % 4 == 0 && (uintptr_t)d_out % 16 == 0) {  // partials in the place of w.y
+            const size_t ps = (size_t)N * d.H;
+            HIP_TRY(launch_kva_tok(st, w.y, ps, d.H, w.hos, w.hos + (size_t)N * d.HO, N, dw.o, d.H, d.HO));
+            HIP_TRY(launch_tree_sum(st, d_out, w.y, ps, ps, residual));
+        } else {
+            HIP_TRY(launch_gemv_xs(st, d_out, d.H, w.hos, N, dw.o, d.H, d.HO, residual));
+        }
         return 0;
     }
-    for (int k0 = 0, z = 0; k0 < N; k0 += kTreeNodes, ++z) {
-        HIP_TRY(launch_tree_generic(st, fmt, tt, nds[z], d, w));
+    HIP_TRY(launch_tree_generic(st, fmt, tt, nd, d, w));
+    for (int k0 = 0; k0 < N; k0 += kMaxBatch) {
         SeqTable t;
         memset(&t, 0, sizeof t);
-        t.n = nds[z].n;
+        t.n = std::min(kMaxBatch, N - k0);
         for (int k = 0; k < t.n; ++k) {
             t.s[k].split0 = k0 + k;
             t.s[k].nsplit = 1;

@@ -19,15 +19,6 @@ namespace kvl {
 //   s_j = (q_lat . lat_j + q_rope . key_j) / sqrt(QD),  mix = sum_j softmax(s)_j lat_j.
 // Rows of other branches are never read for it, so nothing they hold (NaN, infinities) reaches it.
 
-// What the kernels that go by node need of a sequence (kernel arguments stay below 4 KB).
-struct TreeRows {
-    void *a, *b, *c;
-    int ctx, node0, part0, ns;
-};
-struct TreeRowsTable {
-    TreeRows s[kMaxBatch];
-};
-
 template <int FMT>
 __device__ __forceinline__ float tree_lat(const TreeRows &s, size_t row, int R, int k) {
     if (FMT == kFmtQ8) return (float)((const int8_t *)s.a)[row * R + k] * ((const float *)s.b)[row];
@@ -55,11 +46,6 @@ struct TreeNodeArgs {
     float smscale;
     int NH, R, DR;
 };
-static TreeRowsTable tree_rows(const TreeTable &t) {
-    TreeRowsTable r{};
-    for (int b = 0; b < t.n; ++b) r.s[b] = {t.s[b].a, t.s[b].b, t.s[b].c, t.s[b].ctx, t.s[b].node0, t.s[b].part0, t.s[b].ns};
-    return r;
-}
 
 constexpr int kTgRows = 256;  // rows taken at a time: a thread per row
 constexpr int kTgCols = 4;    // latent columns per thread: R <= 1024
@@ -75,13 +61,14 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
     __shared__ int path[kTreeNodes];
     __shared__ int npath;
     const int tid = threadIdx.x, NH = a.NH, R = a.R, DR = a.DR;
-    const int k = a.nd.first + blockIdx.x / NH, h = blockIdx.x % NH;
-    const TreeRows s = a.t.s[a.nd.seq[k - a.nd.first]];
+    const int k = blockIdx.x / NH, h = blockIdx.x % NH;
+    const TreeRows s = a.t.s[a.nd.seq[k]];
     for (int i = tid; i < R + DR; i += 256) q[i] = a.qf[((size_t)k * NH + h) * (R + DR) + i];
     if (tid == 0) {  // the node and its ancestors, in the order of their rows
         int n = 0;
-        for (uint64_t m = a.nd.path[k - a.nd.first]; m; m &= m - 1) path[n++] = __builtin_ctzll(m);
+        for (int i = k - s.node0; i >= 0; i = a.nd.parent[s.node0 + i]) ++n;
         npath = n;
+        for (int i = k - s.node0; i >= 0; i = a.nd.parent[s.node0 + i]) path[--n] = i;
     }
     __syncthreads();
     const int rows = s.ctx + npath;
@@ -677,7 +664,7 @@ struct TreeCombArgs {
     uint16_t *hos;
     size_t plane;  // words between the hi and lo planes of hos
     float smscale;
-    int DN, tn;  // tn: nodes per workgroup (1, 2, 4)
+    int DN, n, tn;  // n nodes, tn of them per workgroup (1, 2, 4)
 };
 
 // Workgroup = one head of tn nodes, eight waves, 8 / tn of them per node (in turn over the history's splits).
@@ -698,25 +685,28 @@ __global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
     const int h = blockIdx.x % NH, tn = a.tn, first = blockIdx.x / NH * tn;
     // this lane's entries of the tables
     const TreeRows q = a.t.s[l];
-    const uint64_t lane_path = a.nd.path[l];
-    const int lane_seq = a.nd.seq[l];
+    const int seq4 = ((const int *)a.nd.seq)[l], parent4 = ((const int *)a.nd.parent)[l];  // four nodes a lane
     const uint16_t *wrow = a.kv_b + ((size_t)h * (a.DN + 128) + a.DN + 16 * w + n) * R + 8 * g;
     v4i wa[16];
 #pragma unroll
     for (int kb = 0; kb < 16; ++kb) wa[kb] = *(const v4i *)(wrow + 32 * kb);
     const int wpn = 8 / tn, j = w / wpn, u = w % wpn;  // node of the workgroup, turn
-    const int k = min(first + j, a.nd.n - 1);
-    const int b = tree_lane(lane_seq, k);
+    const int k = min(first + j, a.n - 1);
+    const int b = (tree_lane(seq4, k >> 2) >> (8 * (k & 3))) & 255;
     const TreeRows s{tree_lane(q.a, b), tree_lane(q.b, b), tree_lane(q.c, b), tree_lane(q.ctx, b), tree_lane(q.node0, b),
                      tree_lane(q.part0, b), tree_lane(q.ns, b)};
-    const int ns = s.ns, i0 = a.nd.first + k - s.node0;
+    const int ns = s.ns, i0 = k - s.node0;
     const float *P = a.part + (size_t)(s.part0 + i0 * ns) * (NH * (R + 2));
     constexpr size_t stride = NH * (R + 2);
     const float *Pm = P + NH * R + h, *Pa = P + h * R + 4 * l;
 
     // ---- the path's requests (the node's first wave): the head's query, the first four rows
-    const uint32_t mlo = (uint32_t)tree_lane((int)(uint32_t)lane_path, k), mhi = (uint32_t)tree_lane((int)(uint32_t)(lane_path >> 32), k);
-    const uint64_t mask = ((uint64_t)mhi << 32) | mlo;
+    uint64_t mask = 0;  // bit i: node i of the tree is on the path
+    for (int i = i0; i >= 0;) {
+        mask |= (uint64_t)1 << i;
+        const int z = s.node0 + i;
+        i = (int8_t)(tree_lane(parent4, z >> 2) >> (8 * (z & 3)));
+    }
     const int np = __builtin_popcountll(mask);
     struct Row {  // four + four latents and a key element of a row, as stored
         v4f f0, f1;
@@ -772,7 +762,7 @@ __global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
     float qk = 0.f;
     uint64_t left = mask;
     if (u == 0) {
-        const float *qr = a.qf + ((size_t)(a.nd.first + k) * NH + h) * (R + DR);
+        const float *qr = a.qf + ((size_t)k * NH + h) * (R + DR);
         q0 = *(const v4f *)(qr + 4 * l);
         q1 = *(const v4f *)(qr + 256 + 4 * l);
         qk = qr[R + l];
@@ -895,14 +885,32 @@ __global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
     for (int i = 0; i < 4; ++i) {
         const float mid = dpp_f32<0x12C>(acc[i]), low = dpp_f32<0x128>(acc[i]);  // row_ror:12, row_ror:8: lanes n + 4, n + 8
         const float v = acc[i] + (mid + low);
-        if (n < tn && node < a.nd.n) {
+        if (n < tn && node < a.n) {
             uint16_t hi, lo;
             split_bf16(v, hi, lo);
-            const size_t o = (size_t)(a.nd.first + node) * (NH * 128) + h * 128 + 16 * w + 4 * g + i;
+            const size_t o = (size_t)node * (NH * 128) + h * 128 + 16 * w + 4 * g + i;
             a.hos[o] = hi;
             a.hos[a.plane + o] = lo;
         }
     }
+}
+
+__global__ __launch_bounds__(256) void k_tree_sum(float *Y, const float *P, size_t pstride, size_t n4, int acc) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= n4) return;
+    v4f p[kGemvKs];
+#pragma unroll
+    for (int q = 0; q < kGemvKs; ++q) p[q] = *(const v4f *)(P + q * pstride + 4 * i);
+    const v4f y = acc ? *(const v4f *)(Y + 4 * i) : v4f{0.f, 0.f, 0.f, 0.f};
+    v4f s = p[0];
+#pragma unroll
+    for (int q = 1; q < kGemvKs; ++q) s += p[q];
+    *(v4f *)(Y + 4 * i) = acc ? y + s : s;
+}
+hipError_t launch_tree_sum(hipStream_t st, float *Y, const float *P, size_t pstride, size_t n, bool accumulate) {
+    if (n == 0 || n % 4 || pstride % 4 || (uintptr_t)Y % 16 || (uintptr_t)P % 16) return hipErrorInvalidValue;
+    hipLaunchKernelGGL(k_tree_sum, dim3((unsigned)((n / 4 + 255) / 256)), dim3(256), 0, st, Y, P, pstride, n / 4, accumulate ? 1 : 0);
+    return hipGetLastError();
 }
 
 // Splits of the history, r rows each (a multiple of the chunk, at least kThMin). A launch of k rounds of
@@ -992,12 +1000,11 @@ hipError_t launch_tree_history(hipStream_t st, int fmt, const TreeTable &t, cons
 
 hipError_t launch_tree_combine(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
                                const uint16_t *kv_b, const DecodeWork &w) {
-    if (!tree_table_ok(fmt, t, d, true) || nd.n < 1 || nd.n > kTreeNodes || nd.first < 0 || nd.first + nd.n > t.nodes)
-        return hipErrorInvalidValue;
-    TreeCombArgs a{tree_rows(t), nd, w.qf, w.part, kv_b, w.hos, (size_t)t.nodes * d.HO, 1.0f / sqrtf((float)d.QD), d.DN, 1};
+    if (!tree_table_ok(fmt, t, d, true)) return hipErrorInvalidValue;
+    TreeCombArgs a{tree_rows(t), nd, w.qf, w.part, kv_b, w.hos, (size_t)t.nodes * d.HO, 1.0f / sqrtf((float)d.QD), d.DN, t.nodes, 1};
     // nodes per workgroup: enough workgroups for the CUs first, then W_UV (128 KB a workgroup) shared by more
-    a.tn = nd.n <= 16 ? 1 : nd.n <= 32 ? 2 : 4;
-    const dim3 grid((unsigned)((nd.n + a.tn - 1) / a.tn * 16));
+    a.tn = t.nodes <= 16 ? 1 : t.nodes <= 32 ? 2 : 4;
+    const dim3 grid((unsigned)((t.nodes + a.tn - 1) / a.tn * 16));
     if (fmt == kFmtQ8) hipLaunchKernelGGL(k_tree_combine<kFmtQ8>, grid, dim3(512), 0, st, a);
     else if (fmt == kFmtF32) hipLaunchKernelGGL(k_tree_combine<kFmtF32>, grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL(k_tree_combine<kFmtBF16>, grid, dim3(512), 0, st, a);
@@ -1005,13 +1012,13 @@ hipError_t launch_tree_combine(hipStream_t st, int fmt, const TreeTable &t, cons
 }
 
 static_assert(sizeof(TreeCombArgs) <= 4096 && sizeof(TreeNodeArgs) <= 4096 && sizeof(TreeArgs) <= 4096, "kernel arguments");
+static_assert(kTreeGroup == 4 * 64, "four nodes a lane");
 
 hipError_t launch_tree_generic(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
                                const DecodeWork &w) {
-    if (!tree_table_ok(fmt, t, d, false) || nd.n < 1 || nd.n > kTreeNodes || nd.first < 0 || nd.first + nd.n > t.nodes)
-        return hipErrorInvalidValue;
+    if (!tree_table_ok(fmt, t, d, false)) return hipErrorInvalidValue;
     const TreeNodeArgs a{tree_rows(t), nd, w.qf, w.part, 1.0f / sqrtf((float)d.QD), d.NH, d.R, d.DR};
-    const dim3 grid((unsigned)(nd.n * d.NH));
+    const dim3 grid((unsigned)(t.nodes * d.NH));
     if (fmt == kFmtQ8) hipLaunchKernelGGL(k_tree_generic<kFmtQ8>, grid, dim3(256), 0, st, a);
     else if (fmt == kFmtF32) hipLaunchKernelGGL(k_tree_generic<kFmtF32>, grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL(k_tree_generic<kFmtBF16>, grid, dim3(256), 0, st, a);
