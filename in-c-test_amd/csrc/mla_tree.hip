@@ -675,8 +675,8 @@ struct TreeCombArgs {
 //   W_UV: head output d = sum_r W[d, r] mix[r] on MFMA, wave w rows 16 w .., its W operands requested at the
 //     start; the mix enters as three bf16 planes (24 bits), plane p of node j as column 4 p + j.
 // The output is written as the bf16 hi | lo planes that o_proj's launch takes.
-template <int FMT>
-__global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
+template <int FMT, bool EARLY>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(EARLY ? 2 : 4))) void k_tree_combine(TreeCombArgs a) {
     constexpr int R = 512, DR = 64, NH = 16;
     __shared__ __attribute__((aligned(16))) uint8_t xs[16 * 1024];  // column c's words of 8: word ^ (c & 15)
     __shared__ __attribute__((aligned(16))) float red[8][R];
@@ -688,8 +688,9 @@ __global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
     const int seq4 = ((const int *)a.nd.seq)[l], parent4 = ((const int *)a.nd.parent)[l];  // four nodes a lane
     const uint16_t *wrow = a.kv_b + ((size_t)h * (a.DN + 128) + a.DN + 16 * w + n) * R + 8 * g;
     v4i wa[16];
+    if constexpr (EARLY)
 #pragma unroll
-    for (int kb = 0; kb < 16; ++kb) wa[kb] = *(const v4i *)(wrow + 32 * kb);
+        for (int kb = 0; kb < 16; ++kb) wa[kb] = *(const v4i *)(wrow + 32 * kb);
     const int wpn = 8 / tn, j = w / wpn, u = w % wpn;  // node of the workgroup, turn
     const int k = min(first + j, a.n - 1);
     const int b = (tree_lane(seq4, k >> 2) >> (8 * (k & 3))) & 255;
@@ -844,6 +845,9 @@ __global__ __launch_bounds__(512) void k_tree_combine(TreeCombArgs a) {
             }
         }
     }
+    if constexpr (!EARLY)
+#pragma unroll
+        for (int kb = 0; kb < 16; ++kb) wa[kb] = *(const v4i *)(wrow + 32 * kb);
     if (wpn > 1) {  // the node's waves in turn order
         *(v4f *)&red[w][4 * l] = c0;
         *(v4f *)&red[w][256 + 4 * l] = c1;
@@ -1005,9 +1009,11 @@ hipError_t launch_tree_combine(hipStream_t st, int fmt, const TreeTable &t, cons
     // nodes per workgroup: enough workgroups for the CUs first, then W_UV (128 KB a workgroup) shared by more
     a.tn = t.nodes <= 16 ? 1 : t.nodes <= 32 ? 2 : 4;
     const dim3 grid((unsigned)((t.nodes + a.tn - 1) / a.tn * 16));
-    if (fmt == kFmtQ8) hipLaunchKernelGGL(k_tree_combine<kFmtQ8>, grid, dim3(512), 0, st, a);
-    else if (fmt == kFmtF32) hipLaunchKernelGGL(k_tree_combine<kFmtF32>, grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL(k_tree_combine<kFmtBF16>, grid, dim3(512), 0, st, a);
+    const bool early = t.nodes <= 64;  // one workgroup per CU
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(512), 0, st, a); };
+    if (fmt == kFmtQ8) early ? go(k_tree_combine<kFmtQ8, true>) : go(k_tree_combine<kFmtQ8, false>);
+    else if (fmt == kFmtF32) early ? go(k_tree_combine<kFmtF32, true>) : go(k_tree_combine<kFmtF32, false>);
+    else early ? go(k_tree_combine<kFmtBF16, true>) : go(k_tree_combine<kFmtBF16, false>);
     return hipGetLastError();
 }
 
