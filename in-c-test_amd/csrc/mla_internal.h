@@ -312,8 +312,9 @@ struct ForkTable {
     ForkDesc d[kForkBatch];
     int n;
     int e[3];
+    uint8_t run[kForkBatch + 1];  // set by the launch: the first pair of each run of one source and range
 };
-hipError_t launch_fork(hipStream_t st, const ForkTable &t);
+hipError_t launch_fork(hipStream_t st, ForkTable &t);
 // Rows start + path[i] to start + i, i < n, path strictly increasing.
 struct AcceptDesc {
     void *p[3];
