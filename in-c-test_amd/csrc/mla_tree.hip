@@ -917,11 +917,17 @@ hipError_t launch_tree_sum(hipStream_t st, float *Y, const float *P, size_t pstr
     return hipGetLastError();
 }
 
-// Splits of the history, r rows each (a multiple of the chunk, at least kThMin). A launch of k rounds of
-// workgroups (ceil(count / nm) per split) on the CUs takes about k (r / kThCh + kThStart) chunks' time, the
-// start of a workgroup (its queries, its first chunk) being worth kThStart chunks: for each k up to
-// kThRounds the fewest rows that make k rounds, and of these the shortest.
-constexpr int kThMin = 64, kThMax = 1 << 19, kThStart = 4, kThRounds = 4;
+// Splits of the history, r rows each: one chunk where that makes at most kThFew workgroups, else a multiple
+// of the chunk, at least kThMin. A launch of k rounds of workgroups (ceil(count / nm) per split) on the CUs
+// takes about k (r / kThCh + kThStart) chunks' time, the start of a workgroup (its queries, its first chunk)
+// being worth kThStart chunks: for each k up to kThRounds the fewest rows that make k rounds, and of these
+// the shortest.
+// kThFew, history and combine together, one chunk against two (FP32, BF16, Q8): 400 rows x 7 nodes (26
+// workgroups) 23.8 / 26.5, 22.5 / 23.0, 24.1 / 25.3 us; 1400 x 8 (88) 28.3 / 28.3, 26.3 / 25.0, 28.3 / 26.9;
+// 2048 x 8 (128) 30.3 / 30.0, 28.8 / 26.3, 30.9 / 28.7.
+// nm: two nodes of a tree of 13 leave half of each pair of tiles' reads to L2: 64 nodes x 32768 rows of Q8
+// 176 us with 2 and 161 with 4, eight trees of at most 24 nodes BF16 89.4 and 85.3.
+constexpr int kThFew = 64, kThMin = 64, kThMax = 1 << 19, kThStart = 4, kThRounds = 4;
 int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
     const bool kimi = d.NH == 16 && d.R == 512 && d.DR == 64 && d.DV == 128;
     int most = 0, longest = 0;
@@ -940,7 +946,7 @@ int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
             return n;
         };
         // at most kThMax rows: offsets within a split stay below 2^31 bytes
-        const long least = kThMin / kThCh;
+        const long least = groups(1) <= kThFew ? 1 : kThMin / kThCh;
         long cost = LONG_MAX, hi = std::max(least, std::min<long>(splits(longest, kThCh), kThMax / kThCh));
         for (int k = 1; k <= kThRounds; ++k) {
             long lo = least, up = hi;
