@@ -294,7 +294,6 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         v2i lc[kQ8 ? NL : 1], kb[NK];
         float rsc;
     };
-    static_assert(KE == 2 || NK == 1, "FP32 rows: eight waves");
     const int lrow = tid >> 6;
     // the split's rows as buffers: a read past the last row gives zeros (its score is masked)
     const int nrow = r1 - r0;
@@ -345,8 +344,9 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 const v2f x = __builtin_bit_cast(v2f, f.kb[q]);
                 const v2bf hi = __builtin_convertvector(x, v2bf);
                 const v2bf lo = __builtin_convertvector((v2f{x.x - (float)hi.x, x.y - (float)hi.y}), v2bf);
-                *(int *)(buf + sk) = __builtin_bit_cast(int, hi);
-                *(int *)(buf + Sh::PlaneB + sk) = __builtin_bit_cast(int, lo);
+                const int at = (sk ^ (64 * q)) + q * 1024;  // 8 rows on (four waves): th_key flips one bit of the word
+                *(int *)(buf + at) = __builtin_bit_cast(int, hi);
+                *(int *)(buf + Sh::PlaneB + at) = __builtin_bit_cast(int, lo);
             } else {
                 *(v2i *)(buf + sk + q * (NT / 16) * 128) = f.kb[q];
             }
@@ -917,48 +917,52 @@ hipError_t launch_tree_sum(hipStream_t st, float *Y, const float *P, size_t pstr
     return hipGetLastError();
 }
 
-// Splits of the history, r rows each: one chunk where that makes at most kThFew workgroups, else a multiple
-// of the chunk, at least kThMin. A launch of k rounds of workgroups (ceil(count / nm) per split) on the CUs
-// takes about k (r / kThCh + kThStart) chunks' time, the start of a workgroup (its queries, its first chunk)
-// being worth kThStart chunks: for each k up to kThRounds the fewest rows that make k rounds, and of these
-// the shortest.
-// kThFew, history and combine together, one chunk against two (FP32, BF16, Q8): 400 rows x 7 nodes (26
-// workgroups) 23.8 / 26.5, 22.5 / 23.0, 24.1 / 25.3 us; 1400 x 8 (88) 28.3 / 28.3, 26.3 / 25.0, 28.3 / 26.9;
-// 2048 x 8 (128) 30.3 / 30.0, 28.8 / 26.3, 30.9 / 28.7.
-// nm: two nodes of a tree of 13 leave half of each pair of tiles' reads to L2: 64 nodes x 32768 rows of Q8
-// 176 us with 2 and 161 with 4, eight trees of at most 24 nodes BF16 89.4 and 85.3.
-constexpr int kThFew = 64, kThMin = 64, kThMax = 1 << 19, kThStart = 4, kThRounds = 4;
+// Nodes per workgroup and rows per split.
+// nm: 4 share a chunk's staging among twice the queries and overlap it with the products; 2 start sooner,
+// waste less of a small tree, and two workgroups a CU cover each other's waits. In chunks' times of the
+// former, four take kThStart4 / 10 + X4 / CUs and two kThStart2 / 10 + 1.1 X2 / (2 CUs), X the chunks times the
+// workgroups that share them: the lesser is taken. History and combine together, 2 / 4 nodes a workgroup
+//   (FP32, BF16, Q8) 400 rows x 7 nodes 19.1 / 23.5, 18.2 / 22.7, 18.9 / 24.5 us; 9000 x 13 44 / 47, 35 / 37,
+//   38 / 41; eight of 32768 x 2 127 / 154, 79 / 89, 67 / 95; 32768 x 16 99 / 91, 63 / 59, 68 / 65; history alone,
+//   eight of at most 32768 x 24 BF16 89 / 85, one of 32768 x 64 Q8 176 / 161.
+// rows: one chunk a split where that makes at most kThFew workgroups, else a multiple of the chunk, at least
+// kThMin. A launch of k rounds of workgroups takes about k (chunks + start), and the combine about one chunk's
+// time for each kThJoin splits of a sequence: for each k up to kThRounds the fewest rows that make k rounds
+// (or the rows at which fewer splits gain less than they cost), and of these the shortest. kThFew, history and
+// combine of 4 nodes per workgroup, one chunk against two (FP32, BF16, Q8): 400 rows x 7 nodes (26 workgroups)
+// 23.8 / 26.5, 22.5 / 23.0, 24.1 / 25.3 us; 1400 x 8 (88) 28.3 / 28.3, 26.3 / 25.0, 28.3 / 26.9; 2048 x 8 (128)
+// 30.3 / 30.0, 28.8 / 26.3, 30.9 / 28.7.
+constexpr int kThFew = 64, kThMin = 64, kThMax = 1 << 19, kThRounds = 4, kThStart4 = 47, kThStart2 = 34, kThJoin = 64;
 int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
     const bool kimi = d.NH == 16 && d.R == 512 && d.DR == 64 && d.DV == 128;
-    int most = 0, longest = 0;
-    for (int b = 0; b < t.n; ++b) {
-        most = std::max(most, t.s[b].count);
-        longest = std::max(longest, t.s[b].ctx);
-    }
-    t.nm = !kimi ? 0 : most > 2 || fmt == kFmtF32 ? 4 : 2;
+    int longest = 0;
+    for (int b = 0; b < t.n; ++b) longest = std::max(longest, t.s[b].ctx);
     auto splits = [](long ctx, long r) { return (ctx + r - 1) / r; };
+    auto groups = [&](long chunks, int nm) {
+        long n = 0;
+        for (int b = 0; b < t.n; ++b) n += (t.s[b].count + nm - 1) / nm * splits(t.s[b].ctx, chunks * kThCh);
+        return n;
+    };
+    t.nm = !kimi ? 0 : 20 * groups(1, 4) + 2L * ncu * kThStart4 < 11 * groups(1, 2) + 2L * ncu * kThStart2 ? 4 : 2;
     long best = kThMin / kThCh;  // in chunks
     if (t.nm) {
-        const long places = (long)ncu * (t.nm == 2 ? 2 : 1);
-        auto groups = [&](long chunks) {
-            long n = 0;
-            for (int b = 0; b < t.n; ++b) n += (t.s[b].count + t.nm - 1) / t.nm * splits(t.s[b].ctx, chunks * kThCh);
-            return n;
-        };
+        const long places = (long)ncu * (t.nm == 2 ? 2 : 1), start = t.nm == 2 ? kThStart2 : kThStart4;
         // at most kThMax rows: offsets within a split stay below 2^31 bytes
-        const long least = groups(1) <= kThFew ? 1 : kThMin / kThCh;
-        long cost = LONG_MAX, hi = std::max(least, std::min<long>(splits(longest, kThCh), kThMax / kThCh));
+        const long all = splits(longest, kThCh), least = groups(1, t.nm) <= kThFew * (4 / t.nm) ? 1 : kThMin / kThCh;
+        long cost = LONG_MAX, hi = std::max(least, std::min<long>(all, kThMax / kThCh)), even = least;
+        while (even * even * kThJoin < all && even < hi) ++even;
         for (int k = 1; k <= kThRounds; ++k) {
             long lo = least, up = hi;
             while (lo < up) {  // groups() does not increase with the chunks
                 const long mid = (lo + up) / 2;
-                if (groups(mid) <= k * places) up = mid;
+                if (groups(mid, t.nm) <= k * places) up = mid;
                 else lo = mid + 1;
             }
-            const long c = k * (lo + kThStart);
+            const long r = std::max(lo, even);
+            const long c = k * (10 * r + start) + 10 * splits(all, r) / kThJoin;
             if (c < cost) {
                 cost = c;
-                best = lo;
+                best = r;
             }
             hi = lo;  // more rounds need no more rows
             if (lo == least) break;
@@ -981,20 +985,15 @@ int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
 
 template <int FMT>
 static void tree_launch(hipStream_t st, const TreeArgs &a, unsigned grid) {
-    if constexpr (FMT != kFmtF32) {
-        if (a.t.nm == 2) {
-            hipLaunchKernelGGL((k_tree_hist<FMT, 2>), dim3(grid), dim3(256), 0, st, a);
-            return;
-        }
-    }
-    hipLaunchKernelGGL((k_tree_hist<FMT, 4>), dim3(grid), dim3(512), 0, st, a);
+    if (a.t.nm == 2) hipLaunchKernelGGL((k_tree_hist<FMT, 2>), dim3(grid), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_tree_hist<FMT, 4>), dim3(grid), dim3(512), 0, st, a);
 }
 
 static bool tree_table_ok(int fmt, const TreeTable &t, const Dims &d, bool kimi) {
     if (t.n < 1 || t.n > kMaxBatch || t.nodes < 1 || t.nodes > kTreeGroup) return false;
     if (fmt != kFmtQ8 && fmt != kFmtF32 && fmt != kFmtBF16) return false;
     if (!kimi) return t.nm == 0 && d.R <= 256 * kTgCols && d.DR <= 256;
-    return (t.nm == 4 || (t.nm == 2 && fmt != kFmtF32)) && d.NH == 16 && d.R == 512 && d.DR == 64 && d.DV == 128;
+    return (t.nm == 4 || t.nm == 2) && d.NH == 16 && d.R == 512 && d.DR == 64 && d.DV == 128;
 }
 
 hipError_t launch_tree_history(hipStream_t st, int fmt, const TreeTable &t, const Dims &d, const DecodeWork &w) {
