@@ -133,7 +133,8 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 // power of two that puts its largest element near 2^10) and the weights are split in fp16, which keeps 22
 // bits. A Q8 row's scale multiplies its latent score and its weight; to keep the weights within fp16
 // whatever the scales, the running maximum is that of score + ln(scale), so that weight times scale stays
-// <= 4.
+// <= 4. A scale below 1e-28 counts as 1e-28 there: over kThMax rows of scale zero the sum of the weights
+// stays below 2^(2 + 93 + 19), and 2^13 splits of them can still be added.
 constexpr int kThCh = 32;  // rows of a chunk (FP32: of two)
 template <int FMT, int NM>
 struct ThShape {
@@ -355,7 +356,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             if (tid < Ch) {
                 float *sc = (float *)(buf + NP * Sh::PlaneB);
                 sc[tid] = f.rsc;
-                sc[Ch + tid] = __builtin_amdgcn_logf(fmaxf(fabsf(f.rsc), 1e-35f));
+                sc[Ch + tid] = __builtin_amdgcn_logf(fmaxf(fabsf(f.rsc), 1e-28f));
             }
         }
     };

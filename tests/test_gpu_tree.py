@@ -218,6 +218,146 @@ def test_batch_equals_definition(models, kind, dims, lens, sizes):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_batch_of_large_trees(models, kind):
+    """Several launch groups, each with work for more than a round of workgroups; ragged trees and splits."""
+    cfg, layer, w = models("kimi")
+    sizes, lens = [64, 63, 61, 64, 62, 64, 64, 5], [3500, 3471, 3049, 4000, 3500, 3001, 3333, 31]
+    ps = [tree("any", n, 20 + i) for i, n in enumerate(sizes)]
+    states = [State(kind, cfg, m + n).load(i, m) for i, (m, n) in enumerate(zip(lens, sizes))]
+    x = hidden(cfg, 0x57, sum(sizes))
+    got = batch_device(kind, cfg, w, states, ps, x)
+    at = 0
+    for i, (m, n) in enumerate(zip(lens, sizes)):
+        some = sorted({0, n - 1, n // 2, n // 3, n - 3, n - 2})
+        want = reference(cfg, layer, x[at:at + n], ps[i], m, states[i].pull(0, m + n), kind, some)
+        e = off(got[at:at + n][some], want)
+        assert e <= TOL, (i, m, n, e)
+        at += n
+    for s in states:
+        s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_nodes_equal_few(models, kind):
+    """The rows of a batch of many nodes are those of its trees alone, bit for bit, and a node that is not
+    finite stays within its tree there too."""
+    cfg, layer, w = models("kimi")
+    sizes, lens = [40, 50, 33], [90, 10, 200]
+    ps = [tree("any", n, 30 + i) for i, n in enumerate(sizes)]
+    x = hidden(cfg, 0x58, sum(sizes))
+    x[44, :] = np.nan
+    both = [State(kind, cfg, m + n).load(i, m) for i, (m, n) in enumerate(zip(lens, sizes))]
+    got = batch_device(kind, cfg, w, both, ps, x)
+    at = 0
+    for i, (m, n) in enumerate(zip(lens, sizes)):
+        alone = State(kind, cfg, m + n).load(i, m)
+        out = batch_device(kind, cfg, w, [alone], [ps[i]], x[at:at + n])
+        rows = [k for k in range(n) if at + k != 44]
+        for a, b in zip(alone.pull(m, m + n), both[i].pull(m, m + n)):
+            np.testing.assert_array_equal(a[rows], b[rows])
+        fine = [k for k in range(n) if at + k != 44 and not (i == 1 and 4 in path_to(ps[1], k))]
+        assert off(got[at:at + n][fine], out[fine].astype(np.float64)) <= 2 * TOL
+        alone.free()
+        at += n
+    assert not np.isfinite(got[44]).all()
+    for s in both:
+        s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("sizes", [[7], [30, 9], [64, 40]])
+def test_unaligned_buffers(models, kind, sizes):
+    """Hidden states and outputs 4 bytes off a 16-byte boundary: the aligned call's outputs; the words
+    around the output stay."""
+    cfg, layer, w = models("kimi")
+    ps = [tree("any", n, 3 + i) for i, n in enumerate(sizes)]
+    states = [State(kind, cfg, 400).load(i, 300 + i) for i in range(len(sizes))]
+    x = hidden(cfg, 0x59, sum(sizes))
+    want = batch_device(kind, cfg, w, states, ps, x, lib.NO_ADVANCE)
+    room = np.full(x.size + 8, 7.25, np.float32)
+    placed = room.copy()
+    placed[1:1 + x.size] = x.ravel()
+    dx, do = Device(placed), Device(room)
+    lib.check(fn("decode_compressed_%stree_batch_device", kind)(do.p + 4, dx.p + 4, ints([len(p) for p in ps]), ints(sum(ps, [])),
+                                                               len(states), C.byref(cfg), C.byref(w), pointers(states),
+                                                               lib.NO_ADVANCE), "tree batch")
+    got = do.get()
+    assert off(got[1:1 + x.size].reshape(x.shape), want.astype(np.float64)) <= 2 * TOL
+    np.testing.assert_array_equal(got[[0, *range(1 + x.size, room.size)]], 7.25)
+    np.testing.assert_array_equal(dx.get(), placed)
+    for b in (dx, do):
+        b.free()
+    for s in states:
+        s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("ctx", [0, 37, 64, 300])
+def test_rows_behind_the_history_do_not_enter(models, kind, ctx):
+    """What a dropped draft left behind the history, not finite here, has no effect."""
+    cfg, layer, w = models("kimi")
+    n = 6
+    x, p = hidden(cfg, 0x5A, n), tree("any", n, 5)
+    st, clean = State(kind, cfg, 400).load(3, 400), State(kind, cfg, 400).load(3, 400)
+    for a in st.arrays():
+        if a.dtype == np.float32:
+            a[ctx:] = np.nan
+        elif a.dtype == np.uint16:
+            a[ctx:] = 0x7FC0
+    lib.check(fn("compressed_%sstate_sync", kind)(st.ref()), "sync")
+    st.upload()
+    for s in (st, clean):
+        lib.check(fn("compressed_%sstate_truncate", kind)(s.ref(), ctx), "truncate")
+    np.testing.assert_array_equal(tree_host(st, layer, x, p, w), tree_host(clean, layer, x, p, w))
+    for s in (st, clean):
+        s.free()
+
+
+def test_q8_scales_of_all_sizes(models):
+    """Q8 rows whose scales run from zero over the smallest numbers to the usual ones: small scales must
+    not push the other rows' weights out of range."""
+    cfg, layer, w = models("kimi")
+    ctx, n = 700, 9
+    st = State("q8", cfg, ctx + n).load(8, ctx)
+    sc = st.arrays()[1]
+    sc[0:100] = 0
+    sc[100:200] = np.float32(1e-40)
+    sc[200:300] = np.float32(1e-30)
+    sc[300:400] *= np.float32(1e-6)
+    sc[650:] *= np.float32(3)
+    lib.check(fn("compressed_%sstate_sync", "q8")(st.ref()), "sync")
+    x, p = hidden(cfg, 0x5B, n), tree("any", n, 6)
+    got = tree_host(st, layer, x, p, w)
+    e = off(got, reference(cfg, layer, x, p, ctx, st.rows(0, ctx + n), "q8"))
+    assert e <= 3 * TOL, e  # three times the logits
+    st.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_long_histories_of_zero_rows(models, kind):
+    """Rows of zeros (Q8: of scale zero too), many to a split: every row has the weight 1."""
+    cfg, layer, w = models("kimi")
+    ctx, n, batch = 40000, 32, 8
+    states = [State(kind, cfg, ctx + n) for _ in range(batch)]
+    states[0].s.len = ctx  # as initialised: zeros
+    for a in states[0].arrays():
+        a[:] = 0
+    lib.check(fn("compressed_%sstate_sync", kind)(states[0].ref()), "sync")
+    lib.check(fn("compressed_%sstate_fork_batch_device", kind)(pointers(states[1:]), pointers(states[:1] * (batch - 1)), ints([0] * (batch - 1)),
+                                                              ints([ctx] * (batch - 1)), batch - 1), "fork")
+    p = tree("any", n, 1)
+    x = hidden(cfg, 0x5C, n)
+    got = batch_device(kind, cfg, w, states, [p] * batch, np.concatenate([x] * batch)).reshape(batch, n, -1)
+    some = [0, n - 1]
+    want = reference(cfg, layer, x, p, ctx, states[-1].pull(0, ctx + n), kind, some)
+    for b in range(batch):
+        e = off(got[b][some], want)
+        assert e <= TOL, (b, e)
+    for s in states:
+        s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("sizes", [[4], [9, 1, 30], [60, 50]])
 def test_layer_form(models, kind, sizes):
     cfg, layer, w = models("kimi")
@@ -284,6 +424,68 @@ def test_captured_tree_replays(models, kind):
     for b in (dx, do):
         b.free()
     for s in states:
+        s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_two_graphs_in_turn(models, kind):
+    """Two captured trees of different sizes, replayed in turn: they share the library's workspaces."""
+    cfg, layer, w = models("kimi")
+    plans = [([8, 3], [700, 20]), ([50, 64], [90, 1200]), ([1], [333])]
+    calls, wants, graphs, keep = [], [], [], []
+    for k, (sizes, lens) in enumerate(plans):
+        ps = [tree("any", n, i + k) for i, n in enumerate(sizes)]
+        states = [State(kind, cfg, m + n).load(i, m) for i, (m, n) in enumerate(zip(lens, sizes))]
+        x = hidden(cfg, 0x7A + k, sum(sizes))
+        wants.append(batch_device(kind, cfg, w, states, ps, x, lib.NO_ADVANCE))
+        dx, do = Device(x), Device(x)
+        keep.append((states, dx, do))
+        calls.append(lambda do=do, dx=dx, sizes=sizes, ps=ps, states=states: fn("decode_compressed_%stree_batch_device", kind)(
+            do.p, dx.p, ints(sizes), ints(sum(ps, [])), len(sizes), C.byref(cfg), C.byref(w), pointers(states), lib.NO_ADVANCE))
+    for call in calls:
+        lib.check(L.kvl_mla_capture_begin(), "capture")
+        rc = call()
+        g = C.c_void_p()
+        lib.check(L.kvl_mla_capture_end(C.byref(g)), "capture end")
+        lib.check(rc, "captured tree")
+        graphs.append(g)
+    for r in range(3):
+        for k, (states, dx, do) in enumerate(keep):
+            do.put(np.zeros(do.shape, np.float32))
+        for g in graphs:
+            lib.check(L.kvl_mla_graph_launch(g), "replay")
+        for k, (states, dx, do) in enumerate(keep):
+            np.testing.assert_array_equal(do.get(), wants[k], err_msg=f"replay {r} of {k}")
+        lib.check(calls[r % 3](), "eager")
+        lib.check(L.kvl_mla_synchronize(), "sync")
+    for g in graphs:
+        L.kvl_mla_graph_destroy(g)
+    for states, dx, do in keep:
+        for s in (*states, dx, do):
+            s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_host_calls_are_refused_in_a_capture(models, kind):
+    cfg, layer, w = models("kimi")
+    a, b = State(kind, cfg, 80).load(1, 40), State(kind, cfg, 80).load(2, 50)
+    x = hidden(cfg, 0x7D, 3)
+    want = tree_host(a, layer, x, [-1, 0, 0], w)
+    lib.check(fn("compressed_%sstate_truncate", kind)(a.ref(), 40), "truncate")
+    out = np.full_like(x, np.nan)
+    lib.check(L.kvl_mla_capture_begin(), "capture")
+    rcs = [fn("decode_compressed_%stree_bf16", kind)(f32p(out), f32p(x), ints([-1, 0, 0]), 3, 40, C.byref(cfg), C.byref(w), a.ref())]
+    whys = [lib.last_error()]
+    for name, args in (("fork", (a.ref(), b.ref(), 0, 50)), ("accept", (b.ref(), 40, ints([1]), 1))):
+        rcs.append(fn("compressed_%sstate_" + name, kind)(*args))
+        whys.append(lib.last_error())
+    g = C.c_void_p()
+    lib.check(L.kvl_mla_capture_end(C.byref(g)), "capture end")
+    L.kvl_mla_graph_destroy(g)
+    assert rcs == [-1] * 3 and all("capture" in y for y in whys), whys
+    assert np.isnan(out).all() and (a.s.len, b.s.len) == (40, 50)
+    np.testing.assert_array_equal(tree_host(a, layer, x, [-1, 0, 0], w), want)
+    for s in (a, b):
         s.free()
 
 
@@ -364,6 +566,31 @@ def test_fork_batch_device(models, kind, dims):
             # behind the copied rows the device still holds the destination's old ones
             np.testing.assert_array_equal(device_array(d, k, r1[i], 390), b[r1[i]:], err_msg=f"{i} {k}")
         own.free()
+    for s in srcs + dsts:
+        s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dims", ["tiny", "lab", "kimi"])
+def test_fork_of_one_range_to_many(models, kind, dims):
+    """Neighbouring pairs of one source and one range are copied together, whatever the range's
+    alignment; a pair of another range or source between them is not."""
+    cfg = models(dims)[0]
+    srcs = [State(kind, cfg, 700).load(i, 600 + i) for i in range(2)]
+    pairs = [(0, 3, 577), (0, 3, 577), (0, 3, 577), (1, 3, 577), (0, 3, 577), (0, 4, 577), (0, 3, 576), (1, 0, 601), (1, 0, 601),
+             (1, 5, 6), (1, 5, 6), (0, 9, 9), (0, 9, 9), (0, 1, 600), (0, 1, 600)]
+    dsts = [State(kind, cfg, 650).load(50 + i, 640).upload() for i in range(len(pairs))]
+    old = [d.rows(0, 640) for d in dsts]
+    lib.check(fn("compressed_%sstate_fork_batch_device", kind)(pointers(dsts), pointers([srcs[k] for k, _, _ in pairs]),
+                                                              ints([lo for _, lo, _ in pairs]), ints([hi for _, _, hi in pairs]),
+                                                              len(pairs)), "fork")
+    for i, (k, lo, hi) in enumerate(pairs):
+        assert dsts[i].s.len == hi
+        for j, (src, was) in enumerate(zip(srcs[k].rows(0, 600), old[i])):
+            now = device_array(dsts[i], j, 0, 640)
+            np.testing.assert_array_equal(now[lo:min(hi, 600)], src[lo:hi], err_msg=f"{i} {j}")
+            np.testing.assert_array_equal(now[:lo], was[:lo], err_msg=f"{i} {j}")
+            np.testing.assert_array_equal(now[hi:], was[hi:], err_msg=f"{i} {j}")
     for s in srcs + dsts:
         s.free()
 

@@ -135,9 +135,9 @@ def rms64(x, w, eps):
     return x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * w
 
 
-def reference(cfg, layer, x, parents, ctx, rows, kind):
+def reference(cfg, layer, x, parents, ctx, rows, kind, nodes=None):
     """out [count, hidden] of a tree decode in 64 bits over `rows`, the state's rows [0, ctx + count)
-    as it stores them (the appended ones among them)."""
+    as it stores them (the appended ones among them); of the given nodes only, if any are given."""
     NH, DN, DR, DV, R = cfg.num_heads, cfg.qk_nope_dim, cfg.qk_rope_dim, cfg.v_head_dim, cfg.kv_lora_rank
     lat, key = values(rows, kind)
     kvb = f64(layer.kv_b_proj).reshape(NH, DN + DV, R)
@@ -145,7 +145,7 @@ def reference(cfg, layer, x, parents, ctx, rows, kind):
     q = (x.astype(np.float64) @ f64(layer.q_proj).T).reshape(-1, NH, DN + DR)
     inv = cfg.rope_theta ** (-2.0 * np.arange(DR // 2) / DR)
     out = []
-    for i in range(len(parents)):
+    for i in range(len(parents)) if nodes is None else nodes:
         p = path_to(parents, i)
         a = (ctx + len(p) - 1) * inv
         e, o = q[i, :, DN::2], q[i, :, DN + 1::2]
