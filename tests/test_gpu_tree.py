@@ -711,8 +711,10 @@ def test_speculative_run_equals_serial_decoding(models, kind, dims):
 
 def test_tree_past_32_bit_offsets(models):
     """An FP32 state whose latent array passes 2^31 bytes: a tree at its end against the block decode of
-    the same chain."""
-    cfg, layer, w = models("kimi")
+    the same chain. A rope_theta of its own: the table of the usual one grows with the positions, and other
+    tests count on positions that it does not reach."""
+    _, layer, w = models("kimi")
+    cfg = inputs.config(**dict(trees.KIMI, rope_theta=30000.0))
     ctx, n = 1_100_000, 6
     st = State("f32", cfg, ctx + n)
     lib.check(L.kvl_mla_compressed_state_fill_synthetic(st.ref(), 0, ctx, 77), "fill")
