@@ -449,13 +449,18 @@ __global__ __launch_bounds__(256) void k_kva_tok(KvaTokArgs a) {
 // waves 0..15). Tiles are numbered row block fastest, then quarter, then token block, and XCD
 // b % 8 takes a contiguous eighth of them, so the row blocks sharing a token block's
 // activations run under one L2.
+// XF: x comes as fp32 (at XH) and is split where its fragments are read, which saves the launch that writes
+// the planes; a token's 128 bytes of a k step (eight slots) take the room of its two planes, slot s stored
+// at s ^ xswz(row), and the two reads of a fragment hit distinct banks too. q_proj | kv_a of trees of 20 /
+// 64 / 170 / 256 nodes (us): k_gemv_ksplit 10.1 / 16.0 / 32 / -, planes and their launch 12.7 / 15.0 / 23.6 /
+// 27, XF 9.4 / 12.0 / 22.0 / 28.
 template <int TU_, int TT_, int WT_, int WR_, int NS_>
 struct KvgShape {
     static constexpr int TU = TU_, TT = TT_, WT = WT_, WR = WR_, NS = NS_;  // NS: ring stages
     static constexpr int BT = 16 * TU * WT, BR = 16 * TT * WR, NT = 64 * WT * WR;
 };
 
-template <class Sh>
+template <class Sh, bool XF>
 __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
     constexpr int TU = Sh::TU, TT = Sh::TT, NS = Sh::NS;
     constexpr int NWV = Sh::WT * Sh::WR, NT = Sh::NT, BT = Sh::BT, BR = Sh::BR;
@@ -472,15 +477,24 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
     const int rb = tile % nrb, kq = (tile / nrb) % kGemvKs, tb = tile / nrb / kGemvKs;
     const int row0 = rb * BR, tok0 = tb * BT;
     auto swz = [](int row) { return (row >> 1) & 3; };
+    auto xswz = [](int row) { return ((row >> 1) & 1) | 6 * ((row >> 3) & 1); };
     // DMA: wave w's instruction i fills slots (i * NWV + w) * 64 .. + 63 of a stage: x hi rows,
     // x lo rows, then W rows, 4 slots each. Rows past the end are clamped (never stored).
     const uint8_t *src[NI];
+    int next[NI];  // bytes from a k step to the next
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
         const int p = min((i * NWV + w) * 64 + l, SLOTS - 1);
-        const int xrow = (p % (BT * 4)) / 4, wrow = (p - 2 * BT * 4) / 4;
+        const int xrow = XF ? p / 8 : (p % (BT * 4)) / 4, wrow = (p - 2 * BT * 4) / 4;
         const uint16_t *rp;
         int s;
+        next[i] = 64;
+        if (XF && p < 2 * BT * 4) {
+            const float *xp = (const float *)a.XH + (size_t)min(tok0 + xrow, a.S - 1) * a.in;
+            src[i] = (const uint8_t *)(xp + kq * 512 + 4 * ((p & 7) ^ xswz(xrow)));
+            next[i] = 128;
+            continue;
+        }
         if (p < 2 * BT * 4) {
             rp = (p < BT * 4 ? a.XH : a.XL) + (size_t)min(tok0 + xrow, a.S - 1) * a.in;
             s = (p & 3) ^ swz(xrow);
@@ -494,13 +508,13 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
         const uint32_t dst = sbase + (j % NS) * STAGE + (uint32_t)w * 1024;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-            if (i < NMIN || (i * NWV + w) * 64 < SLOTS) dma_b128(src[i] + (size_t)j * 64, dst + i * (NWV * 1024));
+            if (i < NMIN || (i * NWV + w) * 64 < SLOTS) dma_b128(src[i] + (XF ? j * next[i] : j * 64), dst + i * (NWV * 1024));
     };
     int fx[TU], fw[TT];  // fragment offsets: row 16 u + n of the wave's tile, logical slot g
 #pragma unroll
     for (int u = 0; u < TU; ++u) {
         const int row = 16 * (TU * wt + u) + n;
-        fx[u] = row * ROWB + 16 * (g ^ swz(row));
+        fx[u] = XF ? row * 2 * ROWB + 16 * ((2 * g) ^ xswz(row)) : row * ROWB + 16 * (g ^ swz(row));
     }
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
@@ -521,8 +535,12 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
         v8bf xh[TU], xl[TU], wv[TT];
 #pragma unroll
         for (int u = 0; u < TU; ++u) {
-            xh[u] = *(const v8bf *)(st + fx[u]);
-            xl[u] = *(const v8bf *)(st + XPL + fx[u]);
+            if constexpr (XF) {
+                split8_cvt(*(const v4f *)(st + fx[u]), *(const v4f *)(st + (fx[u] ^ 16)), xh[u], xl[u]);
+            } else {
+                xh[u] = *(const v8bf *)(st + fx[u]);
+                xl[u] = *(const v8bf *)(st + XPL + fx[u]);
+            }
         }
 #pragma unroll
         for (int t = 0; t < TT; ++t) wv[t] = *(const v8bf *)(st + fw[t]);
@@ -562,43 +580,54 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
     }
 }
 
-template <class Sh>
+template <class Sh, bool XF>
 static hipError_t kva_gemm_launch(hipStream_t st, const KvaTokArgs &a) {
     const size_t tiles = (size_t)((a.out + Sh::BR - 1) / Sh::BR) * kGemvKs * ((a.S + Sh::BT - 1) / Sh::BT);
     if (tiles > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_kva_gemm<Sh>), dim3((unsigned)tiles), dim3(Sh::NT), 0, st, a);
+    hipLaunchKernelGGL((k_kva_gemm<Sh, XF>), dim3((unsigned)tiles), dim3(Sh::NT), 0, st, a);
     return hipGetLastError();
+}
+
+static bool kva_args_ok(const KvaTokArgs &a) {
+    return gemv_ksplit_ok(a.in, a.in) && a.S >= 1 && a.out0 > 0 && a.out >= a.out0 && a.ldy >= a.out &&
+           (a.out == a.out0 || (a.W1 && (uintptr_t)a.W1 % 16 == 0)) && (a.S + 127) / 128 <= 65535 && (uintptr_t)a.XH % 16 == 0 &&
+           (uintptr_t)a.XL % 16 == 0 && (uintptr_t)a.W % 16 == 0 && (uintptr_t)a.Y % 16 == 0 && a.pstride % 4 == 0;
+}
+
+// Small tiles while they do not outnumber the places for them, so that a short prompt spreads
+// over the CUs: first with a ring that holds all 16 k steps (one block per CU; a block then waits
+// for memory about once), then two blocks per CU; large tiles take in fewer bytes per product.
+// us, 32 x 32 and 32 x 64 (16 stages), 32 x 64 (8), 64 x 64, 64 x 96, 128 x 192 (tokens x rows):
+//   37 tokens 5.4 / 6.5 / 6.9 / 9.6 / 11.8 / 17.2   200: 10.3 / 7.2 / 7.4 / 9.9 / - / 19.1
+//   384: 18.5 / 12.5 / 9.2 / 10.3 / - / 19.2        896: 35.7 / 23.9 / 16.5 / 14.3 / - / 20.5
+//   1181: - / - / - / 21.5 / 18.2 / 21.4            16000: - / - / - / - / 171 / 127
+template <bool XF>
+static hipError_t kva_tiles(hipStream_t st, const KvaTokArgs &a) {
+    auto tiles = [&](int bt, int br) { return (long)((a.S + bt - 1) / bt) * kGemvKs * ((a.out + br - 1) / br); };
+    if (tiles(32, 32) <= 256) return kva_gemm_launch<KvgShape<1, 1, 2, 2, 16>, XF>(st, a);
+    if (tiles(32, 64) <= 256) return kva_gemm_launch<KvgShape<1, 2, 2, 2, 16>, XF>(st, a);
+    if (tiles(32, 64) <= 512) return kva_gemm_launch<KvgShape<1, 2, 2, 2, 8>, XF>(st, a);
+    if (tiles(64, 64) <= 512) return kva_gemm_launch<KvgShape<2, 2, 2, 2, 6>, XF>(st, a);
+    if (tiles(64, 96) <= 512) return kva_gemm_launch<KvgShape<2, 3, 2, 2, 4>, XF>(st, a);
+    return kva_gemm_launch<KvgShape<4, 4, 2, 3, 3>, XF>(st, a);
 }
 
 hipError_t launch_kva_tok(hipStream_t st, float *Y, size_t pstride, int ldy, const uint16_t *XH,
                           const uint16_t *XL, int S, const uint16_t *W, int out0, int in, const uint16_t *W1,
                           int out1) {
-    const int out = out0 + out1;
-    if (!gemv_ksplit_ok(in, in) || S < 1 || out0 <= 0 || out1 < 0 || ldy < out || (out1 > 0 && ((uintptr_t)W1 % 16 != 0 || !W1)) || (S + 127) / 128 > 65535 ||
-        ((uintptr_t)XH % 16) != 0 || ((uintptr_t)XL % 16) != 0 || ((uintptr_t)W % 16) != 0 ||
-        ((uintptr_t)Y % 16) != 0 || pstride % 4 != 0)
-        return hipErrorInvalidValue;
-    KvaTokArgs a{Y, XH, XL, W, W1, pstride, ldy, S, out0, out, in};
-    if (in == 2048) {
-        // Small tiles while they do not outnumber the places for them, so that a short prompt spreads
-        // over the CUs: first with a ring that holds all 16 k steps (one block per CU; a block then waits
-        // for memory about once), then two blocks per CU; large tiles take in fewer bytes per product.
-        // us, 32 x 32 and 32 x 64 (16 stages), 32 x 64 (8), 64 x 64, 64 x 96, 128 x 192 (tokens x rows):
-        //   37 tokens 5.4 / 6.5 / 6.9 / 9.6 / 11.8 / 17.2   200: 10.3 / 7.2 / 7.4 / 9.9 / - / 19.1
-        //   384: 18.5 / 12.5 / 9.2 / 10.3 / - / 19.2        896: 35.7 / 23.9 / 16.5 / 14.3 / - / 20.5
-        //   1181: - / - / - / 21.5 / 18.2 / 21.4            16000: - / - / - / - / 171 / 127
-        auto tiles = [&](int bt, int br) { return (long)((S + bt - 1) / bt) * kGemvKs * ((out + br - 1) / br); };
-        if (tiles(32, 32) <= 256) return kva_gemm_launch<KvgShape<1, 1, 2, 2, 16>>(st, a);
-        if (tiles(32, 64) <= 256) return kva_gemm_launch<KvgShape<1, 2, 2, 2, 16>>(st, a);
-        if (tiles(32, 64) <= 512) return kva_gemm_launch<KvgShape<1, 2, 2, 2, 8>>(st, a);
-        if (tiles(64, 64) <= 512) return kva_gemm_launch<KvgShape<2, 2, 2, 2, 6>>(st, a);
-        if (tiles(64, 96) <= 512) return kva_gemm_launch<KvgShape<2, 3, 2, 2, 4>>(st, a);
-        return kva_gemm_launch<KvgShape<4, 4, 2, 3, 3>>(st, a);
-    } else {
-        const dim3 grid((out + 63) / 64, kGemvKs, (S + 127) / 128);
-        hipLaunchKernelGGL((k_kva_tok<2>), grid, dim3(256), 0, st, a);
-    }
+    const KvaTokArgs a{Y, XH, XL, W, W1, pstride, ldy, S, out0, out0 + out1, in};
+    if (!kva_args_ok(a)) return hipErrorInvalidValue;
+    if (in == 2048) return kva_tiles<false>(st, a);
+    const dim3 grid((a.out + 63) / 64, kGemvKs, (S + 127) / 128);
+    hipLaunchKernelGGL((k_kva_tok<2>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
+}
+
+hipError_t launch_kva_x(hipStream_t st, float *Y, size_t pstride, int ldy, const float *X, int S, const uint16_t *W, int out0,
+                        const uint16_t *W1, int out1) {
+    const KvaTokArgs a{Y, (const uint16_t *)X, nullptr, W, W1, pstride, ldy, S, out0, out0 + out1, 2048};
+    if (!kva_args_ok(a)) return hipErrorInvalidValue;
+    return kva_tiles<true>(st, a);
 }
 
 bool gemv_xs_ok(int in) { return in == 2048 || in == 4096; }

@@ -100,6 +100,9 @@ hipError_t launch_gemv_ksplit(hipStream_t st, float *Y, size_t pstride, int ldy,
 hipError_t launch_kva_tok(hipStream_t st, float *Y, size_t pstride, int ldy, const uint16_t *XH,
                           const uint16_t *XL, int S, const uint16_t *W, int out0, int in,
                           const uint16_t *W1 = nullptr, int out1 = 0);
+// The same from fp32 X [S, 2048], W rows of 2048 (finite x: the planes' partials bit for bit).
+hipError_t launch_kva_x(hipStream_t st, float *Y, size_t pstride, int ldy, const float *X, int S, const uint16_t *W, int out0,
+                        const uint16_t *W1, int out1);
 // Y[b, o] (+)= sum_k W[o, k] x[b, k] with x given as bf16 planes XS[2][B][in] (hi, lo), as
 // launch_combine writes them (DecodeWork::hos). Shapes when gemv_xs_ok (in = 2048 or 4096),
 // any B.

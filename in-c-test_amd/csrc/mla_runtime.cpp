@@ -1934,8 +1934,10 @@ size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &t
     return (size_t)plan_tree(fmt, d, tt, ctx().ncu) * d.NH * (d.R + 2) * sizeof(float);
 }
 
-// Nodes from which on a group's projections are products over LDS tiles instead of the decode's GEMVs.
-constexpr int kTreeGemm = 64;
+// Nodes beyond which a group's q_proj | kv_a and o_proj are products over LDS tiles instead of the decode's GEMVs
+// (in groups of 16 tokens). us, GEMV / tiles: q_proj | kv_a at 12 nodes 7.9 / 9.4, 20 10.1 / 9.4, 64 16.0 / 12.0;
+// o_proj at 64 nodes 11.8 / 6.5 + 5 (the sum of its quarters), 170 29.6 / 14.4 + 5.
+constexpr int kTreeGemmX = 16, kTreeGemm = 64;
 
 // One tree decode of a launch group: the steps of decode_group with the group's nodes as its
 // members, each member's row at history row ctx + i and its rotation at position ctx + depth.
@@ -1957,9 +1959,6 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         HIP_TRY(launch_rmsnorm(st, in_norm->buf, d_x, in_norm->w, d.H, N, eps));
         d_x = in_norm->buf;
     }
-    // The projections of many nodes as products over LDS tiles, the same partials bit for bit (launch_kva_tok);
-    // the planes of x take the place of kv, which only the expanded format uses.
-    const bool many = N > kTreeGemm && gemv_ksplit_ok(d.H, d.H) && d.KVB >= d.H;
     if (gemv_ksplit_ok(d.H, d.H)) {
         if (((uintptr_t)d_x % 16) != 0) {  // the kernels read 16-byte vectors
             HIP_TRY(hipMemcpyAsync(w.x, d_x, (size_t)N * d.H * sizeof(float), hipMemcpyDeviceToDevice, st));
@@ -1967,13 +1966,9 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         }
         w.ynp = kGemvKs;
         w.ypstride = (size_t)N * ldy;
-        if (many) {
-            uint16_t *xh = (uint16_t *)w.kv, *xl = xh + (size_t)N * d.H;
-            HIP_TRY(launch_split(st, d_x, d.H, xh, xl, d.H, N, d.H));
-            HIP_TRY(launch_kva_tok(st, w.y, w.ypstride, ldy, xh, xl, N, dw.q, d.QO, d.H, dw.kva, d.KVO));
-        } else {
-            HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
-        }
+        // the same partials bit for bit, as products over LDS tiles
+        if (N > kTreeGemmX && d.H == 2048) HIP_TRY(launch_kva_x(st, w.y, w.ypstride, ldy, d_x, N, dw.q, d.QO, dw.kva, d.KVO));
+        else HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
     } else {
         w.ynp = 1;
         w.ypstride = 0;
@@ -2021,7 +2016,7 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
     if (tt.nm) {
         HIP_TRY(launch_tree_history(st, fmt, tt, d, w));
         HIP_TRY(launch_tree_combine(st, fmt, tt, nd, d, dw.kvb, w));
-        if (many && d.H <= ldy && d.H % 4 == 0 && (uintptr_t)d_out % 16 == 0) {  // partials in the place of w.y
+        if (N > kTreeGemm && gemv_ksplit_ok(d.H, d.H) && d.H <= ldy && d.H % 4 == 0 && (uintptr_t)d_out % 16 == 0) {  // partials in the place of w.y
             const size_t ps = (size_t)N * d.H;
             HIP_TRY(launch_kva_tok(st, w.y, ps, d.H, w.hos, w.hos + (size_t)N * d.HO, N, dw.o, d.H, d.HO));
             HIP_TRY(launch_tree_sum(st, d_out, w.y, ps, ps, residual));
