@@ -1973,7 +1973,6 @@ constexpr int kF32Ch = 16;
 constexpr int kF32Ring = 2;
 constexpr int kF32SpOff = kF32Ring * kB16Slot;
 constexpr int kF32SmemB = kF32SpOff + 2 * 16 * kB16SpHs * 4;
-typedef int v2i __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ int f32r_swz(int row) { return (row >> 1) & 7; }
 
 template <bool ONCE>  // ONCE: each history row is read by one workgroup (non-temporal loads)
@@ -2632,11 +2631,6 @@ __device__ __forceinline__ void row16_max4(float &a, float &b, float &c, float &
         : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
 }
 
-// ds_read_b64_tr_b8: within each 16-lane group, destination lane j byte i comes from the
-// 8 bytes addressed by source lane 2i + (j >> 3), at byte j & 7.
-__device__ __forceinline__ v2i lds_read_tr8(const uint8_t *p) {
-    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i *)(p));
-}
 
 // The three-level quantised weights of this lane's row (rowl) for heads 4g .. 4g+3:
 // v = p * s * wscale in [0, 127] ~= hi + lo/254 + lo2/254^2.

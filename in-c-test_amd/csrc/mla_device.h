@@ -314,6 +314,13 @@ __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(
 // (r3, r1, r0) -> distinct slot pairs for the 8 rows of a transposed half-wave read
 __device__ __forceinline__ int b16_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8); }
 
+typedef int v2i __attribute__((ext_vector_type(2)));
+// ds_read_b64_tr_b8: within each 16-lane group, destination lane j byte i comes from the
+// 8 bytes addressed by source lane 2i + (j >> 3), at byte j & 7.
+__device__ __forceinline__ v2i lds_read_tr8(const uint8_t *p) {
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) v2i *)(p));
+}
+
 typedef short v4s __attribute__((ext_vector_type(4)));
 // ds_read_b64_tr_b16: within each 16-lane group, destination lane i element e is element i & 3
 // of the four addressed by source lane 4e + (i >> 2).

@@ -141,18 +141,21 @@ struct ThShape {
     static constexpr int NW = 2 * NM, NT = 64 * NW, NQ = 16 * NM;
     static constexpr int NP = FMT == kFmtF32 ? 2 : 1;  // planes of a row
     static constexpr int Ch = kThCh / NP;              // rows of a chunk
-    static constexpr int LatB = Ch * 1024, KeyB = Ch * 128, PlaneB = LatB + KeyB;
-    static constexpr int ScB = FMT == kFmtQ8 ? 2 * Ch * 4 : 0;  // scales, their logarithms
+    static constexpr bool Dma = FMT == kFmtQ8;         // rows go to LDS as they are stored
+    static constexpr int RowB = FMT == kFmtQ8 ? 512 : 1024;
+    static constexpr int LatB = Ch * RowB, KeyB = Ch * 128, PlaneB = LatB + KeyB;
+    static constexpr int ScB = FMT == kFmtQ8 ? Ch * 4 : 0;  // scales
     static constexpr int Slot = NP * PlaneB + ScB;
-    static constexpr int Ring = NM < 4 ? 1 : 3;
-    static constexpr bool Pipe = Ring == 3;
+    static constexpr bool Pipe = NM == 4;
+    static constexpr int Ring = Pipe ? (Dma ? 5 : 3) : (Dma ? 2 : 1);
     static constexpr int SpOff = Ring * Slot;
     static constexpr int SpH = NQ * 36;  // floats of a half of the scores (th_sp)
     static constexpr int SpB = 2 * SpH * 4;
     static constexpr int PwOff = SpOff + (Pipe ? 2 : 1) * SpB;
     static constexpr int PwB = NQ * 64;  // bytes of a plane of weights (th_pw)
-    static constexpr int AlOff = PwOff + 2 * PwB;
-    static constexpr int FlOff = AlOff + NQ * 4;
+    static constexpr int PwN = Pipe && Dma ? 2 : 1;  // buffers of weights
+    static constexpr int AlOff = PwOff + PwN * 2 * PwB;
+    static constexpr int FlOff = AlOff + PwN * NQ * 4;
     static constexpr int Smem = FlOff + 2 * 8 * 4;
     static_assert(Smem <= 160 * 1024, "LDS of one CU");
 };
@@ -209,7 +212,6 @@ __device__ __forceinline__ bool tree_unit(const TreeTable &t, TreeUnit &u) {
     return true;
 }
 
-typedef int v2i __attribute__((ext_vector_type(2)));
 
 template <int FMT>
 __device__ __forceinline__ v4f th_mfma(const v4i &a, const v4i &b, const v4f &c) {
@@ -284,39 +286,51 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     const int nch = (r1 - r0 + Ch - 1) / Ch;
     const int first = tile * NM, live = min(NM, s.count - first);  // nodes of this tile
 
-    // ---- staging: a chunk's rows from memory to registers, and from there to an LDS slot. A thread
+    // ---- Q8: a chunk's rows from memory to an LDS slot, asynchronously. One instruction of a wave takes 1 KB,
+    // two rows of codes; the wave's keys and scales are one instruction each. Rows past the split repeat its
+    // last one (their scores are masked).
+    constexpr int KR = Ch / NW, NA = kQ8 ? Ch / 2 / NW : 0, ND = NA + 2;  // a wave's key rows; instructions
+    auto issue = [&](int c, int slot) __attribute__((always_inline)) {
+        if constexpr (kQ8) {
+            const int last = r1 - r0 - 1;
+            const uint32_t to = lds_addr(smem) + slot * Sh::Slot;
+            const int lr = 2 * w + (l >> 5), sw = 16 * ((l & 31) ^ (lr & 15));
+#pragma unroll
+            for (int i = 0; i < NA; ++i)  // row lr + 2 NW i
+                dma_b128_s(s.a + (size_t)r0 * 512, (uint32_t)(min(c * Ch + lr + 2 * NW * i, last) * 512 + (sw ^ (16 * ((2 * NW * i) & 15)))),
+                           to + (NW * i + w) * 1024);
+            const int kr = KR * w + (l >> 3);
+            if (l < 8 * KR)
+                dma_b128_s(s.c + (size_t)r0 * 128, (uint32_t)(min(c * Ch + kr, last) * 128 + 16 * ((l & 7) ^ ((kr >> 1) & 7))),
+                           to + Sh::LatB + 128 * KR * w);
+            if (l < KR) dma_b32(s.b + 4 * ((size_t)r0 + min(c * Ch + KR * w + l, last)), to + Sh::PlaneB + 4 * KR * w);
+        }
+    };
+    // ---- BF16, FP32: from memory to registers, and from there to an LDS slot. A thread
     // takes eight values of a latent row (word tid % 64 of rows tid / 64 + NW i) and eight bytes of a key row
     // (tid % 16 of rows tid / 16 + NT / 16 i; FP32: tid % 32 of rows tid / 32).
     constexpr int NL = Ch / NW, NK = 512 / NT;
-    constexpr int LE = kQ8 ? 1 : FMT == kFmtF32 ? 4 : 2, KE = FMT == kFmtF32 ? 4 : 2;  // bytes of an element
+    constexpr int LE = FMT == kFmtF32 ? 4 : 2, KE = LE;  // bytes of an element
     constexpr int LV = LE == 4 ? 2 : 1;
     struct Held {
-        v4i la[kQ8 ? 1 : NL * LV];
-        v2i lc[kQ8 ? NL : 1], kb[NK];
-        float rsc;
+        v4i la[NL * LV];
+        v2i kb[NK];
     };
     const int lrow = tid >> 6;
     // the split's rows as buffers: a read past the last row gives zeros (its score is masked)
     const int nrow = r1 - r0;
     const auto ba = __builtin_amdgcn_make_buffer_rsrc(s.a + (size_t)r0 * (512 * LE), 0, nrow * (512 * LE), 0x00027000);
-    const auto bk = __builtin_amdgcn_make_buffer_rsrc((kQ8 ? s.c : s.b) + (size_t)r0 * (64 * KE), 0, nrow * (64 * KE), 0x00027000);
-    const auto bs = __builtin_amdgcn_make_buffer_rsrc(s.b + (size_t)r0 * 4, 0, kQ8 ? nrow * 4 : 0, 0x00027000);
+    const auto bk = __builtin_amdgcn_make_buffer_rsrc(s.b + (size_t)r0 * (64 * KE), 0, nrow * (64 * KE), 0x00027000);
     const int va = tid * (8 * LE), vk = tid * 8;  // rows lie one after another, so do the threads' words
     auto fetch = [&](int c, Held &f) __attribute__((always_inline)) {
         const int oa = va + c * (Ch * 512 * LE), ok = vk + c * (Ch * 64 * KE);
 #pragma unroll
-        for (int i = 0; i < NL; ++i) {
-            if constexpr (kQ8)
-                f.lc[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(ba, oa + i * (NT * 8 * LE), 0, 0));
-            else
+        for (int i = 0; i < NL; ++i)
 #pragma unroll
-                for (int v = 0; v < LV; ++v)
-                    f.la[LV * i + v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ba, oa + i * (NT * 8 * LE) + 16 * v, 0, 0));
-        }
+            for (int v = 0; v < LV; ++v)
+                f.la[LV * i + v] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(ba, oa + i * (NT * 8 * LE) + 16 * v, 0, 0));
 #pragma unroll
         for (int i = 0; i < NK; ++i) f.kb[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(bk, ok + i * (NT * 8), 0, 0));
-        if constexpr (kQ8)
-            f.rsc = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(bs, 4 * (c * Ch + (tid & 31)), 0, 0));
     };
     auto put = [&](uint8_t *at, const v4i *v) __attribute__((always_inline)) {
         if constexpr (NP == 2) {
@@ -330,13 +344,12 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
     const int sa = lrow * 1024 + 16 * (l ^ th_swz(lrow));
     const int sk = Sh::LatB + (KE == 4 ? th_key(tid >> 5, (tid >> 2) & 7) + 4 * (tid & 3) : th_key(tid >> 4, (tid >> 1) & 7) + 8 * (tid & 1));
-    // piece i < NL: a latent item; the last piece: the key items and the scales
+    // piece i < NL: a latent item; the last piece: the key items
     auto stage = [&](uint8_t *buf, const Held &f, int i) __attribute__((always_inline)) {
         if (i < NL) {
             // row lrow + NW i: th_swz changes by the bits of NW i below 16
             uint8_t *at = buf + (sa ^ (16 * th_swz((NW * i) & 15))) + NW * i * 1024;
-            if constexpr (kQ8) *(v4i *)at = codes_f16(f.lc[i]);
-            else put(at, f.la + LV * i);
+            put(at, f.la + LV * i);
             return;
         }
 #pragma unroll
@@ -352,13 +365,6 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 *(v2i *)(buf + sk + q * (NT / 16) * 128) = f.kb[q];
             }
         }
-        if constexpr (kQ8) {
-            if (tid < Ch) {
-                float *sc = (float *)(buf + NP * Sh::PlaneB);
-                sc[tid] = f.rsc;
-                sc[Ch + tid] = __builtin_amdgcn_logf(fmaxf(fabsf(f.rsc), 1e-28f));
-            }
-        }
     };
     auto stage_all = [&](uint8_t *buf, const Held &f) __attribute__((always_inline)) {
 #pragma unroll
@@ -366,24 +372,30 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
 
     Held held, ahead;  // the first two chunks are requested together
-    fetch(0, ahead);
-    fetch(1, held);
+    if constexpr (Sh::Dma) {
+        issue(0, 0);
+    } else {
+        fetch(0, ahead);
+        fetch(1, held);
+    }
     // ---- queries: A operand of the scores, head n of node m: columns 32 kb + 8 g .. of the eight
-    // latent blocks kb = 8 kh + j and of the key block kh (j = 8). Scores are in units of log2.
+    // latent blocks kb = 8 kh + j and of the key block kh (the last). Q8: columns 64 kb + 16 g .. of the four blocks
+    // kb = 4 kh + j as whole numbers below 2^22 in three signed bytes, qp[3 j] the high one. Scores are in
+    // units of log2.
     const int m = w % NM, kh = w / NM;
-    v4i qh[9], ql[9];
+    constexpr int NQK = kQ8 ? 1 : 9;
+    v4i qh[NQK], ql[NQK], qp[kQ8 ? 12 : 1];
     float qd[4] = {1.f, 1.f, 1.f, 1.f};  // Q8: undoes the query's power of two, heads 4 g + i
     {
-        const float *qrow = a.qf + ((size_t)(s.node0 + first + min(m, live - 1)) * 16 + n) * 576 + 8 * g;
+        const float *qrow = a.qf + ((size_t)(s.node0 + first + min(m, live - 1)) * 16 + n) * 576;
         const float unit = a.smscale * 1.44269504f;
         v4f qv[18];
 #pragma unroll
         for (int j = 0; j < 9; ++j) {
-            const float *p = qrow + (j < 8 ? 32 * (8 * kh + j) : 512 + 32 * kh);
+            const float *p = qrow + (j == 8 ? 512 + 32 * kh + 8 * g : kQ8 ? 256 * kh + 64 * (j >> 1) + 16 * g + 8 * (j & 1) : 32 * (8 * kh + j) + 8 * g);
             qv[2 * j] = *(const v4f *)p * unit;
             qv[2 * j + 1] = *(const v4f *)(p + 4) * unit;
         }
-        float qs = 1.0f;
         if constexpr (kQ8) {
             float mx = 0.f;
 #pragma unroll
@@ -392,28 +404,51 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(qv[j][e]));
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            // 2^(10 - e) with 2^(e - 1) <= mx < 2^e, from the exponent's bits, kept within 2^+-100 (zero and
-            // values that are not finite among them)
-            const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255) - 126, -90), 100);
-            qs = __uint_as_float((uint32_t)(137 - e) << 23);
-            const float qi = __uint_as_float((uint32_t)(117 + e) << 23);
+            // 2^(22 - e) with 2^(e - 1) <= mx < 2^e, from the exponent's bits, kept within 2^+-104 (zero and values
+            // that are not finite among them: such a node's own row, which it attends, makes its output NaN)
+            const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255) - 126, -82), 100);
+            const float qs = __uint_as_float((uint32_t)(149 - e) << 23);
+            const float qi = __uint_as_float((uint32_t)(105 + e) << 23);
 #pragma unroll
             for (int i = 0; i < 4; ++i) qd[i] = __shfl(qi, 4 * g + i);
-        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) th_split<kQ8>(qv[2 * j] * qs, qv[2 * j + 1] * qs, qh[j], ql[j]);
-        th_split<false>(qv[16], qv[17], qh[8], ql[8]);
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    uint32_t b0 = 0, b1 = 0, b2 = 0;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const int v = (int)rintf(__builtin_amdgcn_fmed3f(qv[4 * j + z][y] * qs, -4194304.f, 4194304.f)), v1 = (v + 128) >> 8, v0 = (v1 + 128) >> 8;  // v - 256 v1, v1 - 256 v0: a byte
+                        b0 |= (uint32_t)(v0 & 255) << (8 * y);
+                        b1 |= (uint32_t)(v1 & 255) << (8 * y);
+                        b2 |= (uint32_t)(v & 255) << (8 * y);
+                    }
+                    qp[3 * j][z] = (int)b0;
+                    qp[3 * j + 1][z] = (int)b1;
+                    qp[3 * j + 2][z] = (int)b2;
+                }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) th_split<false>(qv[2 * j], qv[2 * j + 1], qh[j], ql[j]);
+        }
+        th_split<false>(qv[16], qv[17], qh[NQK - 1], ql[NQK - 1]);
     }
-    stage_all(smem, ahead);
+    if constexpr (!Sh::Dma) stage_all(smem, ahead);
 
-    // score operands: row n of a 16-row half (16 KB / 2 KB apart), block j at bofs[j % 4] + 256 (j / 4)
+    // score operands: row n of a 16-row half, block j at bofs[j % 4] + 256 (j / 4) (Q8: bofs[j])
     int bofs[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) bofs[j] = n * 1024 + 16 * ((4 * (8 * kh + j) + g) ^ th_swz(n));
+    for (int j = 0; j < 4; ++j)
+        bofs[j] = n * Sh::RowB + 16 * (kQ8 ? (4 * (4 * kh + j) + g) ^ n : (4 * (8 * kh + j) + g) ^ th_swz(n));
     const int kofs = Sh::LatB + th_key(n, 4 * kh + g);
     // transposed reads of column block NC w + t (lds_read_tr16): rows 8 g + 4 h + (n >> 2); of the FP32 planes
     // the 16 hi rows for g = 0, 1 and the 16 lo rows for g = 2, 3
+    // Q8 (lds_read_tr8): rows 8 g + (n >> 1), 16 columns a word, read t at tro[0][0] ^ 16 t.
     int tro[2][NC];
+    if constexpr (kQ8) {
+        const int row = 8 * g + (n >> 1);
+        tro[0][0] = row * 512 + 16 * ((NC * w) ^ (row & 15)) + 8 * (n & 1);
+    } else
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int row = 8 * (NP == 2 ? g & 1 : g) + 4 * h + (n >> 2);
@@ -435,7 +470,55 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     // to itself the compiler reads each operand right before its use and waits for LDS every time.
     const int spw = Sh::SpOff + 4 * (kh * Sh::SpH + th_sp(16 * m + 4 * g) + n), spr = Sh::SpOff + 4 * (th_sp(sq) + sr);
     // between(i): other work after read i's products
+    auto scores_q8 = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
+        float *sp = (float *)(smem + spw + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
+        // read i: block i / RB of rows 16 (i % RB); the last RB reads: the keys
+        constexpr int N = 5 * RB, W = 6;
+        auto get = [&](int i) __attribute__((always_inline)) {
+            const int j = i / RB, rb = i % RB;
+            return *(const v4i *)(buf + (j < 4 ? bofs[j] + 8192 * rb : kofs + 2048 * rb));
+        };
+        v4i d[3][RB], bv[W];  // by the bytes of the query
+        v4f dk[RB];
+        float x[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            dk[rb] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int z = 0; z < 3; ++z) d[z][rb] = v4i{0, 0, 0, 0};
+            x[rb] = *(const float *)(buf + Sh::PlaneB + 4 * (16 * rb + n));
+        }
+#pragma unroll
+        for (int i = 0; i < W; ++i) bv[i] = get(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int j = i / RB, rb = i % RB;
+            const v4i v = bv[i % W];
+            if (j < 4) {
+#pragma unroll
+                for (int z = 0; z < 3; ++z) d[z][rb] = mfma_i8(qp[kQ8 ? 3 * j + z : 0], v, d[z][rb]);
+            } else {
+                dk[rb] = th_mfma<kFmtBF16>(qh[0], v, dk[rb]);
+                dk[rb] = th_mfma<kFmtBF16>(ql[0], v, dk[rb]);
+            }
+            if (i + W < N) bv[i % W] = get(i + W);
+            between(i);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float v = fmaf((float)d[0][rb][i], 65536.f, fmaf((float)d[1][rb][i], 256.f, (float)d[2][rb][i]));
+                sp[32 * i + 16 * rb] = fmaf(v, qd[i] * x[rb], dk[rb][i]);
+            }
+    };
     auto scores = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
+        if constexpr (kQ8) {
+            scores_q8(buf, c, between);
+            return;
+        }
         float *sp = (float *)(smem + spw + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
         // read i: plane i % NP of rows 16 (i / NP % RB) of block i / NP / RB
         constexpr int N = 9 * NP * RB, W = 6;
@@ -444,31 +527,24 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             return *(const v4i *)(buf + (i % NP) * Sh::PlaneB + (j < 8 ? bofs[j & 3] + 256 * (j >> 2) + 16384 * rb : kofs + 2048 * rb));
         };
         // sums: d over the latents by rows (FP32: by hi . hi and lo . hi), dk over the key (FP32: hi . lo)
-        v4f d[2], dk[2];
+        v4f d[2], dk;
         v4i bv[W];
-        float x[RB];
 #pragma unroll
-        for (int z = 0; z < 2; ++z) d[z] = dk[z] = v4f{0.f, 0.f, 0.f, 0.f};
-        if constexpr (kQ8)
-#pragma unroll
-            for (int rb = 0; rb < RB; ++rb) x[rb] = *(const float *)(buf + NP * Sh::PlaneB + 4 * (16 * rb + n));
+        for (int z = 0; z < 2; ++z) d[z] = dk = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < W; ++i) bv[i] = get(i);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int j = i / (NP * RB), rb = i / NP % RB;
+            const int j = i / (NP * RB) % NQK, rb = i / NP % RB;
             const v4i v = bv[i % W];
             if constexpr (NP == 2) {  // not lo . lo
                 if (i % 2 == 0) {
                     d[0] = th_mfma<FMT>(qh[j], v, d[0]);
                     d[1] = th_mfma<FMT>(ql[j], v, d[1]);
                 } else {
-                    dk[0] = th_mfma<FMT>(qh[j], v, dk[0]);
+                    dk = th_mfma<FMT>(qh[j], v, dk);
                 }
-            } else if (kQ8 && j == 8) {
-                dk[rb] = th_mfma<kFmtBF16>(qh[j], v, dk[rb]);
-                dk[rb] = th_mfma<kFmtBF16>(ql[j], v, dk[rb]);
             } else {
                 d[rb] = th_mfma<FMT>(qh[j], v, d[rb]);
                 d[rb] = th_mfma<FMT>(ql[j], v, d[rb]);
@@ -477,29 +553,21 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             between(i);
             __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (NP == 2) d[0] += d[1] + dk[0];
+        if constexpr (NP == 2) d[0] += d[1] + dk;
 #pragma unroll
-        for (int rb = 0; rb < RB; ++rb) {
-            if constexpr (kQ8)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) d[rb][i] = fmaf(d[rb][i], qd[i] * x[rb], dk[rb][i]);
+        for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
             for (int i = 0; i < 4; ++i) sp[32 * i + 16 * rb] = d[rb][i];
-        }
     };
     // softmax of a chunk: its reads, then its arithmetic and writes in five pieces
     typedef float vsr __attribute__((ext_vector_type(SR)));
-    vsr sx, st, sr4, sp4;
+    vsr sx, sr4, sp4;
     float cm, alpha;
     bool moved;
     auto softmax_read = [&](const uint8_t *buf, int c) __attribute__((always_inline)) {
-        const float *scl = (const float *)(buf + NP * Sh::PlaneB);
         const float *sp = (const float *)(smem + spr + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
         const vsr s0 = *(const vsr *)sp, s1 = *(const vsr *)(sp + Sh::SpH);
-        if constexpr (kQ8) {
-            sr4 = *(const vsr *)(scl + sr);
-            st = *(const vsr *)(scl + Ch + sr);
-        }
+        if constexpr (kQ8) sr4 = *(const vsr *)(buf + Sh::PlaneB + 4 * sr);
         sx = s0 + s1;
     };
     auto softmax = [&](int c, int piece) __attribute__((always_inline)) {
@@ -509,7 +577,9 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
 #pragma unroll
             for (int e = 0; e < SR; ++e) sx[e] = e < nv ? sx[e] : -INFINITY;
             vsr t = sx;
-            if constexpr (kQ8) t += st;
+            if constexpr (kQ8)
+#pragma unroll
+                for (int e = 0; e < SR; ++e) t[e] += __builtin_amdgcn_logf(fmaxf(fabsf(sr4[e]), 1e-28f));
             cm = fmaxf(t[0], t[1]);
             if constexpr (SR == 4) cm = fmaxf(cm, fmaxf(t[2], t[3]));
             cm = fmaxf(cm, dpp_f32<0xB1>(cm));
@@ -533,7 +603,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             if constexpr (SR == 4) {
                 int2 hi, lo;
                 th_split4<kQ8>(sp4, hi, lo);
-                uint8_t *pw = smem + Sh::PwOff + th_pw(sq, sr >> 3) + 2 * (sr & 4);
+                uint8_t *pw = smem + Sh::PwOff + (Sh::PwN == 2 ? (c & 1) * 2 * Sh::PwB : 0) + th_pw(sq, sr >> 3) + 2 * (sr & 4);
                 *(int2 *)pw = hi;
                 *(int2 *)(pw + Sh::PwB) = lo;
             } else {  // the hi weights in words 0, 1, the lo weights in words 2, 3
@@ -542,17 +612,21 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 *(int *)(smem + Sh::PwOff + th_pw(sq, sr >> 3) + 2 * (sr & 7)) = __builtin_bit_cast(int, hi);
                 *(int *)(smem + Sh::PwOff + th_pw(sq, 2 + (sr >> 3)) + 2 * (sr & 7)) = __builtin_bit_cast(int, lo);
             }
-            if ((tid & 7) == 0) *(float *)(smem + Sh::AlOff + 4 * sq) = alpha;
+            if ((tid & 7) == 0) *(float *)(smem + Sh::AlOff + (Sh::PwN == 2 ? (c & 1) * 4 * Sh::NQ : 0) + 4 * sq) = alpha;
             if (l == 0) *(int *)(smem + Sh::FlOff + 32 * (c & 1) + 4 * w) = moved ? 1 : 0;
         }
     };
     auto mix = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
         // FP32: an operand holds 16 rows twice, for the hi and for the lo plane: ph . (hi | lo) + pl . (hi | lo)
         v4i f[NW / 4], ph[NM], pl[NM], bt[2];
+        v2i raw;  // Q8: the codes of the read after next
 #pragma unroll
         for (int i = 0; i < NW / 4; ++i) f[i] = *(const v4i *)(smem + Sh::FlOff + 32 * (c & 1) + 16 * i);
         auto get = [&](int t) __attribute__((always_inline)) {
-            bt[t & 1] = __builtin_bit_cast(
+            if constexpr (kQ8)
+                raw = lds_read_tr8(buf + (tro[0][0] ^ (16 * t)));
+            else
+                bt[t & 1] = __builtin_bit_cast(
                 v4i, __builtin_shufflevector(lds_read_tr16(buf + tro[0][t]), lds_read_tr16(buf + tro[1][t]), 0, 1, 2, 3, 4, 5, 6, 7));
         };
 #pragma unroll
@@ -561,6 +635,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             if (i == 0) get(0);
             pl[i] = *(const v4i *)(smem + Sh::PwOff + (NP == 2 ? th_pw(16 * i + n, 2 + (g & 1)) : Sh::PwB + th_pw(16 * i + n, g)));
         }
+        if constexpr (kQ8) bt[0] = codes_f16(raw);
         get(1);
         int any = 0;
 #pragma unroll
@@ -580,13 +655,122 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(ph[i], bt[t & 1], acc[i][t]);
 #pragma unroll
             for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(pl[i], bt[t & 1], acc[i][t]);
+            if constexpr (kQ8) bt[(t + 1) & 1] = codes_f16(raw);
             if (t + 2 < NC) get(t + 2);
             between(t);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
 
-    if constexpr (Sh::Pipe) {
+    // A pass of the Q8 pipe: scores of chunk c + 2, softmax of chunk c + 1, mix of chunk c. None needs another's
+    // results, so a pass is one stream of products with the rest laid between them, and one barrier.
+    auto pass = [&](int c, const uint8_t *b0, const uint8_t *b1, const uint8_t *b2) __attribute__((always_inline)) {
+        constexpr int N = 5 * RB, W = 6;  // as scores_q8
+        float *sp = (float *)(smem + spw + (c & 1) * Sh::SpB);
+        const uint8_t *pw = smem + Sh::PwOff + (c & 1) * 2 * Sh::PwB;
+        auto get = [&](int i) __attribute__((always_inline)) {
+            const int j = i / RB, rb = i % RB;
+            return *(const v4i *)(b2 + (j < 4 ? bofs[j] + 8192 * rb : kofs + 2048 * rb));
+        };
+        auto codes = [&](int t) __attribute__((always_inline)) { return lds_read_tr8(b0 + (tro[0][0] ^ (16 * t))); };
+        v4i d[3][RB], bv[W], f[NW / 4], ph[NM], pl[NM], bt[2];
+        v4f dk[RB];
+        v2i raw[2];
+        float x[RB];
+#pragma unroll
+        for (int i = 0; i < W; ++i) bv[i] = get(i);
+        softmax_read(b1, c + 1);
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            dk[rb] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int z = 0; z < 3; ++z) d[z][rb] = v4i{0, 0, 0, 0};
+            x[rb] = *(const float *)(b2 + Sh::PlaneB + 4 * (16 * rb + n));
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int j = i / RB, rb = i % RB;
+            const v4i v = bv[i % W];
+            if (j < 4) {
+#pragma unroll
+                for (int z = 0; z < 3; ++z) d[z][rb] = mfma_i8(qp[kQ8 ? 3 * j + z : 0], v, d[z][rb]);
+            } else {
+                dk[rb] = th_mfma<kFmtBF16>(qh[0], v, dk[rb]);
+                dk[rb] = th_mfma<kFmtBF16>(ql[0], v, dk[rb]);
+            }
+            if (i + W < N) bv[i % W] = get(i + W);
+            else if (i - (N - W) < NM) {  // the mix's operands
+                const int k = i - (N - W);
+                ph[k] = *(const v4i *)(pw + th_pw(16 * k + n, g));
+                pl[k] = *(const v4i *)(pw + Sh::PwB + th_pw(16 * k + n, g));
+                if (k < 2) raw[k] = codes(k);
+                if (k < NW / 4) f[k] = *(const v4i *)(smem + Sh::FlOff + 32 * (c & 1) + 16 * k);
+            }
+            if (i >= 1 && i <= 5) softmax(c + 1, i - 1);
+            if (i == N - 2) bt[0] = codes_f16(raw[0]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        int any = 0;
+#pragma unroll
+        for (int i = 0; i < NW / 4; ++i) any |= f[i][0] | f[i][1] | f[i][2] | f[i][3];
+        if (__builtin_amdgcn_readfirstlane(any)) {
+#pragma unroll
+            for (int i = 0; i < NM; ++i) {
+                const v4f al = *(const v4f *)(smem + Sh::AlOff + (c & 1) * 4 * Sh::NQ + 64 * i + 16 * g);
+#pragma unroll
+                for (int t = 0; t < NC; ++t) acc[i][t] *= al;
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < NC; ++t) {
+#pragma unroll
+            for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(ph[i], bt[t & 1], acc[i][t]);
+#pragma unroll
+            for (int i = 0; i < NM; ++i) acc[i][t] = th_mfma<FMT>(pl[i], bt[t & 1], acc[i][t]);
+            if (t + 1 < NC) bt[(t + 1) & 1] = codes_f16(raw[(t + 1) & 1]);
+            if (t + 2 < NC) raw[t & 1] = codes(t + 2);
+            if (t < RB)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = fmaf((float)d[0][t][i], 65536.f, fmaf((float)d[1][t][i], 256.f, (float)d[2][t][i]));
+                    sp[32 * i + 16 * t] = fmaf(v, qd[i] * x[t], dk[t][i]);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NM; ++i)
+#pragma unroll
+            for (int t = 0; t < NC; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
+    };
+
+    if constexpr (Sh::Pipe && Sh::Dma) {
+        // Five slots: chunks c, c + 1 and c + 2 in use, c + 3 and c + 4 on their way. The passes c = -2, -1 fill the
+        // pipe (the softmax of a chunk below 0 has no rows, the sums are dropped); what the last passes bring and
+        // score is not used.
+        auto slot = [&](int k) __attribute__((always_inline)) { return smem + k * Sh::Slot; };
+        issue(1, 1);
+        wait_vmcnt<ND>();  // chunk 0 has come
+        lds_barrier();
+        int k0 = 3, k1 = 4, k2 = 0, k3 = 1, k4 = 2;  // slots of chunks c .. c + 4
+        for (int c = -2; c < nch; ++c) {
+            issue(c + 4, k4);  // its slot was chunk c - 1's
+            pass(c, slot(k0), slot(k1), slot(k2));
+            if (c < 0) clear();
+            wait_vmcnt<ND>();  // chunk c + 3 has come
+            lds_barrier();
+            const int t = k0;
+            k0 = k1;
+            k1 = k2;
+            k2 = k3;
+            k3 = k4;
+            k4 = t;
+        }
+        wait_vmcnt<0>();  // nothing may land behind the workgroup's end
+    } else if constexpr (Sh::Pipe) {
         // Two barriers a chunk. Between them a wave holds a product and vector work that do not depend on each
         // other, the vector work laid between the products: scores of chunk c + 1 with the softmax of chunk
         // c, then the mix of chunk c with the staging of chunk c + 2. The pass c = -1 fills the pipe (its
@@ -604,17 +788,28 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 if (t == NC - 1) stage(then, held, NL);
             });
             fetch(c + 3, held);
-            if (c < 0) {
-#pragma unroll
-                for (int i = 0; i < NM; ++i)
-#pragma unroll
-                    for (int t = 0; t < NC; ++t) acc[i][t] = v4f{0.f, 0.f, 0.f, 0.f};
-            }
+            if (c < 0) clear();
             lds_barrier();
             uint8_t *t = cur;
             cur = next;
             next = then;
             then = t;
+        }
+    } else if constexpr (Sh::Dma) {
+        wait_vmcnt<0>();
+        lds_barrier();
+        for (int c = 0; c < nch; ++c) {
+            const uint8_t *buf = smem + (c & 1) * Sh::Slot;
+            if (c + 1 < nch) issue(c + 1, (c + 1) & 1);
+            scores(buf, c, [](int) {});
+            lds_barrier();  // both halves of every score are in LDS
+            softmax_read(buf, c);
+#pragma unroll
+            for (int i = 0; i < 5; ++i) softmax(c, i);
+            lds_barrier();  // the weights are in LDS
+            mix(buf, c, [](int) {});
+            wait_vmcnt<0>();  // the next chunk has come
+            lds_barrier();
         }
     } else {
         for (int c = 0; c < nch; ++c) {
