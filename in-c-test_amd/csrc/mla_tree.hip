@@ -289,7 +289,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     // ---- Q8: a chunk's rows from memory to an LDS slot, asynchronously. One instruction of a wave takes 1 KB,
     // two rows of codes; the wave's keys and scales are one instruction each. Rows past the split repeat its
     // last one (their scores are masked).
-    constexpr int KR = Ch / NW, NA = kQ8 ? Ch / 2 / NW : 0, ND = NA + 2;  // a wave's key rows; instructions
+    constexpr int KR = Ch / NW, NA = kQ8 ? Ch / 2 / NW : 0;  // a wave's key rows, pairs of rows of codes
     auto issue = [&](int c, int slot) __attribute__((always_inline)) {
         if constexpr (kQ8) {
             const int last = r1 - r0 - 1;
@@ -469,6 +469,8 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     // The operand reads of a product run W reads ahead of it. The order below is kept as it is written: left
     // to itself the compiler reads each operand right before its use and waits for LDS every time.
     const int spw = Sh::SpOff + 4 * (kh * Sh::SpH + th_sp(16 * m + 4 * g) + n), spr = Sh::SpOff + 4 * (th_sp(sq) + sr);
+    // the sums of a query's three bytes together (256 b + c: below 2^31)
+    auto whole = [](int a, int b, int c) __attribute__((always_inline)) { return fmaf((float)a, 65536.f, (float)(256 * b + c)); };
     // between(i): other work after read i's products
     auto scores_q8 = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
         float *sp = (float *)(smem + spw + (Sh::Pipe ? (c & 1) * Sh::SpB : 0));
@@ -510,8 +512,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         for (int rb = 0; rb < RB; ++rb)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float v = fmaf((float)d[0][rb][i], 65536.f, fmaf((float)d[1][rb][i], 256.f, (float)d[2][rb][i]));
-                sp[32 * i + 16 * rb] = fmaf(v, qd[i] * x[rb], dk[rb][i]);
+                sp[32 * i + 16 * rb] = fmaf(whole(d[0][rb][i], d[1][rb][i], d[2][rb][i]), qd[i] * x[rb], dk[rb][i]);
             }
     };
     auto scores = [&](const uint8_t *buf, int c, auto between) __attribute__((always_inline)) {
@@ -572,21 +573,22 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
     auto softmax = [&](int c, int piece) __attribute__((always_inline)) {
         if (piece == 0) {
-            // of this thread's rows, the ones in the split; none before the first chunk
-            const int nv = (c < 0 ? 0 : r1 - (r0 + c * Ch)) - sr;
+            // of a chunk's rows, the ones in the split; none before the first chunk
+            const int rows = c < 0 ? 0 : r1 - (r0 + c * Ch);
+            if (rows < Ch)
 #pragma unroll
-            for (int e = 0; e < SR; ++e) sx[e] = e < nv ? sx[e] : -INFINITY;
+                for (int e = 0; e < SR; ++e) sx[e] = sr + e < rows ? sx[e] : -INFINITY;
             vsr t = sx;
             if constexpr (kQ8)
 #pragma unroll
-                for (int e = 0; e < SR; ++e) t[e] += __builtin_amdgcn_logf(fmaxf(fabsf(sr4[e]), 1e-28f));
+                for (int e = 0; e < SR; ++e) t[e] += (float)max(__builtin_amdgcn_frexp_expf(sr4[e]), -93);
             cm = fmaxf(t[0], t[1]);
             if constexpr (SR == 4) cm = fmaxf(cm, fmaxf(t[2], t[3]));
             cm = fmaxf(cm, dpp_f32<0xB1>(cm));
         } else if (piece == 1) {
             cm = fmaxf(cm, dpp_f32<0x4E>(cm));
             cm = fmaxf(cm, dpp_f32<0x141>(cm));  // row_half_mirror: the other four of the eight
-            const bool mv = cm > m_run + 2.0f;
+            const bool mv = cm > m_run + 6.0f;
             moved = __any(mv);
             alpha = mv ? __builtin_amdgcn_exp2f(m_run - cm) : 1.0f;
             m_run = mv ? cm : m_run;
@@ -663,9 +665,17 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
 
     // A pass of the Q8 pipe: scores of chunk c + 2, softmax of chunk c + 1, mix of chunk c. None needs another's
-    // results, so a pass is one stream of products with the rest laid between them, and one barrier.
-    auto pass = [&](int c, const uint8_t *b0, const uint8_t *b1, const uint8_t *b2) __attribute__((always_inline)) {
-        constexpr int N = 5 * RB, W = 6;  // as scores_q8
+    // results, so a pass is one stream of products with the rest laid between them, and one barrier. The first
+    // operands of the scores of chunk c + 3 are read at its end: the products start right behind the barrier.
+    constexpr int W = 6;
+    v4i bv[W];
+    float bx[RB];
+    auto first_reads = [&](const uint8_t *b, int i) __attribute__((always_inline)) {
+        bv[i] = *(const v4i *)(b + bofs[i / RB] + 8192 * (i % RB));
+        if (i < RB) bx[i] = *(const float *)(b + Sh::PlaneB + 4 * (16 * i + n));
+    };
+    auto pass = [&](int c, const uint8_t *b0, const uint8_t *b1, const uint8_t *b2, const uint8_t *b3) __attribute__((always_inline)) {
+        constexpr int N = 5 * RB;  // as scores_q8
         float *sp = (float *)(smem + spw + (c & 1) * Sh::SpB);
         const uint8_t *pw = smem + Sh::PwOff + (c & 1) * 2 * Sh::PwB;
         auto get = [&](int i) __attribute__((always_inline)) {
@@ -673,19 +683,17 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             return *(const v4i *)(b2 + (j < 4 ? bofs[j] + 8192 * rb : kofs + 2048 * rb));
         };
         auto codes = [&](int t) __attribute__((always_inline)) { return lds_read_tr8(b0 + (tro[0][0] ^ (16 * t))); };
-        v4i d[3][RB], bv[W], f[NW / 4], ph[NM], pl[NM], bt[2];
+        v4i d[3][RB], f[NW / 4], ph[NM], pl[NM], bt[2];
         v4f dk[RB];
         v2i raw[2];
         float x[RB];
-#pragma unroll
-        for (int i = 0; i < W; ++i) bv[i] = get(i);
         softmax_read(b1, c + 1);
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             dk[rb] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int z = 0; z < 3; ++z) d[z][rb] = v4i{0, 0, 0, 0};
-            x[rb] = *(const float *)(b2 + Sh::PlaneB + 4 * (16 * rb + n));
+            x[rb] = bx[rb];
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -733,10 +741,11 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             if (t + 2 < NC) raw[t & 1] = codes(t + 2);
             if (t < RB)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float v = fmaf((float)d[0][t][i], 65536.f, fmaf((float)d[1][t][i], 256.f, (float)d[2][t][i]));
-                    sp[32 * i + 16 * t] = fmaf(v, qd[i] * x[t], dk[t][i]);
-                }
+                for (int i = 0; i < 4; ++i)
+                    sp[32 * i + 16 * t] = fmaf(whole(d[0][t][i], d[1][t][i], d[2][t][i]), qd[i] * x[t], dk[t][i]);
+            else
+#pragma unroll
+                for (int i = 3 * (t - RB); i < 3 * (t - RB) + 3; ++i) first_reads(b3, i);
             __builtin_amdgcn_sched_barrier(0);
         }
     };
@@ -748,19 +757,20 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     };
 
     if constexpr (Sh::Pipe && Sh::Dma) {
-        // Five slots: chunks c, c + 1 and c + 2 in use, c + 3 and c + 4 on their way. The passes c = -2, -1 fill the
-        // pipe (the softmax of a chunk below 0 has no rows, the sums are dropped); what the last passes bring and
-        // score is not used.
+        // Five slots: chunks c .. c + 3 in use, c + 4 on its way. The passes c = -2, -1 fill the pipe (the softmax of
+        // a chunk below 0 has no rows, the sums are dropped); what the last passes bring and score is not used.
         auto slot = [&](int k) __attribute__((always_inline)) { return smem + k * Sh::Slot; };
         issue(1, 1);
-        wait_vmcnt<ND>();  // chunk 0 has come
+        wait_vmcnt<0>();
         lds_barrier();
+#pragma unroll
+        for (int i = 0; i < W; ++i) first_reads(slot(0), i);
         int k0 = 3, k1 = 4, k2 = 0, k3 = 1, k4 = 2;  // slots of chunks c .. c + 4
         for (int c = -2; c < nch; ++c) {
             issue(c + 4, k4);  // its slot was chunk c - 1's
-            pass(c, slot(k0), slot(k1), slot(k2));
+            pass(c, slot(k0), slot(k1), slot(k2), slot(k3));
             if (c < 0) clear();
-            wait_vmcnt<ND>();  // chunk c + 3 has come
+            wait_vmcnt<0>();  // chunk c + 4 has come
             lds_barrier();
             const int t = k0;
             k0 = k1;
@@ -769,7 +779,6 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             k3 = k4;
             k4 = t;
         }
-        wait_vmcnt<0>();  // nothing may land behind the workgroup's end
     } else if constexpr (Sh::Pipe) {
         // Two barriers a chunk. Between them a wave holds a product and vector work that do not depend on each
         // other, the vector work laid between the products: scores of chunk c + 1 with the softmax of chunk
