@@ -448,7 +448,12 @@ class _State:
     def host(self):
         import ctypes as C
         s, cap = self.s, self.capacity
-        of = lambda p, *shape: np.ctypeslib.as_array((p._type_ * math.prod(shape)).from_address(C.addressof(p.contents))).reshape(shape)  # noqa: E731
+
+        def of(p, *shape):
+            a = (p._type_ * math.prod(shape)).from_address(C.addressof(p.contents))
+            a.owner = self  # the rows live as long as a view of them
+            return np.ctypeslib.as_array(a).reshape(shape)
+
         if self.kind == "q8":
             return [of(s.latent_q8, cap, R), of(s.latent_scale, cap), of(s.rope_bf16, cap, DR)]
         return [of(s.latent, cap, R), of(s.rope, cap, DR)]
