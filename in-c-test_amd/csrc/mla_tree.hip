@@ -125,16 +125,23 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 //   scores: wave (m, kh) = node m's 16 heads x the rows over half kh of the 576 columns, the queries held
 //     in registers; the two halves are added through LDS;
 //   softmax: 8 threads per query, 4 rows (FP32: 2) each, running maximum (moved only when a chunk exceeds it by
-//     more than ln 4) and sum in registers; weights to LDS as the next product's operand;
+//     more than ln 64, so that the sums are rarely scaled) and sum in registers; weights to LDS as the next
+//     product's operand;
 //   mix: every wave 512 / (2 NM) latent columns of all 16 NM queries, the rows read transposed.
 // Operands are 16 bits wide, sums 32: the 32-bit query and weight enter as hi + lo (two products), the
 // BF16 rows as they are, the FP32 rows as hi + lo too (without lo . lo: three products), all in bf16 (what
-// is left out is below 2^-17 of an operand). Q8 codes are exact in fp16, so there the query (times a
-// power of two that puts its largest element near 2^10) and the weights are split in fp16, which keeps 22
-// bits. A Q8 row's scale multiplies its latent score and its weight; to keep the weights within fp16
-// whatever the scales, the running maximum is that of score + ln(scale), so that weight times scale stays
-// <= 4. A scale below 1e-28 counts as 1e-28 there: over kThMax rows of scale zero the sum of the weights
-// stays below 2^(2 + 93 + 19), and 2^13 splits of them can still be added.
+// is left out is below 2^-17 of an operand).
+// Q8: the scores are int8 products of the codes as stored and the query as a whole number below 2^22 (a power of
+// two times it) in three bytes, exact but for that rounding; a row's scale and the query's power multiply the
+// sum. The mix takes the codes as fp16 (exact) and the weights in two fp16 parts, 22 bits; a row's scale
+// multiplies its weight. To keep the weights within fp16 whatever the scales, the running maximum is that of score
+// + the scale's exponent (in units of log2), so that weight times scale stays <= 64. An exponent below -93
+// counts as -93 there: over kThMax rows of scale zero the sum of the weights stays below 2^(6 + 93 + 19), and
+// 2^9 splits of them can still be added.
+// What bounds it: the issue of matrix and vector instructions beside each other. 64 nodes x 32768 Q8 rows: 144 us,
+// 1.04 PFLOP/s of operand products of 16 bits' worth (two per product of the formula) where the library's large
+// bf16 product reaches 1.19; 129 us with rows of zeros, whose products draw less power. The start of a workgroup
+// (table, queries, first chunk, the first pass) is worth 8 us of it, with NM = 2 5.
 constexpr int kThCh = 32;  // rows of a chunk (FP32: of two)
 template <int FMT, int NM>
 struct ThShape {
@@ -163,7 +170,7 @@ struct ThShape {
 // lanes a cycle, and not neighbours: lanes 0-3, 12-15, 20-23, 24-27, then 4-7, 8-11, 16-19, 28-31 and so
 // on (found with patterns of conflicting addresses and the LDS counters). With rows n = lane % 16 and
 // words + lane / 16, as the products read, that is rows 0-3 and 12-15 of one word beside 4-11 of the next.
-//   word c of latent row r: c ^ th_swz(r), which also spreads the transposed reads (4 rows x 32 bytes);
+//   word c of latent row r: c ^ th_swz(r) (Q8, 512 bytes a row: c ^ (r & 15)), which also spreads the transposed reads (4 rows x 32 bytes);
 //   word of 8 weights of query q: th_pw;  score of query q, row 0 (floats): th_sp;
 // 18 + 8 such reads of a chunk and wave: 97 -> 0 cycles of conflicts.
 __device__ __forceinline__ int th_swz(int r) { return ((r & 3) << 1) | ((((r >> 2) ^ (r >> 3)) & 1) << 3) | ((r >> 3) & 1); }
@@ -1125,11 +1132,12 @@ hipError_t launch_tree_sum(hipStream_t st, float *Y, const float *P, size_t pstr
 // Nodes per workgroup and rows per split.
 // nm: 4 share a chunk's staging among twice the queries and overlap it with the products; 2 start sooner,
 // waste less of a small tree, and two workgroups a CU cover each other's waits. In chunks' times of the
-// former, four take kThStart4 / 10 + X4 / CUs and two kThStart2 / 10 + 1.1 X2 / (2 CUs), X the chunks times the
-// workgroups that share them: the lesser is taken. History and combine together, 2 / 4 nodes a workgroup
-//   (FP32, BF16, Q8) 400 rows x 7 nodes 19.1 / 23.5, 18.2 / 22.7, 18.9 / 24.5 us; 9000 x 13 44 / 47, 35 / 37,
-//   38 / 41; eight of 32768 x 2 127 / 154, 79 / 89, 67 / 95; 32768 x 16 99 / 91, 63 / 59, 68 / 65; history alone,
-//   eight of at most 32768 x 24 BF16 89 / 85, one of 32768 x 64 Q8 176 / 161.
+// former, four take kThStart4 / 10 + X4 / CUs and two kThStart2 / 10 + r X2 / (2 CUs), r = 1.2 (Q8 1.1), X the
+// chunks times the workgroups that share them: the lesser is taken. History and combine together, 2 / 4 nodes a
+// workgroup (FP32, BF16, Q8): 400 rows x 7 nodes 20 / 24, 18 / 22, 20 / 26 us; 9000 x 13 43 / 45, 35 / 36, 37 / 40;
+//   32768 x 8 62 / 59, 44 / 44, 45 / 48; 32768 x 16 99 / 90, 62 / 59, 62 / 61; four of 8192 x 16 75 / 73, 49 / 50, 50 /
+//   53; eight of 4096 x 24 100 / 93, 64 / 61, 64 / 64; two of 16384 x 64 259 / 218, 139 / 123, 135 / 125; eight of 32768
+//   x 2 126 / 153, 79 / 87, 61 / 88.
 // rows: one chunk a split where that makes at most kThFew workgroups, else a multiple of the chunk, at least
 // kThMin. A launch of k rounds of workgroups takes about k (chunks + start), and the combine about one chunk's
 // time for each kThJoin splits of a sequence: for each k up to kThRounds the fewest rows that make k rounds
@@ -1148,7 +1156,7 @@ int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
         for (int b = 0; b < t.n; ++b) n += (t.s[b].count + nm - 1) / nm * splits(t.s[b].ctx, chunks * kThCh);
         return n;
     };
-    t.nm = !kimi ? 0 : 20 * groups(1, 4) + 2L * ncu * kThStart4 < 11 * groups(1, 2) + 2L * ncu * kThStart2 ? 4 : 2;
+    t.nm = !kimi ? 0 : 20 * groups(1, 4) + 2L * ncu * kThStart4 < (fmt == kFmtQ8 ? 11 : 12) * groups(1, 2) + 2L * ncu * kThStart2 ? 4 : 2;
     long best = kThMin / kThCh;  // in chunks
     if (t.nm) {
         const long places = (long)ncu * (t.nm == 2 ? 2 : 1), start = t.nm == 2 ? kThStart2 : kThStart4;
