@@ -170,9 +170,10 @@ struct ThShape {
 // lanes a cycle, and not neighbours: lanes 0-3, 12-15, 20-23, 24-27, then 4-7, 8-11, 16-19, 28-31 and so
 // on (found with patterns of conflicting addresses and the LDS counters). With rows n = lane % 16 and
 // words + lane / 16, as the products read, that is rows 0-3 and 12-15 of one word beside 4-11 of the next.
-//   word c of latent row r: c ^ th_swz(r) (Q8, 512 bytes a row: c ^ (r & 15)), which also spreads the transposed reads (4 rows x 32 bytes);
+//   word c of latent row r: c ^ th_swz(r) (Q8, 512 bytes a row: c ^ (r & 15)), which also spreads the
+//     transposed reads (4 rows x 32 bytes; Q8 16 rows x 16 bytes);
 //   word of 8 weights of query q: th_pw;  score of query q, row 0 (floats): th_sp;
-// 18 + 8 such reads of a chunk and wave: 97 -> 0 cycles of conflicts.
+// 18 + 8 such reads of a chunk and wave, BF16: 97 -> 0 cycles of conflicts.
 __device__ __forceinline__ int th_swz(int r) { return ((r & 3) << 1) | ((((r >> 2) ^ (r >> 3)) & 1) << 3) | ((r >> 3) & 1); }
 __device__ __forceinline__ int th_sp(int q) { return (q >> 2) * 144 + (q & 3) * 32; }
 __device__ __forceinline__ int th_pw(int q, int word) {
@@ -219,28 +220,18 @@ __device__ __forceinline__ bool tree_unit(const TreeTable &t, TreeUnit &u) {
     return true;
 }
 
-
 template <int FMT>
 __device__ __forceinline__ v4f th_mfma(const v4i &a, const v4i &b, const v4f &c) {
     if (FMT == kFmtQ8) return mfma_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c);
     return mfma_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c);
 }
 
-// Eight fp32 values as hi and lo operands: bf16, or fp16 for the latents of Q8.
-template <bool F16>
+// Eight fp32 values as hi and lo operands (bf16).
 __device__ __forceinline__ void th_split(const v4f &x0, const v4f &x1, v4i &hi, v4i &lo) {
-    if constexpr (F16) {
-        const float x[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
-        v8h h, r;
-        split8_f16(x, h, r);
-        hi = __builtin_bit_cast(v4i, h);
-        lo = __builtin_bit_cast(v4i, r);
-    } else {
-        v8bf h, r;
-        split8_cvt(x0, x1, h, r);
-        hi = __builtin_bit_cast(v4i, h);
-        lo = __builtin_bit_cast(v4i, r);
-    }
+    v8bf h, r;
+    split8_cvt(x0, x1, h, r);
+    hi = __builtin_bit_cast(v4i, h);
+    lo = __builtin_bit_cast(v4i, r);
 }
 
 // Eight int8 codes -> eight fp16 values, exact: the code + 128 as the low mantissa bits of 1024, minus
@@ -342,7 +333,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     auto put = [&](uint8_t *at, const v4i *v) __attribute__((always_inline)) {
         if constexpr (NP == 2) {
             v4i hi, lo;
-            th_split<false>(__builtin_bit_cast(v4f, v[0]), __builtin_bit_cast(v4f, v[1]), hi, lo);
+            th_split(__builtin_bit_cast(v4f, v[0]), __builtin_bit_cast(v4f, v[1]), hi, lo);
             *(v4i *)at = hi;
             *(v4i *)(at + Sh::PlaneB) = lo;
         } else {
@@ -411,9 +402,9 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, fabsf(qv[j][e]));
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            // 2^(22 - e) with 2^(e - 1) <= mx < 2^e, from the exponent's bits, kept within 2^+-104 (zero and values
-            // that are not finite among them: such a node's own row, which it attends, makes its output NaN)
-            const int e = min(max((int)((__float_as_uint(mx) >> 23) & 255) - 126, -82), 100);
+            // 2^(22 - e) with 2^(e - 1) <= mx < 2^e, from the exponent's bits, at most 2^104. (A query that is not
+            // finite is cut here: the node's own row, which it attends, makes its output NaN.)
+            const int e = max((int)((__float_as_uint(mx) >> 23) & 255) - 126, -82);
             const float qs = __uint_as_float((uint32_t)(149 - e) << 23);
             const float qi = __uint_as_float((uint32_t)(105 + e) << 23);
 #pragma unroll
@@ -436,9 +427,9 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) th_split<false>(qv[2 * j], qv[2 * j + 1], qh[j], ql[j]);
+            for (int j = 0; j < 8; ++j) th_split(qv[2 * j], qv[2 * j + 1], qh[j], ql[j]);
         }
-        th_split<false>(qv[16], qv[17], qh[NQK - 1], ql[NQK - 1]);
+        th_split(qv[16], qv[17], qh[NQK - 1], ql[NQK - 1]);
     }
     if constexpr (!Sh::Dma) stage_all(smem, ahead);
 
