@@ -857,7 +857,6 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
 
 // ---- the nodes' own rows, the merge and W_UV (Kimi shapes, DV = 128) --------------------------------
 
-constexpr int kTcNodes = 4;  // nodes of a combine workgroup (at most)
 constexpr int kTcAhead = 6;  // splits whose loads a wave has in flight
 struct TreeCombArgs {
     TreeRowsTable t;
@@ -867,25 +866,30 @@ struct TreeCombArgs {
     uint16_t *hos;
     size_t plane;  // words between the hi and lo planes of hos
     float smscale;
-    int DN, n, tn;  // n nodes, tn of them per workgroup (1, 2, 4)
+    int DN, n, tn;  // n nodes, tn of them per workgroup (EARLY: 1, 2, 4; else 8)
 };
 
 // Workgroup = one head of tn nodes, eight waves, 8 / tn of them per node (in turn over the history's splits).
+// Bound by latency: table -> path -> partials -> W_UV, 8.5 us for a few nodes of a short history, 16 us at 4 nodes x 256
+// splits, 22 us at 256 nodes x 4 splits (34 MB of partials, 67 MB of W_UV from L2).
 //   merge: mix = (sum_s e^(m_s - M) acc_s + the path's) / (sum_s e^(m_s - M) l_s + the path's), lane l columns
 //     4 l .. and 256 + 4 l ..;
 //   path: the node's first wave takes the node's own row and its ancestors' (rows ctx + i, at most 64), four at
 //     a time: scores in fp32 (row j's in lane j), their weights, their mix. Rows of other branches are not read;
 //   W_UV: head output d = sum_r W[d, r] mix[r] on MFMA, wave w rows 16 w .., its W operands requested at the
-//     start; the mix enters as three bf16 planes (24 bits), plane p of node j as column 4 p + j.
+//     start (EARLY, one workgroup per CU) or after the merge; the mix enters as three bf16 planes (24 bits), plane
+//     p of node j as column TN p + j.
 // The output is written as the bf16 hi | lo planes that o_proj's launch takes.
 template <int FMT, bool EARLY>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(EARLY ? 2 : 4))) void k_tree_combine(TreeCombArgs a) {
     constexpr int R = 512, DR = 64, NH = 16;
-    __shared__ __attribute__((aligned(16))) uint8_t xs[16 * 1024];  // column c's words of 8: word ^ (c & 15)
-    __shared__ __attribute__((aligned(16))) float red[8][R];
+    constexpr int TN = EARLY ? 4 : 8, CB = TN / 4;  // nodes at most, blocks of 16 columns
+    const int tn = EARLY ? a.tn : TN;
+    __shared__ __attribute__((aligned(16))) uint8_t xs[CB * 16 * 1024];  // column c's words of 8: word ^ (c & 15)
+    __shared__ __attribute__((aligned(16))) float red[EARLY ? 8 : 1][R];
     const int tid = threadIdx.x, l = tid & 63, n = l & 15, g = l >> 4;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int h = blockIdx.x % NH, tn = a.tn, first = blockIdx.x / NH * tn;
+    const int h = blockIdx.x % NH, first = blockIdx.x / NH * tn;
     // this lane's entries of the tables
     const TreeRows q = a.t.s[l];
     const int seq4 = ((const int *)a.nd.seq)[l], parent4 = ((const int *)a.nd.parent)[l];  // four nodes a lane
@@ -1051,7 +1055,7 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(EARLY ? 2 :
     if constexpr (!EARLY)
 #pragma unroll
         for (int kb = 0; kb < 16; ++kb) wa[kb] = *(const v4i *)(wrow + 32 * kb);
-    if (wpn > 1) {  // the node's waves in turn order
+    if (EARLY && wpn > 1) {  // the node's waves in turn order
         *(v4f *)&red[w][4 * l] = c0;
         *(v4f *)&red[w][256 + 4 * l] = c1;
         __syncthreads();
@@ -1074,24 +1078,30 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(EARLY ? 2 :
 #pragma unroll
             for (int pl = 0; pl < 3; ++pl) {
                 const v2bf b0 = __builtin_convertvector((v2f{x[0], x[1]}), v2bf), b1 = __builtin_convertvector((v2f{x[2], x[3]}), v2bf);
-                const int col = kTcNodes * pl + j;
-                *(int2 *)(xs + col * 1024 + 16 * ((32 * half + (l >> 1)) ^ col) + 8 * (l & 1)) =
+                const int col = TN * pl + j;
+                *(int2 *)(xs + col * 1024 + 16 * ((32 * half + (l >> 1)) ^ (col & 15)) + 8 * (l & 1)) =
                     int2{__builtin_bit_cast(int, b0), __builtin_bit_cast(int, b1)};
                 x -= v4f{(float)b0.x, (float)b0.y, (float)b1.x, (float)b1.y};
             }
         }
     }
     __syncthreads();
-    v4f acc = {0.f, 0.f, 0.f, 0.f};
+    v4f acc[CB];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) acc[cb] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kb = 0; kb < 16; ++kb)
-        acc = mfma_bf16(__builtin_bit_cast(v8bf, wa[kb]), *(const v8bf *)(xs + n * 1024 + 16 * ((4 * kb + g) ^ n)), acc);
-    // columns j, 4 + j, 8 + j are the planes of node j (columns without one are not used)
+#pragma unroll
+        for (int cb = 0; cb < CB; ++cb)
+            acc[cb] = mfma_bf16(__builtin_bit_cast(v8bf, wa[kb]), *(const v8bf *)(xs + (16 * cb + n) * 1024 + 16 * ((4 * kb + g) ^ n)), acc[cb]);
+    // columns j, TN + j, 2 TN + j are the planes of node j (columns without one are not used)
     const int node = first + n;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float mid = dpp_f32<0x12C>(acc[i]), low = dpp_f32<0x128>(acc[i]);  // row_ror:12, row_ror:8: lanes n + 4, n + 8
-        const float v = acc[i] + (mid + low);
+        // TN = 4: row_ror:12, row_ror:8: lanes n + 4, n + 8
+        const float mid = TN == 4 ? dpp_f32<0x12C>(acc[0][i]) : dpp_f32<0x128>(acc[0][i]);
+        const float low = TN == 4 ? dpp_f32<0x128>(acc[0][i]) : acc[CB - 1][i];
+        const float v = acc[0][i] + (mid + low);
         if (n < tn && node < a.n) {
             uint16_t hi, lo;
             split_bf16(v, hi, lo);
@@ -1215,10 +1225,12 @@ hipError_t launch_tree_combine(hipStream_t st, int fmt, const TreeTable &t, cons
                                const uint16_t *kv_b, const DecodeWork &w) {
     if (!tree_table_ok(fmt, t, d, true)) return hipErrorInvalidValue;
     TreeCombArgs a{tree_rows(t), nd, w.qf, w.part, kv_b, w.hos, (size_t)t.nodes * d.HO, 1.0f / sqrtf((float)d.QD), d.DN, t.nodes, 1};
-    // nodes per workgroup: enough workgroups for the CUs first, then W_UV (128 KB a workgroup) shared by more
-    a.tn = t.nodes <= 16 ? 1 : t.nodes <= 32 ? 2 : 4;
+    // Nodes per workgroup: enough workgroups for the CUs first, then W_UV (128 KB a workgroup) shared by more. 8
+    // nodes (W_UV requested after the merge, two workgroups a CU) against 4: 80 nodes 13.7 / 17.0 us, 128 15.6 /
+    // 18.1, 168 19.4 / 26.4, 256 22.4 / 33.9 (BF16).
+    a.tn = t.nodes <= 16 ? 1 : t.nodes <= 32 ? 2 : t.nodes <= 64 ? 4 : 8;
     const dim3 grid((unsigned)((t.nodes + a.tn - 1) / a.tn * 16));
-    const bool early = t.nodes <= 64;  // one workgroup per CU
+    const bool early = a.tn < 8;  // one workgroup per CU
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(512), 0, st, a); };
     if (fmt == kFmtQ8) early ? go(k_tree_combine<kFmtQ8, true>) : go(k_tree_combine<kFmtQ8, false>);
     else if (fmt == kFmtF32) early ? go(k_tree_combine<kFmtF32, true>) : go(k_tree_combine<kFmtF32, false>);
