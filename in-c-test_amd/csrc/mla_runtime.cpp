@@ -1936,14 +1936,15 @@ size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &t
 
 // Nodes beyond which a group's q_proj | kv_a and o_proj are products over LDS tiles instead of the decode's GEMVs
 // (in groups of 16 tokens). us, GEMV / tiles: q_proj | kv_a at 12 nodes 7.9 / 9.4, 20 10.1 / 9.4, 64 16.0 / 12.0;
-// o_proj at 64 nodes 11.8 / 6.5 + 5 (the sum of its quarters), 170 29.6 / 14.4 + 5.
-constexpr int kTreeGemmX = 16, kTreeGemm = 64;
+// o_proj at 64 nodes 11.8 / 6.5 + 5 (the sum of its quarters), 170 29.6 / 14.4 + 5. From host memory the tiles of
+// many workgroups wait for the bus: 24 nodes 14.7 / 21.6, 32 18.0 / 26.0, 48 23.8 / 17.9.
+constexpr int kTreeGemmX = 16, kTreeGemmHost = 32, kTreeGemm = 64;
 
 // One tree decode of a launch group: the steps of decode_group with the group's nodes as its
 // members, each member's row at history row ctx + i and its rotation at position ctx + depth.
-// Everything it needs has been acquired (tree_prepare).
+// Everything it needs has been acquired (tree_prepare). host: d_x and d_out are pinned host memory.
 int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights &dw, const TreeIn *seqs, int n, bool tokens,
-               const float *d_x, float *d_out, bool residual, DecodeWork &w, const InNorm *in_norm = nullptr) {
+               const float *d_x, float *d_out, bool residual, DecodeWork &w, bool host, const InNorm *in_norm = nullptr) {
     Ctx &c = ctx();
     hipStream_t st = c.stream;
     if (tokens) {
@@ -1967,7 +1968,7 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         w.ynp = kGemvKs;
         w.ypstride = (size_t)N * ldy;
         // the same partials bit for bit, as products over LDS tiles
-        if (N > kTreeGemmX && d.H == 2048) HIP_TRY(launch_kva_x(st, w.y, w.ypstride, ldy, d_x, N, dw.q, d.QO, dw.kva, d.KVO));
+        if (N > (host ? kTreeGemmHost : kTreeGemmX) && d.H == 2048) HIP_TRY(launch_kva_x(st, w.y, w.ypstride, ldy, d_x, N, dw.q, d.QO, dw.kva, d.KVO));
         else HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
     } else {
         w.ynp = 1;
@@ -2167,7 +2168,7 @@ int tree_host(float *out, const float *x, const int *parents, int count, int sta
     memcpy(c.pin_in.p, x, xin);
     wk.rows = (uint8_t *)c.pin_out.p + xin;  // as in decode_block: x, outputs and rows in the pinned buffers
     if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data(), 1, tokens, (const float *)c.pin_in.p,
-                   (float *)c.pin_out.p, false, wk) != 0)
+                   (float *)c.pin_out.p, false, wk, true) != 0)
         return -1;
     HIP_TRY(hipStreamSynchronize(c.stream));
     memcpy(out, c.pin_out.p, xin);
@@ -2209,7 +2210,7 @@ int tree_device(float *d_out, const float *d_x, const int *counts, const int *pa
         DecodeWork wk;
         if (decode_work(d, n, (int)rb, wk) != 0) return -1;
         if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data() + g, e - g, tokens, d_x + at * d.H,
-                       d_out + at * d.H, (flags & KVL_MLA_RESIDUAL) != 0, wk, in_norm) != 0)
+                       d_out + at * d.H, (flags & KVL_MLA_RESIDUAL) != 0, wk, false, in_norm) != 0)
             return -1;
         if (!(flags & KVL_MLA_NO_ADVANCE))
             for (int i = g; i < e; ++i) {

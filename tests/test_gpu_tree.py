@@ -313,6 +313,30 @@ def test_rows_behind_the_history_do_not_enter(models, kind, ctx):
         s.free()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [4096, 328])
+def test_other_hidden_sizes(models, kind, size):
+    """The attention's dims of KIMI under another hidden size: other projections, few nodes and many."""
+    cfg = inputs.config(**dict(trees.KIMI, hidden_size=size))
+    layer = inputs.fast_layer(cfg, 0x5D)
+    w = layer.struct()
+    lib.check(L.kvl_mla_bind_weights(C.byref(cfg), C.byref(w)), "bind")
+    for sizes in ([5], [20, 9], [60, 50]):
+        ps = [tree("any", n, i) for i, n in enumerate(sizes)]
+        states = [State(kind, cfg, 300 + n).load(i, 200 + i) for i, n in enumerate(sizes)]
+        x = hidden(cfg, 0x5E, sum(sizes))
+        got = batch_device(kind, cfg, w, states, ps, x)
+        at = 0
+        for i, n in enumerate(sizes):
+            rows = states[i].pull(0, 200 + i + n)
+            e = off(got[at:at + n], reference(cfg, layer, x[at:at + n], ps[i], 200 + i, rows, kind))
+            assert e <= TOL, (sizes, i, e)
+            at += n
+        for s in states:
+            s.free()
+    L.kvl_mla_release_weights(C.byref(w))
+
+
 def test_q8_scales_of_all_sizes(models):
     """Q8 rows whose scales run from zero over the smallest numbers to the usual ones: small scales must
     not push the other rows' weights out of range."""
