@@ -1967,12 +1967,14 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         }
         w.ynp = kGemvKs;
         w.ypstride = (size_t)N * ldy;
+        StageTimer tm(0);
         // the same partials bit for bit, as products over LDS tiles
         if (N > (host ? kTreeGemmHost : kTreeGemmX) && d.H == 2048) HIP_TRY(launch_kva_x(st, w.y, w.ypstride, ldy, d_x, N, dw.q, d.QO, dw.kva, d.KVO));
         else HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
     } else {
         w.ynp = 1;
         w.ypstride = 0;
+        StageTimer tm(0);
         HIP_TRY(launch_gemv(st, w.y, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H, false));
     }
     TreeNodes nd;
@@ -1991,6 +1993,7 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
     const float2 *cs = nullptr;
     if (rope_table(theta, d.DR, maxpos + 1, &cs) != 0) return -1;
     if (tree_prep_ok(d, w.ynp, dw.ukt)) {
+        StageTimer tm(1);
         HIP_TRY(launch_tree_prep(st, fmt, tt, nd, d, dw.norm, eps, cs, dw.kvb, dw.ukt, w));
     } else {
         const size_t rb = row_bytes_of(fmt, d.R, d.DR, 0);
@@ -2010,13 +2013,21 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
             wk.y += (size_t)k0 * ldy;
             wk.qf += (size_t)k0 * d.NH * std::max(d.R + d.DR, d.QD);
             wk.rows += (size_t)k0 * rb;
+            StageTimer tm(1);
             HIP_TRY(launch_append_qprep(st, fmt, t, d, wk.y, ldy, d.QO, w.ynp, w.ypstride, dw.norm, eps, cs, dw.kvb, dw.ukt, wk,
                                         false));
         }
     }
     if (tt.nm) {
-        HIP_TRY(launch_tree_history(st, fmt, tt, d, w));
-        HIP_TRY(launch_tree_combine(st, fmt, tt, nd, d, dw.kvb, w));
+        if (tt.units > 0) {
+            StageTimer tm(3);
+            HIP_TRY(launch_tree_history(st, fmt, tt, d, w));
+        }
+        {
+            StageTimer tm(4);
+            HIP_TRY(launch_tree_combine(st, fmt, tt, nd, d, dw.kvb, w));
+        }
+        StageTimer tm(5);
         if (N > kTreeGemm && gemv_ksplit_ok(d.H, d.H) && d.H <= ldy && d.H % 4 == 0 && (uintptr_t)d_out % 16 == 0) {  // partials in the place of w.y
             const size_t ps = (size_t)N * d.H;
             HIP_TRY(launch_kva_tok(st, w.y, ps, d.H, w.hos, w.hos + (size_t)N * d.HO, N, dw.o, d.H, d.HO));
@@ -2026,7 +2037,10 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         }
         return 0;
     }
-    HIP_TRY(launch_tree_generic(st, fmt, tt, nd, d, w));
+    {
+        StageTimer tm(3);
+        HIP_TRY(launch_tree_generic(st, fmt, tt, nd, d, w));
+    }
     for (int k0 = 0; k0 < N; k0 += kMaxBatch) {
         SeqTable t;
         memset(&t, 0, sizeof t);
@@ -2038,7 +2052,11 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         DecodeWork wk = w;
         wk.mix += (size_t)k0 * d.NH * std::max(d.R, d.DV);
         wk.ho += (size_t)k0 * d.HO;
-        HIP_TRY(launch_combine(st, fmt, t, d, dw.kvb, wk));
+        {
+            StageTimer tm(4);
+            HIP_TRY(launch_combine(st, fmt, t, d, dw.kvb, wk));
+        }
+        StageTimer tm(5);
         // the planes of a combine's head outputs lie t.n rows apart: o_proj follows slice by slice
         if (combine_writes_hos(fmt, d) && gemv_xs_ok(d.HO))
             HIP_TRY(launch_gemv_xs(st, d_out + (size_t)k0 * d.H, d.H, wk.hos, t.n, dw.o, d.H, d.HO, residual));

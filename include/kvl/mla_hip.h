@@ -350,8 +350,8 @@ int kvl_mla_graph_destroy(void *graph_exec);
  * graph overwrites their timestamps, so read once after the last replay, then destroy the
  * graph before timing anything else). kvl_mla_timing_read() sums the
  * durations (ms) and launch counts of the six stages (gemv_in, append [+ qprep: one launch
- * for the compressed formats], qprep [expanded format], attention,
- * combine, gemv_out) since the last read. kvl_mla_timing_stages(mask) limits the bracketing
+ * for the compressed formats], qprep [expanded format], attention [of a tree: over its history],
+ * combine [of a tree: with its nodes' own rows], gemv_out) since the last read. kvl_mla_timing_stages(mask) limits the bracketing
  * to the stages whose bit is set (bit i: stage i; all six by default): every bracketed launch
  * carries its two event records, whose gaps the durations include. Events: record on the
  * library stream, elapsed time between two recorded events (waits for the second).

@@ -513,6 +513,33 @@ def test_host_calls_are_refused_in_a_capture(models, kind):
         s.free()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dims,sizes,launches", [
+    ("kimi", [7], [1, 1, 0, 1, 1, 1]), ("kimi", [60, 50], [1, 1, 0, 1, 1, 1]), ("kimi", [64] * 5, [2, 2, 0, 2, 2, 2]),
+    ("lab", [60, 50], [1, 2, 0, 1, 2, 2]),
+])
+def test_stage_timing(models, kind, dims, sizes, launches):
+    """A tree decode's launches are bracketed as the other decodes' are."""
+    cfg, layer, w = models(dims)
+    ps = [tree("any", n, i) for i, n in enumerate(sizes)]
+    states = [State(kind, cfg, 200).load(i, 100) for i in range(len(sizes))]
+    x = hidden(cfg, 0x7E, sum(sizes))
+    want = batch_device(kind, cfg, w, states, ps, x, lib.NO_ADVANCE)
+    ms, count = (C.c_double * 6)(), (C.c_int * 6)()
+    lib.check(L.kvl_mla_timing_enable(1), "timing")
+    try:
+        lib.check(L.kvl_mla_timing_read(ms, count), "read")
+        got = batch_device(kind, cfg, w, states, ps, x, lib.NO_ADVANCE)
+        lib.check(L.kvl_mla_timing_read(ms, count), "read")
+    finally:
+        L.kvl_mla_timing_enable(0)
+    np.testing.assert_array_equal(got, want)
+    assert list(count) == launches
+    assert all((t > 0) == (n > 0) for t, n in zip(ms, count))
+    for s in states:
+        s.free()
+
+
 def test_two_threads(models):
     """Calls from two threads take turns; each thread reads its own errors."""
     import threading
