@@ -449,19 +449,25 @@ __global__ __launch_bounds__(256) void k_kva_tok(KvaTokArgs a) {
 // waves 0..15). Tiles are numbered row block fastest, then quarter, then token block, and XCD
 // b % 8 takes a contiguous eighth of them, so the row blocks sharing a token block's
 // activations run under one L2.
-// XF: x comes as fp32 (at XH) and is split where its fragments are read, which saves the launch that writes
-// the planes; a token's 128 bytes of a k step (eight slots) take the room of its two planes, slot s stored
-// at s ^ xswz(row), and the two reads of a fragment hit distinct banks too. q_proj | kv_a of trees of 20 /
-// 64 / 170 / 256 nodes (us): k_gemv_ksplit 10.1 / 16.0 / 32 / -, planes and their launch 12.7 / 15.0 / 23.6 /
-// 27, XF 9.4 / 12.0 / 22.0 / 28.
+// X (what the launch is for): kKvaRows as described, from planes. kKvaX: x comes as fp32 (at XH) and is split
+// where its fragments are read, which saves the launch that writes the planes; a token's 128 bytes of a k step
+// (eight slots) take the room of its two planes, slot s stored at s ^ xswz(row), and the two reads of a fragment
+// hit distinct banks too. Blocks of W's rows alone, whose sums no stored row depends on, keep one running sum
+// for both halves in the MFMA's own accumulator; blocks with rows of W1 (kv_a) add as described. kKvaSum: planes,
+// every block with the one running sum.
+// q_proj | kv_a of trees of 20 / 64 / 170 / 256 nodes (us): k_gemv_ksplit 10.1 / 16.0 / 32 / -, planes and their
+// launch 12.7 / 15.0 / 23.6 / 27, kKvaX 9.1 / 11.5 / 19.0 / 26.8, with every block adding in k order 9.4 / 12.0 / 22.0 /
+// 28; o_proj of 100 / 170 / 256 nodes, kKvaSum 9.3 / 11.2 / 13.4, in k order 11.3 / 14.4 / 16.6.
+enum { kKvaRows, kKvaX, kKvaSum };
 template <int TU_, int TT_, int WT_, int WR_, int NS_>
 struct KvgShape {
     static constexpr int TU = TU_, TT = TT_, WT = WT_, WR = WR_, NS = NS_;  // NS: ring stages
     static constexpr int BT = 16 * TU * WT, BR = 16 * TT * WR, NT = 64 * WT * WR;
 };
 
-template <class Sh, bool XF>
+template <class Sh, int X>
 __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
+    constexpr bool XF = X == kKvaX;
     constexpr int TU = Sh::TU, TT = Sh::TT, NS = Sh::NS;
     constexpr int NWV = Sh::WT * Sh::WR, NT = Sh::NT, BT = Sh::BT, BR = Sh::BR;
     constexpr int ROWB = 64, XPL = BT * ROWB, STAGE = 2 * XPL + BR * ROWB;
@@ -524,7 +530,7 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
     v4f sh[TT][TU], sl[TT][TU];
 #pragma unroll
     for (int j = 0; j < NS - 1; ++j) issue(j);
-    auto step = [&](int j) __attribute__((always_inline)) {
+    auto step = [&](int j, auto one) __attribute__((always_inline)) {  // one: a running sum for both halves
         // stage j has landed when only the NS - 2 stages after it may still be in flight (a wave
         // issues NMIN or NMIN + 1 copies per stage; waiting for NMIN each is exact or conservative)
         if (j + NS - 1 <= 16) wait_vmcnt<(NS - 2) * NMIN>();
@@ -549,15 +555,25 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
         for (int t = 0; t < TT; ++t)
 #pragma unroll
             for (int u = 0; u < TU; ++u) {
+                if constexpr (decltype(one)::value) {
+                    sh[t][u] = mfma_bf16(wv[t], xh[u], j == 0 ? z : sh[t][u]);
+                    sh[t][u] = mfma_bf16(wv[t], xl[u], sh[t][u]);
+                    sl[t][u] = z;
+                    continue;
+                }
                 const v4f rh = mfma_bf16(wv[t], xh[u], z);
                 const v4f rl = mfma_bf16(wv[t], xl[u], z);
                 sh[t][u] = j == 0 ? rh : sh[t][u] + rh;
                 sl[t][u] = j == 0 ? rl : sl[t][u] + rl;
             }
     };
-    step(0);
+    auto steps = [&](auto one) __attribute__((always_inline)) {
+        step(0, one);
 #pragma nounroll
-    for (int j = 1; j < 16; ++j) step(j);
+        for (int j = 1; j < 16; ++j) step(j, one);
+    };
+    if (X == kKvaSum || (X == kKvaX && row0 + BR <= a.out0)) steps(std::true_type());
+    else steps(std::false_type());
     float *y = a.Y + (size_t)kq * a.pstride;
     const bool vec = (a.ldy & 3) == 0;
 #pragma unroll
@@ -580,11 +596,11 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
     }
 }
 
-template <class Sh, bool XF>
+template <class Sh, int X>
 static hipError_t kva_gemm_launch(hipStream_t st, const KvaTokArgs &a) {
     const size_t tiles = (size_t)((a.out + Sh::BR - 1) / Sh::BR) * kGemvKs * ((a.S + Sh::BT - 1) / Sh::BT);
     if (tiles > 0x7fffffff) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((k_kva_gemm<Sh, XF>), dim3((unsigned)tiles), dim3(Sh::NT), 0, st, a);
+    hipLaunchKernelGGL((k_kva_gemm<Sh, X>), dim3((unsigned)tiles), dim3(Sh::NT), 0, st, a);
     return hipGetLastError();
 }
 
@@ -601,23 +617,23 @@ static bool kva_args_ok(const KvaTokArgs &a) {
 //   37 tokens 5.4 / 6.5 / 6.9 / 9.6 / 11.8 / 17.2   200: 10.3 / 7.2 / 7.4 / 9.9 / - / 19.1
 //   384: 18.5 / 12.5 / 9.2 / 10.3 / - / 19.2        896: 35.7 / 23.9 / 16.5 / 14.3 / - / 20.5
 //   1181: - / - / - / 21.5 / 18.2 / 21.4            16000: - / - / - / - / 171 / 127
-template <bool XF>
+// From fp32 x the large tile splits more of it per wave: 64 x 96 up to three rounds (256 tokens 26.8 / 27.8).
+template <int X>
 static hipError_t kva_tiles(hipStream_t st, const KvaTokArgs &a) {
     auto tiles = [&](int bt, int br) { return (long)((a.S + bt - 1) / bt) * kGemvKs * ((a.out + br - 1) / br); };
-    if (tiles(32, 32) <= 256) return kva_gemm_launch<KvgShape<1, 1, 2, 2, 16>, XF>(st, a);
-    if (tiles(32, 64) <= 256) return kva_gemm_launch<KvgShape<1, 2, 2, 2, 16>, XF>(st, a);
-    if (tiles(32, 64) <= 512) return kva_gemm_launch<KvgShape<1, 2, 2, 2, 8>, XF>(st, a);
-    if (tiles(64, 64) <= 512) return kva_gemm_launch<KvgShape<2, 2, 2, 2, 6>, XF>(st, a);
-    if (tiles(64, 96) <= 512) return kva_gemm_launch<KvgShape<2, 3, 2, 2, 4>, XF>(st, a);
-    return kva_gemm_launch<KvgShape<4, 4, 2, 3, 3>, XF>(st, a);
+    if (tiles(32, 32) <= 256) return kva_gemm_launch<KvgShape<1, 1, 2, 2, 16>, X>(st, a);
+    if (tiles(32, 64) <= 256) return kva_gemm_launch<KvgShape<1, 2, 2, 2, 16>, X>(st, a);
+    if (tiles(32, 64) <= 512) return kva_gemm_launch<KvgShape<1, 2, 2, 2, 8>, X>(st, a);
+    if (tiles(64, 64) <= 512) return kva_gemm_launch<KvgShape<2, 2, 2, 2, 6>, X>(st, a);
+    if (tiles(64, 96) <= (X == kKvaX ? 768 : 512)) return kva_gemm_launch<KvgShape<2, 3, 2, 2, 4>, X>(st, a);
+    return kva_gemm_launch<KvgShape<4, 4, 2, 3, 3>, X>(st, a);
 }
 
 hipError_t launch_kva_tok(hipStream_t st, float *Y, size_t pstride, int ldy, const uint16_t *XH,
-                          const uint16_t *XL, int S, const uint16_t *W, int out0, int in, const uint16_t *W1,
-                          int out1) {
-    const KvaTokArgs a{Y, XH, XL, W, W1, pstride, ldy, S, out0, out0 + out1, in};
+                          const uint16_t *XL, int S, const uint16_t *W, int out, int in) {
+    const KvaTokArgs a{Y, XH, XL, W, nullptr, pstride, ldy, S, out, out, in};
     if (!kva_args_ok(a)) return hipErrorInvalidValue;
-    if (in == 2048) return kva_tiles<false>(st, a);
+    if (in == 2048) return kva_tiles<kKvaRows>(st, a);
     const dim3 grid((a.out + 63) / 64, kGemvKs, (S + 127) / 128);
     hipLaunchKernelGGL((k_kva_tok<2>), grid, dim3(256), 0, st, a);
     return hipGetLastError();
@@ -627,7 +643,13 @@ hipError_t launch_kva_x(hipStream_t st, float *Y, size_t pstride, int ldy, const
                         const uint16_t *W1, int out1) {
     const KvaTokArgs a{Y, (const uint16_t *)X, nullptr, W, W1, pstride, ldy, S, out0, out0 + out1, 2048};
     if (!kva_args_ok(a)) return hipErrorInvalidValue;
-    return kva_tiles<true>(st, a);
+    return kva_tiles<kKvaX>(st, a);
+}
+
+hipError_t launch_kva_sum(hipStream_t st, float *Y, size_t pstride, const uint16_t *XH, const uint16_t *XL, int S, const uint16_t *W, int out) {
+    const KvaTokArgs a{Y, XH, XL, W, nullptr, pstride, out, S, out, out, 2048};
+    if (!kva_args_ok(a)) return hipErrorInvalidValue;
+    return kva_tiles<kKvaSum>(st, a);
 }
 
 bool gemv_xs_ok(int in) { return in == 2048 || in == 4096; }

@@ -95,14 +95,16 @@ hipError_t launch_gemv_ksplit(hipStream_t st, float *Y, size_t pstride, int ldy,
                               int out1, int in, unsigned *zero_flags = nullptr, int nzero = 0);
 // The same kGemvKs partials (bit for bit) for S tokens given as bf16 planes XH, XL [S, in]
 // (k_split's rounding), tiled over 128 tokens so a weight tile serves many of them: the
-// prefill's kv_a projection and the state prefill. The output rows are the concatenation of W (out0 rows)
-// and W1 (out1 rows, may be 0). Shapes as launch_gemv_ksplit.
+// prefill's kv_a projection and the state prefill. Shapes as launch_gemv_ksplit.
 hipError_t launch_kva_tok(hipStream_t st, float *Y, size_t pstride, int ldy, const uint16_t *XH,
-                          const uint16_t *XL, int S, const uint16_t *W, int out0, int in,
-                          const uint16_t *W1 = nullptr, int out1 = 0);
-// The same from fp32 X [S, 2048], W rows of 2048 (finite x: the planes' partials bit for bit).
+                          const uint16_t *XL, int S, const uint16_t *W, int out, int in);
+// The same from fp32 X [S, 2048], W (out0 rows of 2048) and W1 (out1): the partials of W1's rows bit for bit (finite
+// x), those of W's in another order of summation.
 hipError_t launch_kva_x(hipStream_t st, float *Y, size_t pstride, int ldy, const float *X, int S, const uint16_t *W, int out0,
                         const uint16_t *W1, int out1);
+// Partials of planes XH, XL [S, 2048] by W [out, 2048], in that other order.
+hipError_t launch_kva_sum(hipStream_t st, float *Y, size_t pstride, const uint16_t *XH, const uint16_t *XL, int S,
+                          const uint16_t *W, int out);
 // Y[b, o] (+)= sum_k W[o, k] x[b, k] with x given as bf16 planes XS[2][B][in] (hi, lo), as
 // launch_combine writes them (DecodeWork::hos). Shapes when gemv_xs_ok (in = 2048 or 4096),
 // any B.

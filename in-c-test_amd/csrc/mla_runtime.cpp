@@ -1935,8 +1935,8 @@ size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &t
 }
 
 // Nodes beyond which a group's q_proj | kv_a and o_proj are products over LDS tiles instead of the decode's GEMVs
-// (in groups of 16 tokens). us, GEMV / tiles: q_proj | kv_a at 12 nodes 7.9 / 9.4, 20 10.1 / 9.4, 64 16.0 / 12.0;
-// o_proj at 64 nodes 11.8 / 6.5 + 5 (the sum of its quarters), 170 29.6 / 14.4 + 5. From host memory the tiles of
+// (in groups of 16 tokens). us, GEMV / tiles: q_proj | kv_a at 12 nodes 7.9 / 9.4, 20 10.1 / 9.1, 64 16.0 / 11.5;
+// o_proj at 64 nodes 11.8 / 6.5 + 5 (the sum of its quarters), 170 29.6 / 11.2 + 5. From host memory the tiles of
 // many workgroups wait for the bus: 24 nodes 14.7 / 21.6, 32 18.0 / 26.0, 48 23.8 / 17.9.
 constexpr int kTreeGemmX = 16, kTreeGemmHost = 32, kTreeGemm = 64;
 
@@ -1968,7 +1968,7 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         w.ynp = kGemvKs;
         w.ypstride = (size_t)N * ldy;
         StageTimer tm(0);
-        // the same partials bit for bit, as products over LDS tiles
+        // the same partials as products over LDS tiles, those of kv_a bit for bit
         if (N > (host ? kTreeGemmHost : kTreeGemmX) && d.H == 2048) HIP_TRY(launch_kva_x(st, w.y, w.ypstride, ldy, d_x, N, dw.q, d.QO, dw.kva, d.KVO));
         else HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
     } else {
@@ -2030,7 +2030,7 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         StageTimer tm(5);
         if (N > kTreeGemm && gemv_ksplit_ok(d.H, d.H) && d.H <= ldy && d.H % 4 == 0 && (uintptr_t)d_out % 16 == 0) {  // partials in the place of w.y
             const size_t ps = (size_t)N * d.H;
-            HIP_TRY(launch_kva_tok(st, w.y, ps, d.H, w.hos, w.hos + (size_t)N * d.HO, N, dw.o, d.H, d.HO));
+            HIP_TRY(launch_kva_sum(st, w.y, ps, w.hos, w.hos + (size_t)N * d.HO, N, dw.o, d.H));
             HIP_TRY(launch_tree_sum(st, d_out, w.y, ps, ps, residual));
         } else {
             HIP_TRY(launch_gemv_xs(st, d_out, d.H, w.hos, N, dw.o, d.H, d.HO, residual));
