@@ -14,10 +14,11 @@
 #include "mla_device.h"
 #include "mla_internal.h"
 
-#include <string.h>
 #include <math.h>
+#include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include <type_traits>
 
@@ -2653,7 +2654,6 @@ __device__ __forceinline__ void row16_max4(float &a, float &b, float &c, float &
         "s_nop 1"
         : "+v"(a), "+v"(b), "+v"(c), "+v"(d));
 }
-
 
 // The three-level quantised weights of this lane's row (rowl) for heads 4g .. 4g+3:
 // v = p * s * wscale in [0, 127] ~= hi + lo/254 + lo2/254^2.

@@ -390,7 +390,10 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
         v4f qv[18];
 #pragma unroll
         for (int j = 0; j < 9; ++j) {
-            const float *p = qrow + (j == 8 ? 512 + 32 * kh + 8 * g : kQ8 ? 256 * kh + 64 * (j >> 1) + 16 * g + 8 * (j & 1) : 32 * (8 * kh + j) + 8 * g);
+            const int col = j == 8 ? 512 + 32 * kh + 8 * g
+                            : kQ8  ? 256 * kh + 64 * (j >> 1) + 16 * g + 8 * (j & 1)
+                                   : 32 * (8 * kh + j) + 8 * g;
+            const float *p = qrow + col;
             qv[2 * j] = *(const v4f *)p * unit;
             qv[2 * j + 1] = *(const v4f *)(p + 4) * unit;
         }
@@ -416,7 +419,8 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                     uint32_t b0 = 0, b1 = 0, b2 = 0;
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        const int v = (int)rintf(__builtin_amdgcn_fmed3f(qv[4 * j + z][y] * qs, -4194304.f, 4194304.f)), v1 = (v + 128) >> 8, v0 = (v1 + 128) >> 8;  // v - 256 v1, v1 - 256 v0: a byte
+                        const int v = (int)rintf(__builtin_amdgcn_fmed3f(qv[4 * j + z][y] * qs, -4194304.f, 4194304.f));
+                        const int v1 = (v + 128) >> 8, v0 = (v1 + 128) >> 8;  // v - 256 v1, v1 - 256 v0: a signed byte each
                         b0 |= (uint32_t)(v0 & 255) << (8 * y);
                         b1 |= (uint32_t)(v1 & 255) << (8 * y);
                         b2 |= (uint32_t)(v & 255) << (8 * y);
@@ -446,13 +450,15 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     if constexpr (kQ8) {
         const int row = 8 * g + (n >> 1);
         tro[0][0] = row * 512 + 16 * ((NC * w) ^ (row & 15)) + 8 * (n & 1);
-    } else
+    } else {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int row = 8 * (NP == 2 ? g & 1 : g) + 4 * h + (n >> 2);
+        for (int h = 0; h < 2; ++h) {
+            const int row = 8 * (NP == 2 ? g & 1 : g) + 4 * h + (n >> 2);
 #pragma unroll
-        for (int t = 0; t < NC; ++t)
-            tro[h][t] = (NP == 2 ? (g >> 1) * Sh::PlaneB : 0) + row * 1024 + 16 * ((2 * (NC * w + t) + ((n >> 1) & 1)) ^ th_swz(row)) + 8 * (n & 1);
+            for (int t = 0; t < NC; ++t)
+                tro[h][t] = (NP == 2 ? (g >> 1) * Sh::PlaneB : 0) + row * 1024 +
+                            16 * ((2 * (NC * w + t) + ((n >> 1) & 1)) ^ th_swz(row)) + 8 * (n & 1);
+        }
     }
     constexpr int SR = Ch / 8;                      // softmax: rows of a thread,
     const int sq = tid >> 3, sr = SR * (tid & 7);  // its query and first row
@@ -950,7 +956,10 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(EARLY ? 2 :
             x0 = x.f0;
             x1 = x.f1;
         } else {
-            auto up = [](uint2 h) { return v4f{__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u), __uint_as_float(h.y << 16), __uint_as_float(h.y & 0xffff0000u)}; };
+            auto up = [](uint2 h) {
+                return v4f{__uint_as_float(h.x << 16), __uint_as_float(h.x & 0xffff0000u), __uint_as_float(h.y << 16),
+                           __uint_as_float(h.y & 0xffff0000u)};
+            };
             x0 = up(x.h0);
             x1 = up(x.h1);
         }
@@ -1159,7 +1168,8 @@ int plan_tree(int fmt, const Dims &d, TreeTable &t, int ncu) {
         for (int b = 0; b < t.n; ++b) n += (t.s[b].count + nm - 1) / nm * splits(t.s[b].ctx, chunks * kThCh);
         return n;
     };
-    t.nm = !kimi ? 0 : 20 * groups(1, 4) + 2L * ncu * kThStart4 < (fmt == kFmtQ8 ? 11 : 12) * groups(1, 2) + 2L * ncu * kThStart2 ? 4 : 2;
+    const long four = 20 * groups(1, 4) + 2L * ncu * kThStart4, two = (fmt == kFmtQ8 ? 11 : 12) * groups(1, 2) + 2L * ncu * kThStart2;
+    t.nm = !kimi ? 0 : four < two ? 4 : 2;
     long best = kThMin / kThCh;  // in chunks
     if (t.nm) {
         const long places = (long)ncu * (t.nm == 2 ? 2 : 1), start = t.nm == 2 ? kThStart2 : kThStart4;

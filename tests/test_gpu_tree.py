@@ -181,6 +181,8 @@ def test_rows_behind_the_tree_stay(models, kind):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dims,lens,sizes", [
     ("lab", [0, 5, 90], [3, 1, 12]),
+    ("lab", [30, 70], [60, 50]),
+    ("nine", [40, 100, 0], [50, 30, 2]),
     ("kimi", [700, 0, 33, 1500, 64], [5, 3, 1, 8, 2]),
     ("kimi", [900, 40, 2000, 300], [64, 30, 40, 1]),
     ("kimi", [100 + 37 * i for i in range(13)], [1] * 13),
