@@ -1936,9 +1936,10 @@ size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &t
 
 // Nodes beyond which a group's q_proj | kv_a and o_proj are products over LDS tiles instead of the decode's GEMVs
 // (in groups of 16 tokens). us, GEMV / tiles: q_proj | kv_a at 12 nodes 7.9 / 9.4, 20 10.1 / 9.1, 64 16.0 / 11.5;
-// o_proj at 64 nodes 11.8 / 6.5 + 5 (the sum of its quarters), 170 29.6 / 11.2 + 5. From host memory the tiles of
-// many workgroups wait for the bus: 24 nodes 14.7 / 21.6, 32 18.0 / 26.0, 48 23.8 / 17.9.
-constexpr int kTreeGemmX = 16, kTreeGemmHost = 32, kTreeGemm = 64;
+// o_proj at 170 nodes 29.6 / 11.2 + 5 (the sum of its quarters), the whole decode with the one or the other
+// at 12 40 / 40, 20 44.4 / 43.1, 32 46.0 / 45.3, 64 55.5 / 52.5. x in host memory: the tiles of many workgroups wait
+// for the bus: q_proj | kv_a at 24 nodes 14.7 / 21.6, 32 18.0 / 26.0, 48 23.8 / 17.9.
+constexpr int kTreeGemm = 16, kTreeGemmHost = 32;
 
 // One tree decode of a launch group: the steps of decode_group with the group's nodes as its
 // members, each member's row at history row ctx + i and its rotation at position ctx + depth.
@@ -1969,7 +1970,7 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         w.ypstride = (size_t)N * ldy;
         StageTimer tm(0);
         // the same partials as products over LDS tiles, those of kv_a bit for bit
-        if (N > (host ? kTreeGemmHost : kTreeGemmX) && d.H == 2048) HIP_TRY(launch_kva_x(st, w.y, w.ypstride, ldy, d_x, N, dw.q, d.QO, dw.kva, d.KVO));
+        if (N > (host ? kTreeGemmHost : kTreeGemm) && d.H == 2048) HIP_TRY(launch_kva_x(st, w.y, w.ypstride, ldy, d_x, N, dw.q, d.QO, dw.kva, d.KVO));
         else HIP_TRY(launch_gemv_ksplit(st, w.y, w.ypstride, ldy, d_x, d.H, N, dw.q, d.QO, dw.kva, d.KVO, d.H));
     } else {
         w.ynp = 1;

@@ -1121,8 +1121,8 @@ __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(EARLY ? 2 :
     }
 }
 
-// Y (+)= the partials of the k quarters in their order, a word of four a thread: 4 to 5 us at 65 to 256 nodes, a
-// launch's latency (10 MB at 256 nodes).
+// Y (+)= the partials of the k quarters in their order, a word of four a thread: 2 us at 20 nodes, 5 at 256 (10 MB),
+// a launch's latency.
 __global__ __launch_bounds__(256) void k_tree_sum(float *Y, const float *P, size_t pstride, size_t n4, int acc) {
     const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
     if (i >= n4) return;
