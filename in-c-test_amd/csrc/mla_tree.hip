@@ -1147,9 +1147,9 @@ hipError_t launch_tree_sum(hipStream_t st, float *Y, const float *P, size_t pstr
 // former, four take kThStart4 / 10 + X4 / CUs and two kThStart2 / 10 + r X2 / (2 CUs), r = 1.2 (Q8 1.1), X the
 // chunks times the workgroups that share them: the lesser is taken. History and combine together, 2 / 4 nodes a
 // workgroup (FP32, BF16, Q8): 400 rows x 7 nodes 20 / 24, 18 / 22, 20 / 26 us; 9000 x 13 43 / 45, 35 / 36, 37 / 40;
-//   32768 x 8 62 / 59, 44 / 44, 45 / 48; 32768 x 16 99 / 90, 62 / 59, 62 / 61; four of 8192 x 16 75 / 73, 49 / 50, 50 /
-//   53; eight of 4096 x 24 100 / 93, 64 / 61, 64 / 64; two of 16384 x 64 259 / 218, 139 / 123, 135 / 125; eight of 32768
-//   x 2 126 / 153, 79 / 87, 61 / 88.
+//   32768 x 8 62 / 59, 44 / 44, 45 / 48; 32768 x 16 99 / 90, 62 / 59, 62 / 61; of several trees, of at most so
+//   many nodes each, four of 8192 x 16 75 / 73, 49 / 50, 50 / 53; eight of 4096 x 24 100 / 93, 64 / 61, 64 / 64; two of
+//   16384 x 64 259 / 218, 139 / 123, 135 / 125; eight of 32768 x 2 126 / 153, 79 / 87, 61 / 88.
 // rows: one chunk a split where that makes at most kThFew workgroups, else a multiple of the chunk, at least
 // kThMin. A launch of k rounds of workgroups takes about k (chunks + start), and the combine about one chunk's
 // time for each kThJoin splits of a sequence: for each k up to kThRounds the fewest rows that make k rounds

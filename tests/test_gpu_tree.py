@@ -414,6 +414,34 @@ def test_layer_form(models, kind, sizes):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("sizes", [[3], [50, 40]])
+def test_layer_form_on_unaligned_buffers(models, kind, sizes):
+    cfg, layer, w = models("kimi")
+    ps = [tree("any", n, 4 + i) for i, n in enumerate(sizes)]
+    states = [State(kind, cfg, 400).load(i, 250 + i) for i in range(len(sizes))]
+    n1, n2 = inputs.normal_bf16(1, "n1", (cfg.hidden_size,), 1.0, 0.1), inputs.normal_bf16(2, "n2", (cfg.hidden_size,), 1.0, 0.1)
+    h = hidden(cfg, 0x67, sum(sizes))
+    u16 = lambda a: trees.abi.ptr(a, C.c_uint16)  # noqa: E731
+    got = []
+    for at in (0, 4):
+        placed = np.full(h.size + 8, 3.5, np.float32)
+        placed[at // 4:at // 4 + h.size] = h.ravel()
+        dh, dn = Device(placed), Device(np.full_like(placed, 3.5))
+        lib.check(fn("attention_layer_%stree_device", kind)(dh.p + at, dn.p + at, ints(sizes), ints(sum(ps, [])), len(sizes), C.byref(cfg),
+                                                           C.byref(w), u16(n1), u16(n2), pointers(states), lib.NO_ADVANCE), "layer")
+        for d in (dh, dn):
+            a = d.get()
+            got.append(a[at // 4:at // 4 + h.size].reshape(h.shape))
+            rest = np.r_[a[:at // 4], a[at // 4 + h.size:]]
+            np.testing.assert_array_equal(rest, 3.5)
+            d.free()
+    for a, b in ((got[0], got[2]), (got[1], got[3])):
+        assert off(b, a.astype(np.float64)) <= 2 * TOL
+    for s in states:
+        s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_captured_tree_replays(models, kind):
     """A graph of the tree call repeats its result on every replay, other work and waits between."""
     cfg, layer, w = models("kimi")
