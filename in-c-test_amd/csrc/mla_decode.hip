@@ -456,9 +456,10 @@ __global__ __launch_bounds__(256) void k_kva_tok(KvaTokArgs a) {
 // hit distinct banks too. Blocks of W's rows alone, whose sums no stored row depends on, keep one running sum
 // for both halves in the MFMA's own accumulator; blocks with rows of W1 (kv_a) add as described. kKvaSum: planes,
 // every block with the one running sum.
-// q_proj | kv_a of trees of 20 / 64 / 170 / 256 nodes (us): k_gemv_ksplit 10.1 / 16.0 / 32 / -, planes and their
-// launch 12.7 / 15.0 / 23.6 / 27, kKvaX 9.1 / 11.5 / 19.0 / 26.8, with every block adding in k order 9.4 / 12.0 / 22.0 /
-// 28; o_proj of 100 / 170 / 256 nodes, kKvaSum 9.3 / 11.2 / 13.4, in k order 11.3 / 14.4 / 16.6.
+// Both read a step's operands a step ahead. q_proj | kv_a of trees of 20 / 64 / 170 / 256 nodes (us): k_gemv_ksplit
+// 10.1 / 16.0 / 32 / -, planes and their launch 12.7 / 15.0 / 23.6 / 27, kKvaX 7.1 / 10.7 / 16.1 / 23.1, without the
+// reads ahead 9.1 / 11.5 / 19.0 / 26.8, with every block adding in k order too 9.4 / 12.0 / 22.0 / 28; o_proj of 100 / 170 / 256
+// nodes, kKvaSum 8.9 / 10.9 / 13.3, in k order 11.3 / 14.4 / 16.6.
 enum { kKvaRows, kKvaX, kKvaSum };
 template <int TU_, int TT_, int WT_, int WR_, int NS_>
 struct KvgShape {
@@ -531,47 +532,87 @@ __global__ __launch_bounds__(Sh::NT) void k_kva_gemm(KvaTokArgs a) {
     v4f sh[TT][TU], sl[TT][TU];
 #pragma unroll
     for (int j = 0; j < NS - 1; ++j) issue(j);
-    auto step = [&](int j, auto one) __attribute__((always_inline)) {  // one: a running sum for both halves
-        // stage j has landed when only the NS - 2 stages after it may still be in flight (a wave
-        // issues NMIN or NMIN + 1 copies per stage; waiting for NMIN each is exact or conservative)
-        if (j + NS - 1 <= 16) wait_vmcnt<(NS - 2) * NMIN>();
-        else wait_vmcnt<0>();
-        lds_barrier();  // also: every wave is done with stage j - 1, refilled next
-        if (j + NS - 1 < 16) issue(j + NS - 1);
-        const uint8_t *st = smem + (j % NS) * STAGE;
+    struct Frags {
         v8bf xh[TU], xl[TU], wv[TT];
+        v4f x0[XF ? TU : 1], x1[XF ? TU : 1];  // fp32 x before it is split
+    };
+    auto read = [&](int j, Frags &f) __attribute__((always_inline)) {
+        const uint8_t *st = smem + (j % NS) * STAGE;
 #pragma unroll
         for (int u = 0; u < TU; ++u) {
             if constexpr (XF) {
-                split8_cvt(*(const v4f *)(st + fx[u]), *(const v4f *)(st + (fx[u] ^ 16)), xh[u], xl[u]);
+                f.x0[u] = *(const v4f *)(st + fx[u]);
+                f.x1[u] = *(const v4f *)(st + (fx[u] ^ 16));
             } else {
-                xh[u] = *(const v8bf *)(st + fx[u]);
-                xl[u] = *(const v8bf *)(st + XPL + fx[u]);
+                f.xh[u] = *(const v8bf *)(st + fx[u]);
+                f.xl[u] = *(const v8bf *)(st + XPL + fx[u]);
             }
         }
 #pragma unroll
-        for (int t = 0; t < TT; ++t) wv[t] = *(const v8bf *)(st + fw[t]);
+        for (int t = 0; t < TT; ++t) f.wv[t] = *(const v8bf *)(st + fw[t]);
+    };
+    auto products = [&](int j, Frags &f, auto one) __attribute__((always_inline)) {  // one: a running sum for both halves
+        if constexpr (XF)
+#pragma unroll
+            for (int u = 0; u < TU; ++u) split8_cvt(f.x0[u], f.x1[u], f.xh[u], f.xl[u]);
         const v4f z = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int t = 0; t < TT; ++t)
 #pragma unroll
             for (int u = 0; u < TU; ++u) {
                 if constexpr (decltype(one)::value) {
-                    sh[t][u] = mfma_bf16(wv[t], xh[u], j == 0 ? z : sh[t][u]);
-                    sh[t][u] = mfma_bf16(wv[t], xl[u], sh[t][u]);
+                    sh[t][u] = mfma_bf16(f.wv[t], f.xh[u], j == 0 ? z : sh[t][u]);
+                    sh[t][u] = mfma_bf16(f.wv[t], f.xl[u], sh[t][u]);
                     sl[t][u] = z;
                     continue;
                 }
-                const v4f rh = mfma_bf16(wv[t], xh[u], z);
-                const v4f rl = mfma_bf16(wv[t], xl[u], z);
+                const v4f rh = mfma_bf16(f.wv[t], f.xh[u], z);
+                const v4f rl = mfma_bf16(f.wv[t], f.xl[u], z);
                 sh[t][u] = j == 0 ? rh : sh[t][u] + rh;
                 sl[t][u] = j == 0 ? rl : sl[t][u] + rl;
             }
     };
     auto steps = [&](auto one) __attribute__((always_inline)) {
-        step(0, one);
+        if constexpr (X == kKvaRows) {
+            auto step = [&](int j) __attribute__((always_inline)) {
+                // stage j has landed when only the NS - 2 stages after it may still be in flight (a wave
+                // issues NMIN or NMIN + 1 copies per stage; waiting for NMIN each is exact or conservative)
+                if (j + NS - 1 <= 16) wait_vmcnt<(NS - 2) * NMIN>();
+                else wait_vmcnt<0>();
+                lds_barrier();  // also: every wave is done with stage j - 1, refilled next
+                if (j + NS - 1 < 16) issue(j + NS - 1);
+                Frags f;
+                read(j, f);
+                products(j, f, one);
+            };
+            step(0);
 #pragma nounroll
-        for (int j = 1; j < 16; ++j) step(j, one);
+            for (int j = 1; j < 16; ++j) step(j);
+        } else {
+            // A step's operands are read a step ahead, beside the products before them.
+            Frags even, odd;
+            auto step = [&](int j, Frags &now, Frags &ahead) __attribute__((always_inline)) {
+                if (j + 1 < 16) {
+                    // stage j + 1 has landed when only the NS - 3 after it may still be in flight
+                    if (j + NS - 2 <= 15) wait_vmcnt<(NS - 3) * NMIN>();
+                    else wait_vmcnt<0>();
+                    lds_barrier();  // also: every wave is done with stage j - 1, refilled next
+                    if (j + NS - 1 < 16) issue(j + NS - 1);
+                    read(j + 1, ahead);
+                }
+                products(j, now, one);
+            };
+            wait_vmcnt<(NS - 2) * NMIN>();
+            lds_barrier();
+            read(0, even);
+            step(0, even, odd);
+            step(1, odd, even);
+#pragma nounroll
+            for (int j = 2; j < 16; j += 2) {
+                step(j, even, odd);
+                step(j + 1, odd, even);
+            }
+        }
     };
     if (X == kKvaSum || (X == kKvaX && row0 + BR <= a.out0)) steps(std::true_type());
     else steps(std::false_type());

@@ -1935,11 +1935,11 @@ size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &t
 }
 
 // Nodes beyond which a group's q_proj | kv_a and o_proj are products over LDS tiles instead of the decode's GEMVs
-// (in groups of 16 tokens). us, GEMV / tiles: q_proj | kv_a at 12 nodes 7.9 / 9.4, 20 10.1 / 9.1, 64 16.0 / 11.5;
-// o_proj at 170 nodes 29.6 / 11.2 + 5 (the sum of its quarters), the whole decode with the one or the other
-// at 12 40 / 40, 20 44.4 / 43.1, 32 46.0 / 45.3, 64 55.5 / 52.5. x in host memory: the tiles of many workgroups wait
-// for the bus: q_proj | kv_a at 24 nodes 14.7 / 21.6, 32 18.0 / 26.0, 48 23.8 / 17.9.
-constexpr int kTreeGemm = 16, kTreeGemmHost = 32;
+// (in groups of 8 and 16 tokens). us, the whole decode over 400 FP32 rows, GEMV / tiles: 5 nodes 33.5 / 34.2, 8
+// 35.3 / 35.0, 9 36.7 / 34.9, 12 37.9 / 34.9, 16 41.1 / 37.1; the projection q_proj | kv_a alone at 64 nodes 16.0 /
+// 10.7, o_proj at 170 nodes 29.6 / 10.9 + 5 (the sum of its quarters). x in host memory: the tiles of many
+// workgroups wait for the bus: the whole call at 12 nodes 63.4 / 65, 24 79 / 83, 32 88 / 94; at 48 the tiles win by 4.
+constexpr int kTreeGemm = 8, kTreeGemmHost = 32;
 
 // One tree decode of a launch group: the steps of decode_group with the group's nodes as its
 // members, each member's row at history row ctx + i and its rotation at position ctx + depth.
