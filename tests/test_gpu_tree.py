@@ -240,6 +240,27 @@ def test_batch_of_large_trees(models, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [9, 16, 17, 32, 33, 63])
+def test_rows_of_any_count_equal_few(models, kind, n):
+    """A node's row does not depend on how many nodes are decoded with it, nor on where x lies."""
+    cfg, layer, w = models("kimi")
+    p, x, ctx = tree("any", n, n), hidden(cfg, 0x60 + n, n), 20
+    rows = []
+    for k in (n, 1, 4, 8):
+        st = State(kind, cfg, ctx + n).load(1, ctx)
+        batch_device(kind, cfg, w, [st], [p[:k]], x[:k])
+        rows.append(st.pull(ctx, ctx + k))
+        st.free()
+    st = State(kind, cfg, ctx + n).load(1, ctx)
+    tree_host(st, layer, x, p, w)
+    rows.append(st.rows(ctx, ctx + n))
+    st.free()
+    for other in rows[1:]:
+        for a, b in zip(rows[0], other):
+            np.testing.assert_array_equal(a[:len(b)], b)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_many_nodes_equal_few(models, kind):
     """The rows of a batch of many nodes are those of its trees alone, bit for bit, and a node that is not
     finite stays within its tree there too."""
@@ -257,6 +278,12 @@ def test_many_nodes_equal_few(models, kind):
         rows = [k for k in range(n) if at + k != 44]
         for a, b in zip(alone.pull(m, m + n), both[i].pull(m, m + n)):
             np.testing.assert_array_equal(a[rows], b[rows])
+        # so are those of the tree's first nodes, which take the projection of few
+        few = State(kind, cfg, m + 8).load(i, m)
+        batch_device(kind, cfg, w, [few], [ps[i][:8]], x[at:at + 8])
+        for a, b in zip(few.pull(m, m + 8), both[i].pull(m, m + 8)):
+            np.testing.assert_array_equal(a[rows[:7]], b[rows[:7]])
+        few.free()
         fine = [k for k in range(n) if at + k != 44 and not (i == 1 and 4 in path_to(ps[1], k))]
         assert off(got[at:at + n][fine], out[fine].astype(np.float64)) <= 2 * TOL
         alone.free()
