@@ -1123,19 +1123,9 @@ __global__ __launch_bounds__(256) void k_rmsnorm(float *y, const float *x, const
 // stack: 6.3 -> 4.7 us per launch (kernel trace), 27 layers 1.73 -> 1.52 ms; bound by two memory
 // round trips and the launch itself.
 template <int NV>
-__global__ __launch_bounds__(256) void k_rmsnorm_reg(float *y, const float *x, const uint16_t *wt, int n, float eps) {
+__device__ __forceinline__ void rmsnorm_row(float *yr, const float (&v)[NV], const uint16_t (&w)[NV], int n, float eps) {
     __shared__ double redd[256];
     const int tid = threadIdx.x, l = tid & 63;
-    const float *xr = x + (size_t)blockIdx.x * n;
-    float *yr = y + (size_t)blockIdx.x * n;
-    float v[NV];
-    uint16_t w[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-        const int k = min(tid + 256 * i, n - 1);
-        v[i] = xr[k];
-        w[i] = wt[k];
-    }
     double ss = 0.0;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -1154,6 +1144,50 @@ __global__ __launch_bounds__(256) void k_rmsnorm_reg(float *y, const float *x, c
         const float u = v[i] * inv;
         if (tid + 256 * i < n) yr[tid + 256 * i] = u * bf16_to_f32(w[i]);
     }
+}
+
+template <int NV>
+__global__ __launch_bounds__(256) void k_rmsnorm_reg(float *y, const float *x, const uint16_t *wt, int n, float eps) {
+    const float *xr = x + (size_t)blockIdx.x * n;
+    float v[NV];
+    uint16_t w[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int k = min((int)threadIdx.x + 256 * i, n - 1);
+        v[i] = xr[k];
+        w[i] = wt[k];
+    }
+    rmsnorm_row(y + (size_t)blockIdx.x * n, v, w, n, eps);
+}
+
+// Y += the kGemvKs partials' sum in their order, y = RMSNorm(Y): k_tree_sum and the norm of a tree's layer in one
+// launch, the same bits as the two. Latency bound: 4.7 us at 49 nodes,
+// the two 3.9 + 3.9.
+template <int NV>
+__global__ __launch_bounds__(256) void k_tree_sum_norm(float *Y, const float *P, size_t pstride, float *y, const uint16_t *wt, int n,
+                                                       float eps) {
+    const size_t row = (size_t)blockIdx.x * n;
+    float v[NV];
+    uint16_t w[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int k = min((int)threadIdx.x + 256 * i, n - 1);
+        float s = P[row + k];
+#pragma unroll
+        for (int q = 1; q < kGemvKs; ++q) s += P[q * pstride + row + k];
+        v[i] = Y[row + k] + s;
+        w[i] = wt[k];
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if ((int)threadIdx.x + 256 * i < n) Y[row + threadIdx.x + 256 * i] = v[i];
+    rmsnorm_row(y + row, v, w, n, eps);
+}
+hipError_t launch_tree_sum_norm(hipStream_t st, float *Y, const float *P, size_t pstride, float *y, const uint16_t *w, int n, int rows,
+                                float eps) {
+    if (n < 1 || n > 256 * 8 || rows < 1) return hipErrorInvalidValue;
+    hipLaunchKernelGGL((k_tree_sum_norm<8>), dim3(rows), dim3(256), 0, st, Y, P, pstride, y, w, n, eps);
+    return hipGetLastError();
 }
 
 hipError_t launch_rmsnorm(hipStream_t st, float *y, const float *x, const uint16_t *w, int n,

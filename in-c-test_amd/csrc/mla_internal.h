@@ -301,6 +301,9 @@ hipError_t launch_tree_combine(hipStream_t st, int fmt, const TreeTable &t, cons
                                const uint16_t *kv_b, const DecodeWork &w);
 // Y[b, o] (+)= the kGemvKs partials' sum in their order, [n] values pstride apart (n % 4 == 0, 16-byte aligned).
 hipError_t launch_tree_sum(hipStream_t st, float *Y, const float *P, size_t pstride, size_t n, bool accumulate);
+// The same with accumulation on rows of n <= 2048, and y = RMSNorm(Y) as launch_rmsnorm has it.
+hipError_t launch_tree_sum_norm(hipStream_t st, float *Y, const float *P, size_t pstride, float *y, const uint16_t *w, int n, int rows,
+                                float eps);
 // Attention of the nodes over all their rows into w.part (nm == 0).
 hipError_t launch_tree_generic(hipStream_t st, int fmt, const TreeTable &t, const TreeNodes &nd, const Dims &d,
                                const DecodeWork &w);

@@ -1941,17 +1941,26 @@ size_t tree_plan(int fmt, const Dims &d, const TreeIn *seqs, int n, TreeTable &t
 // workgroups wait for the bus: the whole call at 12 nodes 63.4 / 65, 24 79 / 83, 32 88 / 94; at 48 the tiles win by 4.
 constexpr int kTreeGemm = 8, kTreeGemmHost = 32;
 
+// RMSNorm of a layer's outputs into another buffer.
+struct OutNorm {
+    const uint16_t *w;
+    float *out;
+};
+
 // One tree decode of a launch group: the steps of decode_group with the group's nodes as its
 // members, each member's row at history row ctx + i and its rotation at position ctx + depth.
 // Everything it needs has been acquired (tree_prepare). host: d_x and d_out are pinned host memory.
 int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights &dw, const TreeIn *seqs, int n, bool tokens,
-               const float *d_x, float *d_out, bool residual, DecodeWork &w, bool host, const InNorm *in_norm = nullptr) {
+               const float *d_x, float *d_out, bool residual, DecodeWork &w, bool host, const InNorm *in_norm = nullptr,
+               const OutNorm *out_norm = nullptr) {
     Ctx &c = ctx();
     hipStream_t st = c.stream;
     if (tokens) {
         SeqIn one[kMaxBatch];
         for (int b = 0; b < n; ++b) one[b] = {seqs[b].m, seqs[b].ctx};
-        return decode_group(fmt, d, eps, theta, dw, one, n, d_x, d_out, residual, w, false, 0, in_norm);
+        if (decode_group(fmt, d, eps, theta, dw, one, n, d_x, d_out, residual, w, false, 0, in_norm) != 0) return -1;
+        if (out_norm) HIP_TRY(launch_rmsnorm(st, out_norm->out, d_out, out_norm->w, d.H, n, eps));
+        return 0;
     }
     TreeTable tt;
     const size_t part_bytes = tree_plan(fmt, d, seqs, n, tt);
@@ -2032,10 +2041,15 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         if (N > kTreeGemm && gemv_ksplit_ok(d.H, d.H) && d.H <= ldy && d.H % 4 == 0 && (uintptr_t)d_out % 16 == 0) {  // partials in the place of w.y
             const size_t ps = (size_t)N * d.H;
             HIP_TRY(launch_kva_sum(st, w.y, ps, w.hos, w.hos + (size_t)N * d.HO, N, dw.o, d.H));
+            if (out_norm && residual && d.H <= 2048) {
+                HIP_TRY(launch_tree_sum_norm(st, d_out, w.y, ps, out_norm->out, out_norm->w, d.H, N, eps));
+                return 0;
+            }
             HIP_TRY(launch_tree_sum(st, d_out, w.y, ps, ps, residual));
         } else {
             HIP_TRY(launch_gemv_xs(st, d_out, d.H, w.hos, N, dw.o, d.H, d.HO, residual));
         }
+        if (out_norm) HIP_TRY(launch_rmsnorm(st, out_norm->out, d_out, out_norm->w, d.H, N, eps));
         return 0;
     }
     {
@@ -2064,6 +2078,7 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
         else
             HIP_TRY(launch_gemv(st, d_out + (size_t)k0 * d.H, d.H, wk.ho, d.HO, t.n, dw.o, d.H, nullptr, 0, d.HO, residual));
     }
+    if (out_norm) HIP_TRY(launch_rmsnorm(st, out_norm->out, d_out, out_norm->w, d.H, N, eps));
     return 0;
 }
 
@@ -2201,7 +2216,7 @@ int tree_host(float *out, const float *x, const int *parents, int count, int sta
 // Stream-ordered tree decode of a batch over device buffers.
 template <class S>
 int tree_device(float *d_out, const float *d_x, const int *counts, const int *parents, int batch, const KvlMlaConfig *cfg,
-                const KvlMlaBF16 *w, S *const *states, unsigned flags, const InNorm *in_norm = nullptr) {
+                const KvlMlaBF16 *w, S *const *states, unsigned flags, const InNorm *in_norm = nullptr, const OutNorm *out_norm = nullptr) {
     Dims d;
     if (!d_out || !d_x || !counts || !parents || batch <= 0 || !states || !weights_ok(w) || !dims_of(cfg, d)) {
         set_err("invalid arguments");
@@ -2228,8 +2243,10 @@ int tree_device(float *d_out, const float *d_x, const int *counts, const int *pa
         for (int i = g; i < e; ++i) n += counts[i];
         DecodeWork wk;
         if (decode_work(d, n, (int)rb, wk) != 0) return -1;
-        if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data() + g, e - g, tokens, d_x + at * d.H,
-                       d_out + at * d.H, (flags & KVL_MLA_RESIDUAL) != 0, wk, false, in_norm) != 0)
+        OutNorm on{};
+        if (out_norm) on = {out_norm->w, out_norm->out + at * d.H};
+        if (tree_group(fmt, d, cfg->rms_eps, cfg->rope_theta, dw, in.data() + g, e - g, tokens, d_x + at * d.H, d_out + at * d.H,
+                       (flags & KVL_MLA_RESIDUAL) != 0, wk, false, in_norm, out_norm ? &on : nullptr) != 0)
             return -1;
         if (!(flags & KVL_MLA_NO_ADVANCE))
             for (int i = g; i < e; ++i) {
@@ -2274,9 +2291,8 @@ int attention_layer_tree(float *d_h, float *d_n2, const int *counts, const int *
         if (dev_reserve(c.layer, need) != 0) return -1;
     }
     const InNorm in{din, (float *)c.layer.p};
-    if (tree_device(d_h, d_h, counts, parents, batch, cfg, w, states, flags | KVL_MLA_RESIDUAL, &in) != 0) return -1;
-    HIP_TRY(launch_rmsnorm(c.stream, d_n2, d_h, dpost, d.H, rows, cfg->rms_eps));
-    return 0;
+    const OutNorm out{dpost, d_n2};
+    return tree_device(d_h, d_h, counts, parents, batch, cfg, w, states, flags | KVL_MLA_RESIDUAL, &in, &out);
 }
 
 // ---------------------------------------------------------------- rows ------------------
