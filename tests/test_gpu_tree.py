@@ -411,10 +411,10 @@ def test_long_histories_of_zero_rows(models, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("sizes", [[4], [9, 1, 30], [60, 50]])
+@pytest.mark.parametrize("sizes", [[4], [9, 1, 30], [60, 50], [1, 1, 1], [64, 64, 64, 63, 60]])
 def test_layer_form(models, kind, sizes):
     cfg, layer, w = models("kimi")
-    lens = [333, 20, 800][:len(sizes)]
+    lens = [333, 20, 800, 50, 0][:len(sizes)]
     ps = [tree("any", n, 7 + i) for i, n in enumerate(sizes)]
     states = [State(kind, cfg, m + n).load(i, m) for i, (m, n) in enumerate(zip(lens, sizes))]
     n1, n2 = inputs.normal_bf16(1, "n1", (cfg.hidden_size,), 1.0, 0.1), inputs.normal_bf16(2, "n2", (cfg.hidden_size,), 1.0, 0.1)
