@@ -140,8 +140,8 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 // 2^9 splits of them can still be added.
 // What bounds it: the issue of matrix and vector instructions beside each other. 64 nodes x 32768 Q8 rows: 144 us,
 // 1.04 PFLOP/s of operand products of 16 bits' worth (two per product of the formula) where the library's large
-// bf16 product reaches 1.19; 129 us with rows of zeros, whose products draw less power. The start of a workgroup
-// (table, queries, first chunk, the first pass) is worth 8 us of it, with NM = 2 5.
+// bf16 product reaches 1.19; 129 us with rows of zeros, whose products draw less power. A launch of one chunk a
+// workgroup (table, queries, chunk, the passes that fill the pipe) takes 8 to 10 us with NM = 2, 12 to 16 with NM = 4.
 constexpr int kThCh = 32;  // rows of a chunk (FP32: of two)
 template <int FMT, int NM>
 struct ThShape {
