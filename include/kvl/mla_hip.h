@@ -237,7 +237,7 @@ int kvl_mla_prefill_compressed_bf16_state_device(float *d_out, const float *d_x,
  * is row n + i, and it attends rows [0, n), the rows of its ancestors and its own; rows of other
  * branches do not enter, whatever they hold. A tree of one node is a single-token decode, a chain a
  * block decode: the appended rows equal theirs bit for bit, the outputs up to the order of
- * summation.
+ * summation (over Q8 rows also up to those decodes' 15-bit query; a tree's has 22).
  * After a tree decode len = n + count: *_accept keeps one path's rows, *_truncate(state, n) drops
  * the draft. Until then rows n .. n + count - 1 are the tree's, in node order, not a continuation.
  *
@@ -255,8 +255,8 @@ int kvl_mla_decode_compressed_q8_tree_bf16(float *out, const float *x, const int
 /* Stream-ordered, a batch of sequences each with its own tree, over device buffers: tree b has
  * counts[b] nodes (1 .. 64); the nodes of all trees stand one tree after another in parents (host,
  * within-tree indices), d_x and d_out ([sum of counts, hidden] fp32). flags as the batch decodes:
- * KVL_MLA_RESIDUAL, and KVL_MLA_NO_ADVANCE (rows written at len + i, len left). counts and parents
- * are read during the call only; no state may stand twice. The appended rows stay on the device.
+ * KVL_MLA_RESIDUAL, and KVL_MLA_NO_ADVANCE (rows written at len + i, len left: they are not the
+ * state's, *_accept needs a call without the flag). counts and parents are read during the call only; no state may stand twice. The appended rows stay on the device.
  * Capturable once warm (trees, lengths and buffers are the captured ones). */
 int kvl_mla_decode_compressed_tree_batch_device(float *d_out, const float *d_x, const int *counts,
                                                    const int *parents, int batch, const KvlMlaConfig *cfg,
