@@ -2021,7 +2021,7 @@ int tree_group(int fmt, const Dims &d, float eps, float theta, const DevWeights 
             }
             DecodeWork wk = w;
             wk.y += (size_t)k0 * ldy;
-            wk.qf += (size_t)k0 * d.NH * std::max(d.R + d.DR, d.QD);
+            wk.qf += (size_t)k0 * d.NH * (d.R + d.DR);  // a query's stride, where the workspace has room for QD too
             wk.rows += (size_t)k0 * rb;
             StageTimer tm(1);
             HIP_TRY(launch_append_qprep(st, fmt, t, d, wk.y, ldy, d.QO, w.ynp, w.ypstride, dw.norm, eps, cs, dw.kvb, dw.ukt, wk,
