@@ -133,16 +133,22 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 // is left out is below 2^-17 of an operand).
 // Q8: the scores are int8 products of the codes as stored and the query as a whole number below 2^22 (a power of
 // two times it) in three bytes, exact but for that rounding; a row's scale and the query's power multiply the
-// sum. The mix takes the codes as fp16 (exact) and the weights in two fp16 parts, 22 bits; a row's scale
-// multiplies its weight. To keep the weights within fp16 whatever the scales, the running maximum is that of score
-// + the scale's exponent (in units of log2), so that weight times scale stays <= 64. An exponent below -93
-// counts as -93 there: over kThMax rows of scale zero the sum of the weights stays below 2^(6 + 93 + 19), and
-// 2^9 splits of them can still be added.
+// sum. The mix takes the codes as fp16 (exact) and the weights in two fp16 parts; a row's scale multiplies its
+// weight. To keep the weights within fp16 whatever the scales, the running maximum is that of score + the scale's
+// exponent (in units of log2); the reference lies kThLow below it, so that weight times scale stays below 2^15 and
+// fp16's smallest step, 2^-24, is 2^-32 of the largest weight. Both parts round to nearest: where one row outweighs
+// many small ones, a loss that is always downward adds up over them, and the lo parts of the small ones, which a
+// matrix instruction drops (it adds at most eight rows at a time) beside a sum 2^25 times theirs, are as often negative. Eight trees,
+// one row of about 0.6 of the weight, latents with a common mean: an output of 32768 / 131072 rows (a quarter of them a
+// split) is off by 3.5e-6 / 3.3e-6; parts cut toward zero 9e-6 / 2.9e-5, with the reference at the maximum too 1.6e-4 /
+// 5.8e-4. An exponent below -84 counts as -84 there: over kThMax rows of scale zero the sum of the weights stays below
+// 2^(15 + 84 + 19), and 2^9 splits of them can still be added.
 // What bounds it: the issue of matrix and vector instructions beside each other. 64 nodes x 32768 Q8 rows: 144 us,
 // 1.04 PFLOP/s of operand products of 16 bits' worth (two per product of the formula) where the library's large
 // bf16 product reaches 1.19; 129 us with rows of zeros, whose products draw less power. A launch of one chunk a
 // workgroup (table, queries, chunk, the passes that fill the pipe) takes 8 to 10 us with NM = 2, 12 to 16 with NM = 4.
 constexpr int kThCh = 32;  // rows of a chunk (FP32: of two)
+constexpr float kThLow = 9.0f;  // Q8: the reference of the weights below the running maximum, log2
 template <int FMT, int NM>
 struct ThShape {
     static constexpr int NW = 2 * NM, NT = 64 * NW, NQ = 16 * NM;
@@ -248,15 +254,14 @@ __device__ __forceinline__ v4i codes_f16(const v2i &c) {
     return v4i{(int)o[0], (int)o[1], (int)o[2], (int)o[3]};
 }
 
-// Four weights as hi and lo halves. fp16: both cut toward zero (one instruction per pair), what is left
-// out is below 2^-20 of the weight.
+// Four weights as hi and lo halves, rounded to nearest: what is left out is at most 2^-17 of the weight (bf16) or 2^-23
+// (fp16; 2^-25 absolute where that is more, below a weight of 1/4).
 template <bool F16>
 __device__ __forceinline__ void th_split4(const v4f &x, int2 &hi, int2 &lo) {
     if constexpr (F16) {
-        const v2h h0 = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[0], x[1]));
-        const v2h h1 = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[2], x[3]));
-        const v2h l0 = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[0] - (float)h0.x, x[1] - (float)h0.y));
-        const v2h l1 = __builtin_bit_cast(v2h, __builtin_amdgcn_cvt_pkrtz(x[2] - (float)h1.x, x[3] - (float)h1.y));
+        const v2h h0 = __builtin_convertvector((v2f{x[0], x[1]}), v2h), h1 = __builtin_convertvector((v2f{x[2], x[3]}), v2h);
+        const v2h l0 = __builtin_convertvector((v2f{x[0] - (float)h0.x, x[1] - (float)h0.y}), v2h);
+        const v2h l1 = __builtin_convertvector((v2f{x[2] - (float)h1.x, x[3] - (float)h1.y}), v2h);
         hi = int2{__builtin_bit_cast(int, h0), __builtin_bit_cast(int, h1)};
         lo = int2{__builtin_bit_cast(int, l0), __builtin_bit_cast(int, l1)};
     } else {
@@ -585,9 +590,10 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
             vsr t = sx;
             if constexpr (kQ8)
 #pragma unroll
-                for (int e = 0; e < SR; ++e) t[e] += (float)max(__builtin_amdgcn_frexp_expf(sr4[e]), -93);
+                for (int e = 0; e < SR; ++e) t[e] += (float)max(__builtin_amdgcn_frexp_expf(sr4[e]), -84);
             cm = fmaxf(t[0], t[1]);
             if constexpr (SR == 4) cm = fmaxf(cm, fmaxf(t[2], t[3]));
+            if constexpr (kQ8) cm -= kThLow;
             cm = fmaxf(cm, dpp_f32<0xB1>(cm));
         } else if (piece == 1) {
             cm = fmaxf(cm, dpp_f32<0x4E>(cm));
