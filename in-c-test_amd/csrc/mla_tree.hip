@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 // sum. The mix takes the codes as fp16 (exact) and the weights in two fp16 parts; a row's scale multiplies its
 // weight. To keep the weights within fp16 whatever the scales, the running maximum is that of score + the scale's
 // exponent (in units of log2); the reference lies kThLow below it, so that weight times scale stays below 2^15 and
-// fp16's smallest step, 2^-24, is 2^-32 of the largest weight. Both parts round to nearest: where one row outweighs
+// fp16's smallest step, 2^-24, is 2^-30 of the largest weight. Both parts round to nearest: where one row outweighs
 // many small ones, a loss that is always downward adds up over them, and the lo parts of the small ones, which a
 // matrix instruction drops (it adds at most eight rows at a time) beside a sum 2^25 times theirs, are as often negative. Eight trees,
 // one row of about 0.6 of the weight, latents with a common mean: an output of 32768 / 131072 rows (a quarter of them a
@@ -148,7 +148,9 @@ __global__ __launch_bounds__(256) void k_tree_generic(TreeNodeArgs a) {
 // bf16 product reaches 1.19; 129 us with rows of zeros, whose products draw less power. A launch of one chunk a
 // workgroup (table, queries, chunk, the passes that fill the pipe) takes 8 to 10 us with NM = 2, 12 to 16 with NM = 4.
 constexpr int kThCh = 32;  // rows of a chunk (FP32: of two)
-constexpr float kThLow = 9.0f;  // Q8: the reference of the weights below the running maximum, log2
+// Q8: the reference of the weights lies kThLow below the maximum that moves it (rounded: at most 8, whatever the size of
+// the logits), which a later maximum may pass by kThTop.
+constexpr float kThLow = 7.0f, kThTop = 15.0f;
 template <int FMT, int NM>
 struct ThShape {
     static constexpr int NW = 2 * NM, NT = 64 * NW, NQ = 16 * NM;
@@ -593,15 +595,16 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
                 for (int e = 0; e < SR; ++e) t[e] += (float)max(__builtin_amdgcn_frexp_expf(sr4[e]), -84);
             cm = fmaxf(t[0], t[1]);
             if constexpr (SR == 4) cm = fmaxf(cm, fmaxf(t[2], t[3]));
-            if constexpr (kQ8) cm -= kThLow;
             cm = fmaxf(cm, dpp_f32<0xB1>(cm));
         } else if (piece == 1) {
             cm = fmaxf(cm, dpp_f32<0x4E>(cm));
             cm = fmaxf(cm, dpp_f32<0x141>(cm));  // row_half_mirror: the other four of the eight
-            const bool mv = cm > m_run + 6.0f;
+            // as differences, exact where they decide: of logits past 2^24 sums would round by more than 1
+            const bool mv = cm - m_run > (kQ8 ? kThTop : 6.0f);
+            const float to = kQ8 ? cm - kThLow : cm;
             moved = __any(mv);
-            alpha = mv ? __builtin_amdgcn_exp2f(m_run - cm) : 1.0f;
-            m_run = mv ? cm : m_run;
+            alpha = mv ? __builtin_amdgcn_exp2f(m_run - to) : 1.0f;
+            m_run = mv ? to : m_run;
         } else if (piece == 2) {
 #pragma unroll
             for (int e = 0; e < SR; ++e) sp4[e] = __builtin_amdgcn_exp2f(sx[e] - m_run);

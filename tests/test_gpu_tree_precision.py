@@ -36,6 +36,16 @@ def latent_queries(cfg, layer, x):
     return np.stack([np.matmul(kvb[h, :DN].T, q[:, h, :DN].T).T for h in range(NH)], 1) / np.sqrt(DN + DR)
 
 
+def rope_scores(cfg, layer, x, keys, pos):
+    """[count, heads]: what the rotated query of each node, at one position, scores against its own key."""
+    NH, DN, DR = cfg.num_heads, cfg.qk_nope_dim, cfg.qk_rope_dim
+    q = (x.astype(np.float64) @ f64(layer.q_proj).T).reshape(-1, NH, DN + DR)
+    a = pos * cfg.rope_theta ** (-2.0 * np.arange(DR // 2) / DR)
+    e, o = q[..., DN::2], q[..., DN + 1::2]
+    qr = np.concatenate([e * np.cos(a) - o * np.sin(a), o * np.cos(a) + e * np.sin(a)], -1)
+    return (qr * keys[:, None]).sum(-1) / np.sqrt(DN + DR)
+
+
 def put_rows(st, lat, key):
     """The state's rows become these, rounded to its format."""
     n, a = len(lat), st.arrays()
@@ -219,3 +229,39 @@ def test_q8_rows_of_the_smallest_scales(models):  # noqa: F811
         assert relative(got[b][some], want) <= 2 * NEAR
     for s in states:
         s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_logits_past_the_integers(models, kind):  # noqa: F811
+    """Logits of 2^24 to 2^30 (in steps of the reference's own rounding: 2 to 128), equal over the history's rows,
+    whose scale lies just below a power of two: the weights stay finite. Each head takes the history's row or the
+    best of the node's path; nodes whose heads do that by a margin of 2^-8 of the logit are compared."""
+    cfg, layer, w = models("kimi")
+    ctx, n = 100, 24
+    rng = np.random.default_rng(6)
+    lat = rng.integers(-127, 128, cfg.kv_lora_rank).astype(np.float64)
+    lat[0] = 127
+    st = State(kind, cfg, ctx + n)
+    put_rows(st, np.tile(lat, (ctx, 1)), np.zeros((ctx, cfg.qk_rope_dim)))
+    if kind == "q8":
+        st.arrays()[1][:ctx] = np.float32(2 - 2.0 ** -23)
+        lib.check(fn("compressed_%sstate_sync", kind)(st.ref()), "sync")
+    compared = 0
+    for e in range(18, 28):
+        x = (hidden(cfg, 0xE6, n) * np.float32(2.0 ** e)).astype(np.float32)
+        p = [-1] * n
+        got = tree_host(st, layer, x, p, w)
+        assert np.isfinite(got).all(), e
+        rows = st.rows(0, ctx + n)
+        want = reference(cfg, layer, x, p, ctx, rows, kind)
+        hist, own = trees.values(rows, kind)[0][[0]], trees.values(rows, kind)[0][ctx:]
+        q = latent_queries(cfg, layer, x)
+        a = np.matmul(q, hist.T)[:, :, 0]
+        b = np.stack([q[i] @ own[i] for i in range(n)]) + rope_scores(cfg, layer, x, trees.values(rows, kind)[1][ctx:], ctx)
+        for i in range(n):
+            if (np.abs(a[i] - b[i]) > 2.0 ** -8 * np.abs(a[i]) + 64).all():
+                compared += 1
+                assert relative(got[i:i + 1], want[i:i + 1]) <= NEAR, (e, i)
+        lib.check(fn("compressed_%sstate_truncate", kind)(st.ref(), ctx), "truncate")
+    assert compared > 20
+    st.free()
