@@ -2365,6 +2365,24 @@ int fork_rows(S *const *dsts, S *const *srcs, const int *row0, const int *row1, 
     }
     ForkTable t;
     memset(&t, 0, sizeof t);
+    int done = 0;
+    auto taken = [&](int end) {  // the copies of pairs [done, end) are queued, of a host call they have ended
+        for (int i = done; i < end; ++i) {
+            if (host) {
+                const HostView vs = view_of(srcs[i]), vd = view_of(dsts[i]);
+                int e[3];
+                void *p[3];
+                comps_of(*ms[i], e, p);
+                for (int k = 0; k < 3; ++k)
+                    if (e[k])
+                        memcpy((char *)host_comp(vd, k) + (size_t)row0[i] * e[k], (const char *)host_comp(vs, k) + (size_t)row0[i] * e[k],
+                               (size_t)(row1[i] - row0[i]) * e[k]);
+            }
+            dsts[i]->len = row1[i];
+            md[i]->synced = row1[i];
+        }
+        done = end;
+    };
     for (int i = 0; i < n; ++i) {
         if (row1[i] > row0[i]) {
             ForkDesc &f = t.d[t.n++];
@@ -2379,23 +2397,11 @@ int fork_rows(S *const *dsts, S *const *srcs, const int *row0, const int *row1, 
         if (t.n == kForkBatch || (i == n - 1 && t.n > 0)) {
             HIP_TRY(launch_fork(c.stream, t));
             t.n = 0;
+            if (!host) taken(i + 1);
         }
     }
     if (host) HIP_TRY(hipStreamSynchronize(c.stream));  // also: the uploads above have read the host rows
-    for (int i = 0; i < n; ++i) {
-        if (host) {
-            const HostView vs = view_of(srcs[i]), vd = view_of(dsts[i]);
-            int e[3];
-            void *p[3];
-            comps_of(*ms[i], e, p);
-            for (int k = 0; k < 3; ++k)
-                if (e[k])
-                    memcpy((char *)host_comp(vd, k) + (size_t)row0[i] * e[k], (const char *)host_comp(vs, k) + (size_t)row0[i] * e[k],
-                           (size_t)(row1[i] - row0[i]) * e[k]);
-        }
-        dsts[i]->len = row1[i];
-        md[i]->synced = row1[i];
-    }
+    taken(n);
     return 0;
 }
 
@@ -2444,6 +2450,27 @@ int accept_rows(S *const *states, const int *starts, const int *counts, const in
         if (mirror_get(states[i], view_of(states[i]), &ms[i]) != 0) return -1;
     AcceptTable t;
     memset(&t, 0, sizeof t);
+    int done = 0;
+    size_t done_at = 0;
+    auto taken = [&](int end) {  // the moves of states [done, end) are queued, of a host call they have ended
+        for (int i = done; i < end; ++i) {
+            if (host) {
+                const HostView v = view_of(states[i]);
+                int e[3];
+                void *p[3];
+                comps_of(*ms[i], e, p);
+                for (int j = 0; j < counts[i]; ++j)
+                    for (int k = 0; k < 3; ++k)
+                        if (e[k] && paths[done_at + j] != j)
+                            memcpy((char *)host_comp(v, k) + (size_t)(starts[i] + j) * e[k],
+                                   (const char *)host_comp(v, k) + (size_t)(starts[i] + paths[done_at + j]) * e[k], (size_t)e[k]);
+            }
+            states[i]->len = starts[i] + counts[i];
+            ms[i]->synced = states[i]->len;
+            done_at += (size_t)counts[i];
+        }
+        done = end;
+    };
     at = 0;
     for (int i = 0; i < batch; ++i) {
         const int *path = paths + at;
@@ -2459,27 +2486,12 @@ int accept_rows(S *const *states, const int *starts, const int *counts, const in
         if (t.n == kAcceptBatch || (i == batch - 1 && t.n > 0)) {
             HIP_TRY(launch_accept(c.stream, t));
             t.n = 0;
+            if (!host) taken(i + 1);
         }
         at += (size_t)counts[i];
     }
     if (host) HIP_TRY(hipStreamSynchronize(c.stream));
-    at = 0;
-    for (int i = 0; i < batch; ++i) {
-        if (host) {
-            const HostView v = view_of(states[i]);
-            int e[3];
-            void *p[3];
-            comps_of(*ms[i], e, p);
-            for (int j = 0; j < counts[i]; ++j)
-                for (int k = 0; k < 3; ++k)
-                    if (e[k] && paths[at + j] != j)
-                        memcpy((char *)host_comp(v, k) + (size_t)(starts[i] + j) * e[k],
-                               (const char *)host_comp(v, k) + (size_t)(starts[i] + paths[at + j]) * e[k], (size_t)e[k]);
-        }
-        states[i]->len = starts[i] + counts[i];
-        ms[i]->synced = states[i]->len;
-        at += (size_t)counts[i];
-    }
+    taken(batch);
     return 0;
 }
 

@@ -240,6 +240,9 @@ int kvl_mla_prefill_compressed_bf16_state_device(float *d_out, const float *d_x,
  * summation (over Q8 rows also up to those decodes' 15-bit query; a tree's has 22).
  * After a tree decode len = n + count: *_accept keeps one path's rows, *_truncate(state, n) drops
  * the draft. Until then rows n .. n + count - 1 are the tree's, in node order, not a continuation.
+ * A refused call changes nothing. Where a batched call (*_batch_device, *_tree_device) fails at a
+ * launch, the states of the launches before it are done, which their len says, and the others hold
+ * the rows [0, len) of before.
  *
  * Host buffers, one sequence: out, x [count, hidden]; start_position must equal len. Synchronous;
  * host rows written. */
