@@ -20,8 +20,6 @@
 #include <algorithm>
 #include <type_traits>
 
-#include <type_traits>
-
 namespace kvl {
 
 // ================================================================ GEMV =================
@@ -1537,8 +1535,7 @@ __global__ __launch_bounds__(256) void k_append_qprep(SeqTable t, Dims d, Append
     else if (qa.quarter) {
         const int lane_pos = t.s[threadIdx.x & 63].pos;
         qprep_quarter(t.n, [&](int b) { return __shfl(lane_pos, b); }, qa, blockIdx.x - na, d.NH);
-    }
-    else qprep_body(t, d, qa, blockIdx.x - na);
+    } else qprep_body(t, d, qa, blockIdx.x - na);
 }
 
 static QprepArgs qprep_args(int fmt, const Dims &d, const uint16_t *kv_b, const uint16_t *ukt,
@@ -1875,6 +1872,10 @@ constexpr int kB16SpHs = 36;                       // floats per head in a score
 constexpr int kB16SpOff = kB16Ring * kB16Slot;     // score halves [2][16 heads][kB16SpHs]
 constexpr int kB16SmemB = kB16SpOff + 2 * 16 * kB16SpHs * 4;
 static_assert(kB16SmemB <= 160 * 1024, "LDS of one CU");
+
+// bits (r3, r2, r1, r0) of a chunk row -> slot XOR (r3, r1, r0, r2): a bijection on 16 rows, and
+// (r3, r1, r0) -> distinct slot pairs for the 8 rows of a transposed half-wave read
+__device__ __forceinline__ int b16_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8); }
 
 // Max / sum over lanes l, l ^ 16, l ^ 32, l ^ 48 with the gfx950 lane-swap instructions (VALU,
 // no LDS round trip): v_permlane16_swap with both operands v gives every lane the values of its

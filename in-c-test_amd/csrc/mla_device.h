@@ -308,12 +308,6 @@ __device__ __forceinline__ void wait_vmcnt() {
 // Workgroup barrier after this wave's LDS writes have completed.
 __device__ __forceinline__ void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-// 16-byte slots of a 1 KB latent row in LDS, XOR-swizzled so that the score reads (16 rows, one slot)
-// and the transposed reads (4 rows x 32 bytes per 16 lanes) spread over the banks:
-// bits (r3, r2, r1, r0) of a chunk row -> slot XOR (r3, r1, r0, r2): a bijection on 16 rows, and
-// (r3, r1, r0) -> distinct slot pairs for the 8 rows of a transposed half-wave read
-__device__ __forceinline__ int b16_swz(int row) { return ((row & 3) << 1) | ((row >> 2) & 1) | (row & 8); }
-
 typedef int v2i __attribute__((ext_vector_type(2)));
 // ds_read_b64_tr_b8: within each 16-lane group, destination lane j byte i comes from the
 // 8 bytes addressed by source lane 2i + (j >> 3), at byte j & 7.
