@@ -1,5 +1,6 @@
 """Tree decodes at dims whose nope dim is larger than the latent rank (a head's projected query is then longer
 than the row it is scored against), more nodes in a launch than a slice of them takes."""
+import numpy as np
 import pytest
 
 import trees
@@ -57,6 +58,34 @@ def test_batch_at_other_dims(kind, dims, lens, sizes):
     for i, (m, n) in enumerate(zip(lens, sizes)):
         e = off(got[at:at + n], reference(cfg, layer, x[at:at + n], ps[i], m, states[i].pull(0, m + n), kind))
         assert e <= TOL, (i, m, n, e)
+        at += n
+    for s in states:
+        s.free()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dims", [dict(trees.KIMI, num_heads=64), dict(trees.KIMI, hidden_size=4096)], ids=["heads64", "hidden4096"])
+def test_batch_of_large_projections(kind, dims):
+    """Projections of so many rows that their largest tiles are taken; the rows are a decode's of few nodes."""
+    cfg = inputs.config(**dims)
+    layer = inputs.fast_layer(cfg, 0x80)
+    w = layer.struct()
+    sizes, lens = [64, 64, 64, 63], [20, 50, 0, 33]
+    ps = [tree("any", n, i) for i, n in enumerate(sizes)]
+    states = [State(kind, cfg, m + n).load(i, m) for i, (m, n) in enumerate(zip(lens, sizes))]
+    x = hidden(cfg, 0x57, sum(sizes))
+    got = batch_device(kind, cfg, w, states, ps, x)
+    at = 0
+    for i, (m, n) in enumerate(zip(lens, sizes)):
+        rows = states[i].pull(0, m + n)
+        some = [0, 1, n // 2, n - 1]
+        e = off(got[at:at + n][some], reference(cfg, layer, x[at:at + n], ps[i], m, rows, kind, some))
+        assert e <= TOL, (i, m, n, e)
+        few = State(kind, cfg, m + 8).load(i, m)
+        batch_device(kind, cfg, w, [few], [ps[i][:8]], x[at:at + 8])
+        for a, b in zip(few.pull(m, m + 8), rows):
+            np.testing.assert_array_equal(a, b[m:m + 8])
+        few.free()
         at += n
     for s in states:
         s.free()
