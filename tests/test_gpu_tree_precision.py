@@ -76,8 +76,12 @@ def test_first_row_that_draws_much_of_the_weight(models, kind, ctx):  # noqa: F8
     """The usual history of a trained model: its first token draws more than half of the attention, and the latents
     share a mean, so that what is lost of the many small weights adds up. Eight trees of 32 nodes, so that a split
     holds a quarter of the history. NEAR, and as much again for the sums over a split: two additions per chunk of
-    32 rows and eight of its rows at a time, each off by 2^-25 of the sum in the mean and not always up or down."""
+    32 rows and eight of its rows at a time, each off by 2^-25 of the sum in the mean and not always up or down.
+    A rope_theta of its own past 65536 rows: the table of the usual one grows with the positions, and other tests
+    count on positions that it does not reach."""
     cfg, layer, w = models("kimi")
+    if ctx > 65536:
+        cfg = inputs.config(**dict(trees.KIMI, rope_theta=30000.0))
     n, batch = 32, 8
     rng = np.random.default_rng(ctx)
     base = 4 * hidden(cfg, 0xE1, 1)
