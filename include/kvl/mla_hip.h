@@ -259,8 +259,9 @@ int kvl_mla_decode_compressed_q8_tree_bf16(float *out, const float *x, const int
  * counts[b] nodes (1 .. 64); the nodes of all trees stand one tree after another in parents (host,
  * within-tree indices), d_x and d_out ([sum of counts, hidden] fp32). flags as the batch decodes:
  * KVL_MLA_RESIDUAL, and KVL_MLA_NO_ADVANCE (rows written at len + i, len left: they are not the
- * state's, *_accept needs a call without the flag). counts and parents are read during the call only; no state may stand twice. The appended rows stay on the device.
- * Capturable once warm (trees, lengths and buffers are the captured ones). */
+ * state's, *_accept needs a call without the flag). counts and parents are read during the call
+ * only; no state may stand twice. The appended rows stay on the device. Capturable once warm
+ * (trees, lengths and buffers are the captured ones). */
 int kvl_mla_decode_compressed_tree_batch_device(float *d_out, const float *d_x, const int *counts,
                                                    const int *parents, int batch, const KvlMlaConfig *cfg,
                                                    const KvlMlaBF16 *w, KvlMlaCompressedState *const *states,
@@ -307,7 +308,8 @@ int kvl_mla_compressed_q8_state_fork_batch_device(KvlMlaCompressedQ8State *const
  * become rows start + i and len becomes start + n (n = 0 drops the whole tree). path: strictly
  * increasing node indices, below 64 and below len - start; the nodes of a path from a child of the
  * history down, so that a row's rotation is that of its new place. On the device and in the host
- * arrays. Synchronous. */
+ * arrays (host rows that were never written, as after stream-ordered calls, are moved as they are).
+ * Synchronous. */
 int kvl_mla_compressed_state_accept(KvlMlaCompressedState *state, int start, const int *path, int n);
 int kvl_mla_compressed_bf16_state_accept(KvlMlaCompressedBF16State *state, int start, const int *path, int n);
 int kvl_mla_compressed_q8_state_accept(KvlMlaCompressedQ8State *state, int start, const int *path, int n);
