@@ -472,7 +472,7 @@ __global__ __launch_bounds__(128 * NM) __attribute__((amdgpu_waves_per_eu(2, 2))
     }
     constexpr int SR = Ch / 8;                      // softmax: rows of a thread,
     const int sq = tid >> 3, sr = SR * (tid & 7);  // its query and first row
-    float m_run = -1e30f, l_run = 0.f;  // (a maximum of -inf would make its own rows' weights NaN)
+    float m_run = -3e38f, l_run = 0.f;  // below any score but those at fp32's end (-inf would make its own rows' weights NaN)
     v4f acc[NM][NC];
 #pragma unroll
     for (int i = 0; i < NM; ++i)

@@ -236,36 +236,39 @@ def test_q8_rows_of_the_smallest_scales(models):  # noqa: F811
 
 
 @pytest.mark.parametrize("kind", KINDS)
-def test_logits_past_the_integers(models, kind):  # noqa: F811
-    """Logits of 2^24 to 2^30 (in steps of the reference's own rounding: 2 to 128), equal over the history's rows,
-    whose scale lies just below a power of two: the weights stay finite. Each head takes the history's row or the
-    best of the node's path; nodes whose heads do that by a margin of 2^-8 of the logit are compared."""
+@pytest.mark.parametrize("exponents,keys", [(range(18, 28), False), ((40, 47, 48, 49, 50, 51, 52, 55, 58), True)], ids=["past integers", "huge"])
+def test_large_logits(models, kind, exponents, keys):  # noqa: F811
+    """Logits of 2^21 to 2^30 (past 2^24 in steps of 2 to 128), and with keys as large as the queries up to 2^118, of
+    either sign, equal over the history's rows, whose scale lies just below a power of two: the weights stay finite.
+    Each head takes the history's row or the node's own; nodes whose heads do that by a margin of 2^-8 of the logit
+    are compared."""
     cfg, layer, w = models("kimi")
     ctx, n = 100, 24
     rng = np.random.default_rng(6)
     lat = rng.integers(-127, 128, cfg.kv_lora_rank).astype(np.float64)
     lat[0] = 127
+    key = rng.standard_normal(cfg.qk_rope_dim)
     st = State(kind, cfg, ctx + n)
-    put_rows(st, np.tile(lat, (ctx, 1)), np.zeros((ctx, cfg.qk_rope_dim)))
-    if kind == "q8":
-        st.arrays()[1][:ctx] = np.float32(2 - 2.0 ** -23)
-        lib.check(fn("compressed_%sstate_sync", kind)(st.ref()), "sync")
     compared = 0
-    for e in range(18, 28):
+    for e in exponents:
+        st.s.len = 0
+        put_rows(st, np.tile(lat, (ctx, 1)), np.tile(key * 2.0 ** e * keys, (ctx, 1)))
+        if kind == "q8":
+            st.arrays()[1][:ctx] = np.float32(2 - 2.0 ** -23)
+            lib.check(fn("compressed_%sstate_sync", kind)(st.ref()), "sync")
         x = (hidden(cfg, 0xE6, n) * np.float32(2.0 ** e)).astype(np.float32)
         p = [-1] * n
         got = tree_host(st, layer, x, p, w)
         assert np.isfinite(got).all(), e
         rows = st.rows(0, ctx + n)
         want = reference(cfg, layer, x, p, ctx, rows, kind)
-        hist, own = trees.values(rows, kind)[0][[0]], trees.values(rows, kind)[0][ctx:]
+        lats, ks = trees.values(rows, kind)
         q = latent_queries(cfg, layer, x)
-        a = np.matmul(q, hist.T)[:, :, 0]
-        b = np.stack([q[i] @ own[i] for i in range(n)]) + rope_scores(cfg, layer, x, trees.values(rows, kind)[1][ctx:], ctx)
+        a = np.matmul(q, lats[0]) + rope_scores(cfg, layer, x, np.tile(ks[:1], (n, 1)), ctx)
+        b = np.stack([q[i] @ lats[ctx + i] for i in range(n)]) + rope_scores(cfg, layer, x, ks[ctx:], ctx)
         for i in range(n):
             if (np.abs(a[i] - b[i]) > 2.0 ** -8 * np.abs(a[i]) + 64).all():
                 compared += 1
                 assert relative(got[i:i + 1], want[i:i + 1]) <= NEAR, (e, i)
-        lib.check(fn("compressed_%sstate_truncate", kind)(st.ref(), ctx), "truncate")
     assert compared > 20
     st.free()
